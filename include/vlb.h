@@ -338,6 +338,42 @@ int vlb_sgd_update_many(vlb_ctx* ctx, int count, vlb_param_update const* u, doub
 int vlb_solver_update_many(vlb_ctx* ctx, int solver, int count, vlb_param_update const* u, double gradMult,
                            vlb_solver_opts const* opts);
 
+/* ---- operators of language models' training steps; no counterparts among the reference's operator classes ---- */
+/* Layer normalisation over the channels of every position (h, w, n), as vlb_softmax_* and vlb_lrn_* treat positions; a sequence of tokens is a
+ * batch of 1 x 1 x C images.  With the mean m and the variance v of a position's C values and r = 1/sqrt(v + eps):
+ *   Y = g * (X - m) * r + b.
+ * g and b: C floats each.  The variance is the mean of the squared differences from m (two passes over the values, which are held on chip). */
+int vlb_lnorm_forward(vlb_ctx* ctx, float* Y, float const* X, float const* g, float const* b, int H, int W, int C, int N, double eps);
+/* With x^ = (X - m) * r and means over the channels of a position:  dX = r * (g*dY - mean(g*dY) - x^ * mean(g*dY*x^)),
+ * dG = sum over positions of dY * x^, dB = sum of dY.  m and r are computed from X.  dX, dG, dB are overwritten; any may be NULL.  The sums over
+ * positions are added in a fixed order. */
+int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float const* X, float const* g, float const* dY,
+                       int H, int W, int C, int N, double eps);
+
+/* A fully connected prediction layer over K classes and the softmax loss behind it, vlb_fc_forward followed by vlb_softmaxloss_forward, without the
+ * predictions in between: they are made in pieces of classes, in scratch, and never kept, so that K can be a vocabulary.  X: H x W x C x N,
+ * F: H x W x C x K, b: K floats or NULL, labels: one 1-based class label (as float) per image; label 0 skips the image and a label above K is
+ * skipped and reported, as vlb_softmaxloss_* do.  With z = F'x + b of an image:
+ *   lse = log(sum of exp(z)), 0 for an image that is skipped;  loss = (sum over the other images of lse - z[label]) / N.
+ * lse: N floats or NULL.  What X holds at skipped images, infinities and not-a-numbers included, reaches no result. */
+int vlb_fc_softmaxloss_forward(vlb_ctx* ctx, float* loss, float* lse, float const* X, float const* F, float const* b, float const* labels,
+                               int H, int W, int C, int N, int K);
+/* With dz = (exp(z - lse) - [class is the label]) * dzdy / N, 0 for skipped images:  dX = F dz, dF = sum of x dz', db = sum of dz.  dX, dF, db
+ * are overwritten; any may be NULL.  The predictions are made again, in pieces.  lse: what the forward pass gave, or NULL to have it computed. */
+int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, float const* X, float const* F, float const* b,
+                                float const* labels, float const* lse, double dzdy, int H, int W, int C, int N, int K);
+
+/* The Muon solver (Jordan and others, "Muon: an optimizer for hidden layers in neural networks", 2024) after the gradient exchange, beside
+ * vlb_solver_update_many.  A parameter is a matrix of `rows` rows of `cols` neighbouring floats: a filter bank FH x FW x FC x K has K rows.
+ *   g = gradMult*G + decay*W;  S1 = momentum*S1 + g;  u = nesterov ? g + momentum*S1 : S1;  X = u / (|u| + epsilon), |.| the Frobenius norm;
+ *   `steps` times:  A = X X',  X = a*X + (b*A + c*A*A) X     (rows > cols: A = X'X and products from the right, the same matrix);
+ *   W -= lr * sqrt(max(1, rows/cols)) * X.
+ * W and S1 (zero before the first step) are updated in place, G is only read.  All parameters go through every step together, in shared launches;
+ * the result is that of one after the other: an item whose tensors overlap an earlier one's begins a pass of its own. */
+typedef struct { double momentum, epsilon, a, b, c; int nesterov, steps; } vlb_muon_opts;
+typedef struct { float *W, *S1; float const* G; int rows, cols; double decay, lr; } vlb_muon_param;
+int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* opts);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,6 +51,18 @@ class ParamUpdate(C.Structure):
                                                                     ("t", C.c_longlong)]
 
 
+# the published coefficients and defaults of the Muon solver (not one of the reference's)
+MUON_DEFAULTS = dict(momentum=0.95, nesterov=True, steps=5, a=3.4445, b=-4.7750, c=2.0315, epsilon=1e-7)
+
+
+class MuonOpts(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("momentum", "epsilon", "a", "b", "c")] + [("nesterov", C.c_int), ("steps", C.c_int)]
+
+
+class MuonParam(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("W", "S1", "G")] + [("rows", C.c_int), ("cols", C.c_int), ("decay", C.c_double), ("lr", C.c_double)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _D = C.c_double
@@ -122,6 +134,11 @@ SIGNATURES = {
     "vlb_mul": (_I, [_P, _P, _P, _P, _Z]),
     "vlb_sgd_update_many": (_I, [_P, _I, C.POINTER(ParamUpdate), _D, _D, _I]),
     "vlb_solver_update_many": (_I, [_P, _I, _I, C.POINTER(ParamUpdate), _D, C.POINTER(SolverOpts)]),
+    "vlb_lnorm_forward": (_I, [_P] * 5 + [_I] * 4 + [_D]),
+    "vlb_lnorm_backward": (_I, [_P] * 7 + [_I] * 4 + [_D]),
+    "vlb_fc_softmaxloss_forward": (_I, [_P] * 7 + [_I] * 5),
+    "vlb_fc_softmaxloss_backward": (_I, [_P] * 9 + [_D] + [_I] * 5),
+    "vlb_muon_update_many": (_I, [_P, _I, C.POINTER(MuonParam), _D, C.POINTER(MuonOpts)]),
     "vlb_solver_update": (_I, [_P, _I, _P, _P, _P, _P, _Z, _D, _D, _D, C.POINTER(SolverOpts), C.c_longlong]),
 }
 

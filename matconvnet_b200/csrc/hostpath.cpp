@@ -8,6 +8,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -623,6 +624,126 @@ PyObject* softmaxloss(PyObject*, Args a, Py_ssize_t n)
   });
 }
 
+// The operators below launch on the current device's stream: refuses tensors of any other.
+void on_device_of(at::Tensor const& x, std::initializer_list<at::Tensor const*> others)
+{
+  for (at::Tensor const* t : others)
+    if (t->defined() && t->device() != x.device()) fail(PyExc_ValueError, "all tensors must be on the device of X.");
+  if (x.device().index() != c10::cuda::current_device()) fail(PyExc_ValueError, "X must be on the current CUDA device.");
+}
+
+// ---------------------------------------------------------------- vl_nnlayernorm: ctx, x, g, b, dzdy, epsilon, der_out
+PyObject* lnorm(PyObject*, Args a, Py_ssize_t n)
+{
+  return guarded(n, 7, [&]() -> PyObject* {
+    Ctx ctx(a[0]);
+    at::Tensor x = need_one(a[1], "x"), g = need_one(a[2], "g"), b = need_one(a[3], "b"), dzdy = need(a[4], "dzdy");
+    on_device_of(x, {&g, &b, &dzdy});
+    Shape const s = shape4(x);
+    int const H = (int)s.d[0], W = (int)s.d[1], C = (int)s.d[2], N = (int)s.d[3];
+    double const eps = as_double(a[5]);
+    if (g.numel() != C) fail(PyExc_ValueError, "The number of elements of G is not the same as the depth of X.");
+    if (b.numel() != C) fail(PyExc_ValueError, "The number of elements of B is not the same as the depth of X.");
+    if (!dzdy.defined()) {
+      at::Tensor y;
+      ctx.run([&] {
+        y = empty_cm(x.sizes(), x.device());
+        return vlb_lnorm_forward(ctx.h, ptr(y), ptr(x), ptr(g), ptr(b), H, W, C, N, eps);
+      });
+      return wrap(y);
+    }
+    if (!same4(shape4(dzdy), H, W, C, N)) fail(PyExc_ValueError, "DZDY dimensions are incompatible with X.");
+    PyRef held;
+    Pair const given = two_items(a[6], held);
+    int64_t const sc[2] = {C, 1};
+    at::Tensor dx, dg = der_out(given.first, at::IntArrayRef(sc, 2), "DG"), db = der_out(given.second, at::IntArrayRef(sc, 2), "DB");
+    ctx.run([&] {
+      dx = empty_cm(x.sizes(), x.device());
+      if (!dg.defined()) dg = empty_cm(C, 1, x.device());
+      if (!db.defined()) db = empty_cm(C, 1, x.device());
+      return vlb_lnorm_backward(ctx.h, ptr(dx), ptr(dg), ptr(db), ptr(x), ptr(g), ptr(dzdy), H, W, C, N, eps);
+    });
+    return tuple_of({dx, dg, db});
+  });
+}
+
+// ---------------------------------------------------------------- vl_nnfcsoftmaxloss
+// ctx, x, f, b, c, dzdy (None or a number), lse, no_der_data, no_der_filters, no_der_biases, der_out
+PyObject* fcsoftmaxloss(PyObject*, Args a, Py_ssize_t n)
+{
+  return guarded(n, 11, [&]() -> PyObject* {
+    Ctx ctx(a[0]);
+    at::Tensor x = need_one(a[1], "x"), f = need_one(a[2], "f"), b = need(a[3], "b"), c = need_one(a[4], "c"), lse = need(a[6], "lse");
+    on_device_of(x, {&f, &b, &c, &lse});
+    Shape const s = shape4(x), sf = shape4(f);
+    int const H = (int)s.d[0], W = (int)s.d[1], C = (int)s.d[2], N = (int)s.d[3], K = (int)sf.d[3];
+    if (sf.d[0] != H || sf.d[1] != W || sf.d[2] != C) fail(PyExc_ValueError, "The FILTERS must be as large as the images of X.");
+    if (b.defined() && b.numel() != K) fail(PyExc_ValueError, "The number of elements of BIASES is not the same as the number of filters.");
+    if (c.numel() != N) fail(PyExc_ValueError, "one label per image expected");
+    if (lse.defined() && lse.numel() != N) fail(PyExc_ValueError, "one LSE per image expected");
+    if (a[5] == Py_None) {
+      at::Tensor loss, out;
+      ctx.run([&] {
+        loss = at::empty({1}, x.options());
+        out = at::empty({N}, x.options());
+        return vlb_fc_softmaxloss_forward(ctx.h, ptr(loss), ptr(out), ptr(x), ptr(f), ptr(b), ptr(c), H, W, C, N, K);
+      });
+      return tuple_of({loss, out});
+    }
+    double const dzdy = as_double(a[5]);
+    PyRef held;
+    Pair const given = two_items(a[10], held);
+    bool const wantX = !as_bool(a[7]), wantF = !as_bool(a[8]), wantB = !as_bool(a[9]) && b.defined();
+    int64_t const sb[2] = {K, 1};
+    at::Tensor dx, df, db;
+    if (wantF) df = der_out(given.first, at::IntArrayRef(sf.d, 4), "DF");
+    if (wantB) db = der_out(given.second, at::IntArrayRef(sb, 2), "DB");
+    ctx.run([&] {
+      if (wantX) dx = empty4(s, x.device());
+      if (wantF && !df.defined()) df = empty_cm(at::IntArrayRef(sf.d, 4), x.device());
+      if (wantB && !db.defined()) db = empty_cm(K, 1, x.device());
+      return vlb_fc_softmaxloss_backward(ctx.h, ptr(dx), ptr(df), ptr(db), ptr(x), ptr(f), ptr(b), ptr(c), ptr(lse), dzdy, H, W, C, N, K);
+    });
+    return tuple_of({dx, df, db});
+  });
+}
+
+// ---------------------------------------------------------------- the Muon solver
+// ctx, [(w, s1, g, decay, lr)], grad_mult, (momentum, epsilon, a, b, c, nesterov, steps)
+PyObject* muon(PyObject*, Args a, Py_ssize_t n)
+{
+  return guarded(n, 4, [&]() -> PyObject* {
+    Ctx ctx(a[0]);
+    if (!PyList_CheckExact(a[1]) || !PyTuple_CheckExact(a[3]) || PyTuple_GET_SIZE(a[3]) != 7) fail(PyExc_TypeError, "a list of updates and seven options expected");
+    Py_ssize_t const count = PyList_GET_SIZE(a[1]);
+    std::vector<vlb_muon_param> u((size_t)count);
+    std::vector<at::Tensor> held;
+    held.reserve(3 * (size_t)count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      PyObject* t = PyList_GET_ITEM(a[1], i);
+      if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 5) fail(PyExc_TypeError, "an update is a tuple of five");
+      at::Tensor const w = flat32(PyTuple_GET_ITEM(t, 0), "w"), s1 = flat32(PyTuple_GET_ITEM(t, 1), "momentum_state"), g = need_one(PyTuple_GET_ITEM(t, 2), "grad");
+      if (w.numel() != g.numel() || w.numel() != s1.numel()) fail(PyExc_ValueError, "parameter, momentum and gradient do not have the same number of elements.");
+      if (!column_major(w) || !column_major(s1)) fail(PyExc_ValueError, "parameter and momentum must be column-major tensors of one shape.");
+      on_device_of(w, {&s1, &g});
+      Shape const s = shape4(w);
+      int64_t const cols = s.d[0] * s.d[1] * s.d[2];
+      if (cols > INT32_MAX || s.d[3] > INT32_MAX) fail(PyExc_ValueError, "the parameter is too large.");
+      vlb_muon_param& p = u[(size_t)i];
+      p.W = ptr(w); p.S1 = ptr(s1); p.G = ptr(g); p.rows = (int)s.d[3]; p.cols = (int)cols;
+      held.insert(held.end(), {w, s1, g});
+      p.decay = as_double(PyTuple_GET_ITEM(t, 3)); p.lr = as_double(PyTuple_GET_ITEM(t, 4));
+    }
+    vlb_muon_opts o = {};
+    o.momentum = as_double(PyTuple_GET_ITEM(a[3], 0)); o.epsilon = as_double(PyTuple_GET_ITEM(a[3], 1));
+    o.a = as_double(PyTuple_GET_ITEM(a[3], 2)); o.b = as_double(PyTuple_GET_ITEM(a[3], 3)); o.c = as_double(PyTuple_GET_ITEM(a[3], 4));
+    o.nesterov = as_bool(PyTuple_GET_ITEM(a[3], 5)) ? 1 : 0; o.steps = as_int(PyTuple_GET_ITEM(a[3], 6));
+    double const gm = as_double(a[2]);
+    ctx.run([&] { return vlb_muon_update_many(ctx.h, (int)count, u.data(), gm, &o); });
+    Py_RETURN_NONE;
+  });
+}
+
 // ---------------------------------------------------------------- vl_taccum: ctx, alpha, a, beta, b, out
 PyObject* taccum(PyObject*, Args a, Py_ssize_t n)
 {
@@ -694,6 +815,7 @@ PyObject* setup(PyObject*, Args a, Py_ssize_t n)      // nn._pair, nn._quad, cap
 #define VLB_FN(name) {#name, (PyCFunction)(void*)name, METH_FASTCALL, nullptr}
 PyMethodDef gMethods[] = {VLB_FN(setup), VLB_FN(conv), VLB_FN(convt), VLB_FN(bnorm), VLB_FN(pool), VLB_FN(roipool), VLB_FN(sampler), VLB_FN(relu),
                           VLB_FN(normalize), VLB_FN(softmax), VLB_FN(dropout), VLB_FN(softmaxloss), VLB_FN(taccum), VLB_FN(update),
+                          VLB_FN(lnorm), VLB_FN(fcsoftmaxloss), VLB_FN(muon),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef gModule = {PyModuleDef_HEAD_INIT, "_hostpath", "Native host side of matconvnet_b200.nn", -1, gMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -100,6 +100,15 @@ def vl_nnbnorm(x, g, b, dzdy=None, epsilon=1e-4, moments=None, der_out=None, rel
     return _hostpath.bnorm(ctx or default_context(), x, g, b, dzdy, epsilon, moments, der_out, relu)
 
 
+# --------------------------------------------------------------------- vl_nnlayernorm
+def vl_nnlayernorm(x, g, b, dzdy=None, epsilon=1e-5, der_out=None, ctx=None):
+    """Y = VL_NNLAYERNORM(X, G, B) / [DX, DG, DB] = VL_NNLAYERNORM(X, G, B, DZDY): normalises the channels of every position
+    (h, w, n) to mean 0 and variance 1, then scales them by G and shifts them by B, C elements each.  No counterpart in the
+    reference; the signature is vl_nnbnorm's.  A sequence of tokens is a batch of 1 x 1 x C images.  The backward pass computes
+    mean and variance from X again.  der_out=(DG, DB) as in vl_nnconv."""
+    return _hostpath.lnorm(ctx or default_context(), x, g, b, dzdy, epsilon, der_out)
+
+
 # --------------------------------------------------------------------- vl_nnpool
 def vl_nnpool(x, pool, dzdy=None, stride=1, pad=0, method="max", through_relu=False, ctx=None):
     """Y = VL_NNPOOL(X, POOL) / DX = VL_NNPOOL(X, POOL, DZDY) (matlab/vl_nnpool.m; gateway
@@ -195,7 +204,11 @@ def solver_update_(solver, w, state, grad, grad_mult, decay, lr, opts=None, ctx=
 
 
 def solver_update_many_(solver, updates, grad_mult, opts=None, ctx=None):
-    """solver_update_ on several parameter tensors in one launch; updates: [(w, state, grad, decay, lr)]."""
+    """solver_update_ on several parameter tensors in one launch; updates: [(w, state, grad, decay, lr)].  The solver 'muon' (not
+    one of the reference's; include/vlb.h has its formula) takes filter banks FH x FW x FC x K, matrices of K rows; its state is
+    the momentum tensor and the step count, and it updates all of them together in a few launches."""
+    if solver == "muon":
+        return _muon_update_many(updates, grad_mult, opts, ctx)
     if solver not in capi.SOLVERS:
         raise ValueError("unknown solver '%s'" % solver)
     o = dict(capi.SOLVER_DEFAULTS[solver])
@@ -217,6 +230,28 @@ def solver_update_many_(solver, updates, grad_mult, opts=None, ctx=None):
         items.append((w, state["s1"], state["s2"] if two else None, g, decay, lr, state["t"]))
     _hostpath.update(ctx or default_context(), capi.SOLVERS[solver], items, grad_mult, 0.0, False,
                      (o.get("rho", 0.0), o["epsilon"], o.get("beta1", 0.0), o.get("beta2", 0.0)))
+
+
+def _muon_update_many(updates, grad_mult, opts, ctx):
+    o = dict(capi.MUON_DEFAULTS)
+    o.update(opts or {})
+    for w, state, g, _, _ in updates:         # a refused list leaves every state and step count as it was
+        if not all(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.float32 for t in (w, g)):
+            raise TypeError("w and grad must be CUDA float32 tensors")
+        if w.numel() != g.numel():
+            raise ValueError("parameter and gradient do not have the same number of elements.")
+        if not mat.is_mat(w) or ("s1" in state and (state["s1"].shape != w.shape or not mat.is_mat(state["s1"]))):
+            raise ValueError("parameter and momentum must be column-major tensors of one shape.")
+        if g.shape != w.shape:
+            raise ValueError("parameter and gradient must have the same shape.")
+    if int(o["steps"]) < 0 or not o["epsilon"] >= 0:
+        raise ValueError("steps and epsilon must not be negative.")
+    items = [(w, state["s1"] if "s1" in state else torch.zeros_like(w), g, decay, lr) for w, state, g, decay, lr in updates]
+    _hostpath.muon(ctx or default_context(), items, grad_mult,
+                   (o["momentum"], o["epsilon"], o["a"], o["b"], o["c"], bool(o["nesterov"]), int(o["steps"])))
+    for (_, state, _, _, _), item in zip(updates, items):
+        state["s1"] = item[1]
+        state["t"] = state.get("t", 0) + 1
 
 
 # --------------------------------------------------------------------- MATLAB-only blocks
@@ -254,3 +289,14 @@ def vl_nndropout(x, dzdy=None, rate=0.5, mask=None, seed=0, ctx=None):
 def vl_nnsoftmaxloss(x, c, dzdy=None, ctx=None):
     """matlab/vl_nnsoftmaxloss.m:56-84 with one class label (1-based) per image."""
     return _hostpath.softmaxloss(ctx or default_context(), x, c, dzdy)
+
+
+def vl_nnfcsoftmaxloss(x, f, b, c, dzdy=None, lse=None, no_der_data=False, no_der_filters=False, no_der_biases=False, der_out=None,
+                       ctx=None):
+    """[LOSS, LSE] = VL_NNFCSOFTMAXLOSS(X, F, B, C) / [DX, DF, DB] = VL_NNFCSOFTMAXLOSS(X, F, B, C, DZDY, 'lse', LSE): a fully
+    connected layer whose outputs are the predictions of K classes and the softmax loss behind it,
+    vl_nnsoftmaxloss(vl_nnconv(X, F, B), C), without the predictions: they are made in pieces and never kept, so that K can be a
+    vocabulary.  F is H x W x C x K, as large as X's images; B may be None; C holds one label (1-based, 0 skips the image) per
+    image.  LSE, the logarithm of the sum of exponentials of an image's predictions (0 where the image is skipped), spares the
+    backward pass a pass over F; without it the backward pass computes it.  The flags and der_out=(DF, DB) as in vl_nnconv."""
+    return _hostpath.fcsoftmaxloss(ctx or default_context(), x, f, b, c, dzdy, lse, no_der_data, no_der_filters, no_der_biases, der_out)

@@ -5,6 +5,9 @@ A network is ``{'layers': [layer, ...]}`` with layers shaped like the reference'
   {'type': 'relu'}   {'type': 'pool', 'method': 'max'|'avg', 'pool': [ph pw], 'stride': s, 'pad': p}
   {'type': 'bnorm', 'weights': [g, b, moments], 'epsilon': e}   {'type': 'softmaxloss', 'class': c}
   {'type': 'normalize', 'param': [N kappa alpha beta]}   {'type': 'softmax'}
+  {'type': 'layernorm', 'weights': [g, b], 'epsilon': e}
+  {'type': 'fcsoftmaxloss', 'weights': [f, b], 'class': c}  (a fully connected layer and the softmax loss behind it, its predictions
+  never stored; the images' log-sum-exp are kept in res[i]['aux'] for the backward pass)
   {'type': 'dropout', 'rate': r}  (training mode: a new mask per forward pass, kept in res[i]['aux'] for the backward pass)
 ``vl_simplenn(net, x, dzdy)`` runs the forward pass storing every intermediate (res[i]['x'],
 vl_simplenn.m:294-398) and, when dzdy is given, the backward pass in reverse order
@@ -25,12 +28,12 @@ def grad_name(i, j):
 
 
 def gradient_specs(net):
-    """[(name, MATLAB shape)] of the parameter derivatives of conv and bnorm layers in the order the backward pass
+    """[(name, MATLAB shape)] of the parameter derivatives of layers with weights in the order the backward pass
     produces them (last layer first, filters before biases): the input of GradientExchange.plan."""
     specs = []
     for i in range(len(net["layers"]) - 1, -1, -1):
         l = net["layers"][i]
-        if l["type"] in ("conv", "bnorm"):
+        if l["type"] in ("conv", "bnorm", "layernorm", "fcsoftmaxloss"):
             for j, w in enumerate(l["weights"][:2]):
                 if w is not None:
                     specs.append((grad_name(i, j), tuple(int(v) for v in w.shape)))
@@ -81,8 +84,12 @@ def vl_simplenn(net, x, dzdy=None, res=None, on_dzdw=None, ctx=None, skip_forwar
                     res[i + 1]["x"], res[i + 2]["x"] = None, y
                 else:
                     res[i + 1]["x"] = y
+            elif t == "layernorm":
+                res[i + 1]["x"] = nn.vl_nnlayernorm(xi, l["weights"][0], l["weights"][1], epsilon=_get(l, "epsilon", 1e-5), ctx=ctx)
             elif t == "softmaxloss":
                 res[i + 1]["x"] = nn.vl_nnsoftmaxloss(xi, l["class"], ctx=ctx)
+            elif t == "fcsoftmaxloss":
+                res[i + 1]["x"], res[i]["aux"] = nn.vl_nnfcsoftmaxloss(xi, l["weights"][0], l["weights"][1], l["class"], ctx=ctx)
             elif t == "normalize":
                 res[i + 1]["x"] = nn.vl_nnnormalize(xi, l["param"], ctx=ctx)
             elif t == "softmax":
@@ -128,8 +135,16 @@ def vl_simplenn(net, x, dzdy=None, res=None, on_dzdw=None, ctx=None, skip_forwar
             dx, dg, db, mom = nn.vl_nnbnorm(xi, l["weights"][0], l["weights"][1], d, epsilon=_get(l, "epsilon", 1e-4),
                                             der_out=(grad_out.get((i, 0)), grad_out.get((i, 1))), ctx=ctx)
             res[i]["dzdx"], res[i]["dzdw"] = dx, [dg, db, mom]
+        elif t == "layernorm":
+            dx, dg, db = nn.vl_nnlayernorm(xi, l["weights"][0], l["weights"][1], d, epsilon=_get(l, "epsilon", 1e-5),
+                                           der_out=(grad_out.get((i, 0)), grad_out.get((i, 1))), ctx=ctx)
+            res[i]["dzdx"], res[i]["dzdw"] = dx, [dg, db]
         elif t == "softmaxloss":
             res[i]["dzdx"] = nn.vl_nnsoftmaxloss(xi, l["class"], d, ctx=ctx)
+        elif t == "fcsoftmaxloss":
+            dx, df, db = nn.vl_nnfcsoftmaxloss(xi, l["weights"][0], l["weights"][1], l["class"], d, lse=res[i]["aux"],
+                                               der_out=(grad_out.get((i, 0)), grad_out.get((i, 1))), ctx=ctx)
+            res[i]["dzdx"], res[i]["dzdw"] = dx, [df, db]
         elif t == "normalize":
             dx = nn.vl_nnnormalize(xi, l["param"], d, ctx=ctx, through_relu=through)
             res[i]["dzdx"], res[i - 1 if through else i]["dzdx"] = None, dx

@@ -5,7 +5,8 @@ moments), move the stored moments towards the batch's (cnn_train.m:468-476).
 
 ``params``: dict with learning_rate, weight_decay, momentum, nesterov_update (cnn_train.m:17-45 defaults: 0.001, 0.0005,
 0.9, False) and optionally solver ('adagrad', 'adadelta', 'adam' or 'rmsprop': examples/+solver/*.m, called at
-cnn_train.m:503-507 instead of the momentum step) with solver_opts (the solver's own defaults otherwise).  A layer may carry 'learningRate' / 'weightDecay' lists (per parameter multipliers, default 1;
+cnn_train.m:503-507 instead of the momentum step) with solver_opts (the solver's own defaults otherwise).  The solver 'muon'
+takes the filter banks of conv and fcsoftmaxloss layers; biases and multipliers, which are no matrices, take the momentum step beside it.  A layer may carry 'learningRate' / 'weightDecay' lists (per parameter multipliers, default 1;
 vl_simplenn_tidy).  ``state`` maps (layer index, parameter index) to the momentum tensor, created as zeros on first use
 (cnn_train.m:292-301).  Every tensor operation is a call into the C ABI.
 """
@@ -25,7 +26,7 @@ def accumulate_gradients(net, res, state, params, num_workers=1, pulled=None, ct
     num_workers (cnn_train.m:455,482), so an exchange built with average=True must not be combined with num_workers > 1."""
     layers = net["layers"]
     solver, base_lr, base_wd = params.get("solver"), params["learning_rate"], params["weight_decay"]
-    updates = []                      # all parameter tensors of the network are updated by one launch
+    updates, plain = [], []           # all parameter tensors of the network are updated by one launch (muon: by a few)
     for l in range(len(layers) - 1, -1, -1):
         dzdw = res[l]["dzdw"]
         if dzdw is None:
@@ -46,11 +47,12 @@ def accumulate_gradients(net, res, state, params, num_workers=1, pulled=None, ct
             lr = base_lr * lr_mult
             if lr > 0 or decay > 0:
                 key = (l, j)
+                momentum_step = not solver or (solver == "muon" and (j > 0 or layer["type"] not in ("conv", "fcsoftmaxloss")))
                 if key not in state:
-                    state[key] = {} if solver else torch.zeros_like(w)
-                updates.append((w, state[key], der, decay, lr))
-    if updates and solver:
+                    state[key] = torch.zeros_like(w) if momentum_step else {}
+                (plain if momentum_step else updates).append((w, state[key], der, decay, lr))
+    if updates:
         nn.solver_update_many_(solver, updates, 1.0 / num_workers, params.get("solver_opts"), ctx)
-    elif updates:
-        nn.sgd_update_many_(updates, 1.0 / num_workers, params["momentum"], params.get("nesterov_update", False), ctx)
+    if plain:
+        nn.sgd_update_many_(plain, 1.0 / num_workers, params["momentum"], params.get("nesterov_update", False), ctx)
     return state
