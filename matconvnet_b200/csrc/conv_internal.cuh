@@ -56,5 +56,6 @@ int conv_wgrad_half(vlb_ctx* ctx, ConvGeom const& g, float* dF, float* db, float
 int fc_dgrad_half(vlb_ctx* ctx, ConvGeom const& g, float* dX, float const* F, float const* dY);
 int fc_wgrad_half(vlb_ctx* ctx, ConvGeom const& g, float* dF, float const* X, float const* dY);
 cudaError_t half_set_wait_limit(long long cycles, cudaStream_t stream);
+cudaError_t pairs_set_wait_limit(long long cycles, cudaStream_t stream);
 
 }  // namespace vlb

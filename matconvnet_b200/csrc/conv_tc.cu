@@ -2344,6 +2344,7 @@ extern "C" int vlb_ctx_set_wait_limit(vlb_ctx* ctx, long long cycles)
   // ordered behind the kernels already enqueued on the context's stream, which keep the limit they were launched under
   cudaError_t e = cudaMemcpyToSymbolAsync(gWaitCycles, &v, sizeof(v), 0, cudaMemcpyHostToDevice, ctx->stream);
   if (e == cudaSuccess) e = vlb::half_set_wait_limit(cycles, ctx->stream);
+  if (e == cudaSuccess) e = vlb::pairs_set_wait_limit(cycles, ctx->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) { cudaGetLastError(); return vlb::set_error(ctx, VLB_Cuda, cudaGetErrorString(e)); }
   return VLB_Success;

@@ -1,10 +1,10 @@
 // A fully connected prediction layer and the softmax loss behind it, in pieces of classes (include/vlb.h has the formulas).
+#include "pairs.cuh"
 #include "products.cuh"
 #include <algorithm>
 
 namespace {
 
-using vlb::Operand;
 
 constexpr int kThreads = 256;
 
@@ -114,6 +114,235 @@ __global__ void db_kernel(float* __restrict__ db, float const* __restrict__ dz, 
   db[c] = s;
 }
 
+// ------------------------------------------------------------------ on pairs of halves (pairs.cu)
+struct Part { float top, sum; };
+
+__device__ __forceinline__ Part together(Part a, Part b)
+{
+  float const top = fmaxf(a.top, b.top);
+  return {top, a.sum * exp_below(a.top, top) + b.sum * exp_below(b.top, top)};
+}
+
+// lse of 32 images per block from the parts of their predictions, and the loss by the block that is through last, which adds the blocks' sums in their order.
+// lse and labels: of the images first ... first + rows - 1; sums: one per block of 32 images of all `blocks`.
+__global__ void __launch_bounds__(1024)
+lse_kernel(float* __restrict__ loss, float* __restrict__ lse, float2 const* __restrict__ parts, int count, float const* __restrict__ label,
+           float const* __restrict__ labels, int rows, int first, int N, int K, double* sums, int blocks, int* ticket, int* status)
+{
+  vlb::pdl_wait();
+  __shared__ Part all[32][33];
+  int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, row = (int)blockIdx.x * 32 + tx;
+  Part p = {-INFINITY, 0.f};
+  if (row < rows)
+#pragma unroll 4
+    for (int i = ty; i < count; i += 32) {
+      float2 const v = parts[(long long)i * rows + row];
+      p = together(p, {v.x, v.y});
+    }
+  all[ty][tx] = p;
+  __syncthreads();
+  if (ty) return;
+  for (int i = 1; i < 32; ++i) p = together(p, all[i][tx]);
+  double term = 0;
+  if (row < rows) {
+    Label const l = label_of(labels, row, K, status);
+    float v = 0.f;
+    if (l.real) { v = p.top + logf(p.sum); term = (double)v - label[row]; }
+    if (lse) lse[row] = v;
+  }
+  for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
+  if (!loss) return;
+  bool mine = false;
+  if (tx == 0) {
+    sums[first / 32 + blockIdx.x] = term;
+    __threadfence();
+    mine = atomicAdd(ticket, 1) == blocks - 1;
+    __threadfence();
+  }
+  if (!__shfl_sync(0xffffffffu, (int)mine, 0)) return;
+  double sum = 0;
+  for (int i = tx; i < blocks; i += 32) sum += __ldcg(sums + i);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (tx == 0) { *loss = (float)(sum / N); *ticket = 0; }
+}
+
+// db[c] (+)= scale * sum of the rows of parts.
+__global__ void db_parts_kernel(float* __restrict__ db, float const* __restrict__ parts, long long ld, int cols, int rows, float scale, bool add)
+{
+  vlb::pdl_wait();
+  int const c = blockIdx.x * kThreads + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) s += parts[r * ld + c];
+  db[c] = add ? db[c] + s * scale : s * scale;
+}
+
+constexpr int kMostImages = 16384;          // images at a time
+constexpr int kDzExp = 14;                  // derivatives of the predictions, at most 1 in magnitude, times 2^14
+constexpr size_t kMostScratch = 1u << 30;   // what the pieces of classes may take
+
+// The call's scratch, cut up.
+struct Plan {
+  int images, piece;                        // images at a time, classes at a time
+  size_t bytes;
+  unsigned* largest;                        // of X, of the piece of F
+  char *x, *f, *dz, *split;
+  float2* parts; float *label, *lse, *db;
+  double* sums;
+
+  Plan(int N, int D, int K, bool back, size_t scratch, char* at = nullptr)
+  {
+    images = std::min(N, kMostImages);
+    size_t const perClass = 4 * (size_t)vlb::pair_ld(D) + (back ? 4 * (size_t)images + (size_t)images / 8 + 64 : 0);
+    long long const most = std::max<long long>(256, (long long)(scratch / perClass) / 256 * 256);
+    int const pieces = vlb::ceil_div(K, most);
+    piece = (int)std::min<long long>(K, vlb::ceil_div(vlb::ceil_div(K, pieces), 256) * 256ll);
+    bytes = 0;
+    auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
+    largest = (unsigned*)take(256);
+    x = take(vlb::pair_bytes(images, D));
+    f = take(vlb::pair_bytes(piece, D));
+    split = take(vlb::kPairSplitBytes);
+    parts = (float2*)take(sizeof(float2) * (size_t)images * vlb::pair_parts(piece) * pieces);
+    label = (float*)take(sizeof(float) * (size_t)images);
+    lse = (float*)take(sizeof(float) * (size_t)images);
+    sums = (double*)take(sizeof(double) * (size_t)vlb::ceil_div(N, 32));
+    dz = back ? take(vlb::pair_bytes(images, piece)) : nullptr;
+    db = back ? (float*)take(sizeof(float) * (size_t)vlb::ceil_div(images, 32) * vlb::pair_ld(piece)) : nullptr;
+  }
+};
+
+// A plan whose scratch there is: smaller pieces where there is less.
+bool plan_for(vlb_ctx* ctx, Plan& plan, int N, int D, int K, bool back)
+{
+  for (size_t scratch = kMostScratch; scratch >= (16u << 20); scratch /= 4) {
+    plan = Plan(N, D, K, back, scratch);
+    void* const p = scratch / 4 >= (16u << 20) ? vlb::try_workspace(ctx, plan.bytes) : vlb::workspace(ctx, plan.bytes);
+    if (p) { plan = Plan(N, D, K, back, scratch, (char*)p); return true; }
+  }
+  return false;
+}
+
+struct Problem {
+  vlb_ctx* ctx;
+  float const *X, *F, *b, *labels;
+  int N, D, K;
+};
+
+// The pair of a piece of F.
+vlb::Pair filters(Problem const& q, Plan const& plan, int k0, int cols)
+{
+  float const* const f = q.F + (size_t)k0 * q.D;
+  vlb::Pair const to = vlb::pair_at(plan.f, cols, q.D);
+  cudaMemsetAsync(plan.largest + 1, 0, sizeof(unsigned), q.ctx->stream);
+  vlb::largest_of(q.ctx, plan.largest + 1, f, cols, q.D, nullptr, 0);
+  vlb::make_pair(q.ctx, to, f, plan.largest + 1, nullptr, 0);
+  return to;
+}
+
+vlb::Pair images(Problem const& q, Plan const& plan, int n0, int rows)
+{
+  float const* const x = q.X + (size_t)n0 * q.D;
+  vlb::Pair const to = vlb::pair_at(plan.x, rows, q.D);
+  cudaMemsetAsync(plan.largest, 0, sizeof(unsigned), q.ctx->stream);
+  vlb::largest_of(q.ctx, plan.largest, x, rows, q.D, q.labels + n0, q.K);
+  vlb::make_pair(q.ctx, to, x, plan.largest, q.labels + n0, q.K);
+  return to;
+}
+
+vlb::PairProduct predictions(Problem const& q, Plan const& plan, vlb::Pair x, vlb::Pair f, int n0, int k0)
+{
+  vlb::PairProduct p = {};
+  p.a = {x, false}; p.b = {f, false};
+  p.M = x.rows; p.N = f.rows; p.K = q.D;
+  p.e.ea.largest = plan.largest; p.e.eb.largest = plan.largest + 1;
+  p.e.bias = q.b ? q.b + k0 : nullptr;
+  p.e.labels = q.labels + n0;
+  p.e.firstClass = k0; p.e.classes = q.K;
+  return p;
+}
+
+// lse of images n0 ... and, after the last of them, the loss (either may be null).
+int seen(Problem const& q, Plan const& plan, vlb::Pair x, int n0, float* lse, float* loss, int* status)
+{
+  int count = 0;
+  for (int k0 = 0; k0 < q.K; k0 += plan.piece) {
+    vlb::Pair const f = filters(q, plan, k0, std::min(plan.piece, q.K - k0));
+    vlb::PairProduct p = predictions(q, plan, x, f, n0, k0);
+    p.e.parts = plan.parts + (size_t)count * x.rows; p.e.label = plan.label;
+    int n = 0;
+    if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairSeen, &p, 1, plan.split, &n)) return rc;
+    count += n;
+  }
+  vlb::launch(q.ctx->stream, lse_kernel, (unsigned)vlb::ceil_div(x.rows, 32), 1024, 0, loss, lse, plan.parts, count, plan.label, q.labels + n0, x.rows, n0,
+              q.N, q.K, plan.sums, vlb::ceil_div(q.N, 32), q.ctx->deviceStatus + 64 + 4095, status);
+  VLB_LAUNCHED(q.ctx, 1);
+  return VLB_Success;
+}
+
+int forward_on_pairs(Problem const& q, float* loss, float* lse)
+{
+  Plan plan(1, 1, 1, false, 0);
+  if (!plan_for(q.ctx, plan, q.N, q.D, q.K, false)) return q.ctx->lastError;
+  vlb::ProfScope prof(q.ctx, vlb::kProfFc);
+  prof.rec.flops = 2.0 * q.N * q.D * q.K;
+  for (int n0 = 0; n0 < q.N; n0 += plan.images) {
+    vlb::Pair const x = images(q, plan, n0, std::min(plan.images, q.N - n0));
+    if (int const rc = seen(q, plan, x, n0, lse ? lse + n0 : nullptr, loss, q.ctx->deviceStatus)) return rc;
+  }
+  return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_forward");
+}
+
+int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float const* lse, float scale)
+{
+  Plan plan(1, 1, 1, true, 0);
+  if (!plan_for(q.ctx, plan, q.N, q.D, q.K, true)) return q.ctx->lastError;
+  vlb::ProfScope prof(q.ctx, vlb::kProfFc);
+  prof.rec.flops = 2.0 * q.N * q.D * q.K * ((dX ? 1 : 0) + (dF ? 1 : 0) + (lse ? 1 : 2));
+  for (int n0 = 0; n0 < q.N; n0 += plan.images) {
+    vlb::Pair const x = images(q, plan, n0, std::min(plan.images, q.N - n0));
+    if (!lse)
+      if (int const rc = seen(q, plan, x, n0, plan.lse, nullptr, nullptr)) return rc;
+    for (int k0 = 0; k0 < q.K; k0 += plan.piece) {
+      int const cols = std::min(plan.piece, q.K - k0);
+      vlb::Pair const f = filters(q, plan, k0, cols), dz = vlb::pair_at(plan.dz, x.rows, cols);
+      vlb::PairProduct p = predictions(q, plan, x, f, n0, k0);
+      p.e.lse = lse ? lse + n0 : plan.lse;
+      p.e.to = dz; p.e.toExp = kDzExp; p.e.db = db ? plan.db : nullptr;
+      p.e.status = q.ctx->deviceStatus;
+      if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairGrad, &p, 1, plan.split)) return rc;
+      if (db) {
+        vlb::launch(q.ctx->stream, db_parts_kernel, (unsigned)vlb::ceil_div(cols, kThreads), kThreads, 0, db + k0, plan.db, dz.ld, cols,
+                    vlb::ceil_div(x.rows, 32), scale, n0 > 0);
+        VLB_LAUNCHED(q.ctx, 1);
+      }
+      // both derivatives in one launch, the longer reduction first
+      vlb::PairProduct two[2] = {};
+      int count = 0;
+      if (dX) {
+        vlb::PairProduct& d = two[count++];
+        d.a = {dz, false}; d.b = {f, true};
+        d.M = x.rows; d.N = q.D; d.K = cols;
+        d.e.eb.largest = plan.largest + 1;
+        d.e.out = dX + (size_t)n0 * q.D; d.e.beta = k0 ? 1.f : 0.f;
+      }
+      if (dF) {
+        vlb::PairProduct& d = two[count++];
+        d.a = {dz, true}; d.b = {x, true};
+        d.M = cols; d.N = q.D; d.K = x.rows;
+        d.e.eb.largest = plan.largest;
+        d.e.out = dF + (size_t)k0 * q.D; d.e.beta = n0 ? 1.f : 0.f;
+      }
+      for (int i = 0; i < count; ++i) { two[i].e.ea.value = kDzExp; two[i].e.alpha = scale; two[i].e.ldc = q.D; }
+      if (count == 2 && two[1].K > two[0].K) std::swap(two[0], two[1]);
+      if (count)
+        if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairOut, two, count, plan.split)) return rc;
+    }
+  }
+  return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_backward");
+}
+
 // Classes per piece: predictions of a piece up to 64 MB.
 int piece_of(int N, int K) { return (int)std::min<long long>(K, std::max<long long>(64, (16ll << 20) / N / 64 * 64)); }
 
@@ -127,6 +356,8 @@ int vlb_fc_softmaxloss_forward(vlb_ctx* ctx, float* loss, float* lse, float cons
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W * C <= INT32_MAX, "fc_softmaxloss_forward: bad shape");
   VLB_REQUIRE(ctx, loss && X && F && labels, "fc_softmaxloss_forward: null tensor");
+  if (ctx->precision != VLB_PRECISION_FP32)
+    return vlb::pass_error(ctx, forward_on_pairs({ctx, X, F, b, labels, N, H * W * C, K}, loss, lse), "vlb_fc_softmaxloss_forward");
   int const D = H * W * C, piece = piece_of(N, K);
   char* const ws = (char*)vlb::workspace(ctx, sizeof(float) * (size_t)N * piece + sizeof(Seen) * (size_t)N);
   if (!ws) return vlb::pass_error(ctx, ctx->lastError, "vlb_fc_softmaxloss_forward");
@@ -149,6 +380,8 @@ int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, f
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W * C <= INT32_MAX, "fc_softmaxloss_backward: bad shape");
   VLB_REQUIRE(ctx, X && F && labels, "fc_softmaxloss_backward: null tensor");
+  if (ctx->precision != VLB_PRECISION_FP32)
+    return vlb::pass_error(ctx, backward_on_pairs({ctx, X, F, b, labels, N, H * W * C, K}, dX, dF, db, lse, (float)(dzdy / N)), "vlb_fc_softmaxloss_backward");
   int const D = H * W * C, piece = piece_of(N, K);
   size_t const ND = (size_t)N * D;
   float* const z = (float*)vlb::workspace(ctx, sizeof(float) * ((size_t)N * piece + N + ND) + sizeof(Seen) * (size_t)N);

@@ -1,4 +1,5 @@
 // The Muon solver (include/vlb.h has the formulas).
+#include "pairs.cuh"
 #include "products.cuh"
 #include <math.h>
 #include <algorithm>
@@ -45,6 +46,242 @@ __global__ void step_kernel(float* __restrict__ w, float const* __restrict__ x, 
   for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kThreads) w[i] -= rate * x[i];
 }
 
+// ------------------------------------------------------------------ on pairs of halves (pairs.cu)
+constexpr int kMost = vlb::kMaxPairProducts;
+
+// One parameter's share of a launch over several: blocks block0 ... block0 + blocks - 1.
+struct Job {
+  float *w, *s1; float const* g; float* u;
+  size_t n;
+  float decay, rate;
+  double* parts;                     // sums of squares, one per block of momentum_many_kernel
+  int partCount, block0, blocks, vec;
+  vlb::Pair x;
+  int rowsPer; vlb::FastDiv perRow;  // make_x_kernel: rows of a block, sixteen columns at a time
+};
+struct Jobs { Job j[kMost]; int count; };
+
+__device__ __forceinline__ Job const& job_of(Jobs const& jobs, int& block)
+{
+  int i = 0;
+  while (i + 1 < jobs.count && block >= jobs.j[i + 1].block0) ++i;
+  block -= jobs.j[i].block0;
+  return jobs.j[i];
+}
+
+__device__ __forceinline__ double block_sum(double sum)
+{
+  __shared__ double all[kThreads / 32];
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = all[0];
+  for (int i = 1; i < kThreads / 32; ++i) sum += all[i];
+  return sum;
+}
+
+__global__ void __launch_bounds__(kThreads)
+momentum_many_kernel(const __grid_constant__ Jobs jobs, float gradMult, float momentum, int nesterov)
+{
+  vlb::pdl_wait();
+  int block = blockIdx.x;
+  Job const& j = job_of(jobs, block);
+  double sum = 0;
+  auto one = [&](float w, float& m, float g) {
+    float const d = gradMult * g + j.decay * w;
+    m = momentum * m + d;
+    float const v = nesterov ? d + momentum * m : m;
+    sum += (double)v * v;
+    return v;
+  };
+  size_t const step = (size_t)j.blocks * kThreads;
+  if (j.vec) {
+    for (size_t i = (size_t)block * kThreads + threadIdx.x; i < j.n / 4; i += step) {
+      float4 const w = ((float4 const*)j.w)[i], g = ((float4 const*)j.g)[i];
+      float4 m = ((float4 const*)j.s1)[i], v;
+      v.x = one(w.x, m.x, g.x); v.y = one(w.y, m.y, g.y); v.z = one(w.z, m.z, g.z); v.w = one(w.w, m.w, g.w);
+      ((float4*)j.s1)[i] = m;
+      ((float4*)j.u)[i] = v;
+    }
+  } else {
+    for (size_t i = (size_t)block * kThreads + threadIdx.x; i < j.n; i += step) {
+      float m = j.s1[i];
+      j.u[i] = one(j.w[i], m, j.g[i]);
+      j.s1[i] = m;
+    }
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) j.parts[block] = sum;
+}
+
+__device__ __forceinline__ float norm_factor(Job const& j, double epsilon)
+{
+  double sum = 0;
+  for (int i = threadIdx.x; i < j.partCount; i += kThreads) sum += j.parts[i];
+  return (float)(1. / (sqrt(block_sum(sum)) + epsilon));
+}
+
+// u / (|u| + epsilon) as a pair scaled by 2^e.
+__global__ void __launch_bounds__(kThreads)
+make_x_kernel(const __grid_constant__ Jobs jobs, double epsilon, int e)
+{
+  vlb::pdl_wait();
+  int block = blockIdx.x;
+  Job const& j = job_of(jobs, block);
+  float const norm = norm_factor(j, epsilon), f = vlb::pow2(e);
+  int const groups = (int)(j.x.ld / 16);
+  for (int t = threadIdx.x; t < j.rowsPer * groups; t += kThreads) {
+    int const r = j.perRow(t), c = (t - r * groups) * 16;
+    long long const row = (long long)block * j.rowsPer + r;
+    if (row >= j.x.rows) break;
+    float const* const p = j.u + row * j.x.cols + c;
+    float v[16];
+    if (j.x.cols % 4 == 0 && c + 16 <= j.x.cols) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4 const q = __ldg((float4 const*)p + i);
+        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = c + i < j.x.cols ? __ldg(p + i) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = v[i] * norm * f;
+    vlb::store_pair16(j.x, row, c, v);
+  }
+}
+
+// Without a Newton-Schulz step.
+__global__ void __launch_bounds__(kThreads)
+step_many_kernel(const __grid_constant__ Jobs jobs, double epsilon)
+{
+  vlb::pdl_wait();
+  int block = blockIdx.x;
+  Job const& j = job_of(jobs, block);
+  float const f = norm_factor(j, epsilon);
+  for (size_t i = (size_t)block * kThreads + threadIdx.x; i < j.n; i += (size_t)j.blocks * kThreads) j.w[i] -= j.rate * (j.u[i] * f);
+}
+
+// The largest magnitude of t + b t' + c t'' over [0, s]: of a*t + b*t^3 + c*t^5 or of b*t + c*t^2, with 2% for what lies between the samples.
+template <class F>
+double most(F f, double s)
+{
+  double m = 0;
+  for (int i = 0; i <= 1024; ++i) m = std::max(m, fabs(f(s * i / 1024)));
+  return 1.02 * m;
+}
+
+// The exponent that keeps magnitudes up to m below 2^15.
+int exp_below_half(double m)
+{
+  if (!(m < 1e30)) return -100;
+  return m < 1e-25 ? 97 : 14 - (int)ceil(log2(m));
+}
+
+int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* o)
+{
+  Jobs jobs = {};
+  vlb::PairProduct gram[kMost] = {}, poly[kMost] = {}, next[kMost] = {};
+  vlb::Pair x[2][kMost], a[kMost], q[kMost];
+  size_t bytes = 0;
+  char* at = nullptr;
+  auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
+  char* split = nullptr;
+  for (int pass = 0; pass < 2; ++pass) {
+    bytes = 0;
+    split = take(vlb::kPairSplitBytes);
+    for (int i = 0; i < count; ++i) {
+      int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
+      jobs.j[i].u = (float*)take(sizeof(float) * (size_t)rows * cols);
+      jobs.j[i].parts = (double*)take(sizeof(double) * kMaxParts);
+      x[0][i] = vlb::pair_at(take(vlb::pair_bytes(rows, cols)), rows, cols);
+      x[1][i] = vlb::pair_at(take(vlb::pair_bytes(rows, cols)), rows, cols);
+      a[i] = vlb::pair_at(take(vlb::pair_bytes(m, m)), m, m);
+      q[i] = vlb::pair_at(take(vlb::pair_bytes(m, m)), m, m);
+    }
+    if (pass == 0 && !(at = (char*)vlb::workspace(ctx, bytes))) return ctx->lastError;
+  }
+  jobs.count = count;
+  int blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    Job& j = jobs.j[i];
+    j.w = u[i].W; j.s1 = u[i].S1; j.g = u[i].G;
+    j.n = (size_t)u[i].rows * u[i].cols;
+    j.decay = (float)u[i].decay;
+    j.rate = (float)(u[i].lr * sqrt(std::max(1., (double)u[i].rows / u[i].cols)));
+    j.vec = j.n % 4 == 0 && (((uintptr_t)j.w | (uintptr_t)j.s1 | (uintptr_t)j.g) & 15) == 0;
+    j.block0 = blocks;
+    j.blocks = j.partCount = (int)vlb::grid_for((j.n + 3) / 4, kThreads, kMaxParts);
+    blocks += j.blocks;
+    j.x = x[0][i];
+  }
+  vlb::launch(ctx->stream, momentum_many_kernel, (unsigned)blocks, kThreads, 0, jobs, (float)gradMult, (float)o->momentum, o->nesterov);
+  VLB_LAUNCHED(ctx, 1);
+  if (o->steps == 0) {
+    vlb::launch(ctx->stream, step_many_kernel, (unsigned)blocks, kThreads, 0, jobs, o->epsilon);
+    VLB_LAUNCHED(ctx, 1);
+    return VLB_Success;
+  }
+  double s = 1;                                        // no singular value is larger
+  int ex = exp_below_half(s);
+  blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    Job& j = jobs.j[i];
+    int const groups = (int)(j.x.ld / 16);
+    j.rowsPer = std::max(1, 512 / groups);
+    j.perRow = vlb::FastDiv(groups);
+    j.block0 = blocks;
+    j.blocks = vlb::ceil_div(j.x.rows, j.rowsPer);
+    blocks += j.blocks;
+  }
+  vlb::launch(ctx->stream, make_x_kernel, (unsigned)blocks, kThreads, 0, jobs, o->epsilon, ex);
+  VLB_LAUNCHED(ctx, 1);
+  for (int k = 0; k < o->steps; ++k) {
+    // every element of a matrix is at most its largest singular value, which the polynomials bound
+    double const s2 = s * s;
+    s = most([&](double t) { return t * (o->a + t * t * (o->b + t * t * o->c)); }, s);
+    int const ea = exp_below_half(s2), eq = exp_below_half(most([&](double t) { return t * (o->b + t * o->c); }, s2)), en = exp_below_half(s);
+    for (int i = 0; i < count; ++i) {
+      int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
+      bool const tall = rows > cols;
+      vlb::Pair const& xi = x[k & 1][i];
+      vlb::PairProduct &g = gram[i], &p = poly[i], &n = next[i];
+      g.a = g.b = {xi, tall};
+      g.M = g.N = m; g.K = std::max(rows, cols);
+      g.symmetric = true;
+      g.e.ea.value = g.e.eb.value = ex; g.e.alpha = 1.f; g.e.to = a[i]; g.e.toExp = ea;
+      p.a = p.b = {a[i], false};
+      p.M = p.N = p.K = m;
+      p.symmetric = true;
+      p.e.ea.value = p.e.eb.value = ea; p.e.alpha = (float)o->c; p.e.beta = (float)o->b; p.e.add = a[i]; p.e.addExp = ea; p.e.to = q[i]; p.e.toExp = eq;
+      n.a = tall ? vlb::PairSide{xi, false} : vlb::PairSide{q[i], false};
+      n.b = tall ? vlb::PairSide{q[i], false} : vlb::PairSide{xi, true};
+      n.M = rows; n.N = cols; n.K = m;
+      n.e.ea.value = tall ? ex : eq; n.e.eb.value = tall ? eq : ex;
+      n.e.alpha = 1.f; n.e.beta = (float)o->a; n.e.add = xi; n.e.addExp = ex;
+      if (k + 1 < o->steps) { n.e.to = x[(k + 1) & 1][i]; n.e.toExp = en; }
+      else                  { n.e.out = u[i].W; n.e.ldc = cols; n.e.rate = jobs.j[i].rate; }
+    }
+    for (auto const* set : {gram, poly, next})
+      if (int const rc = vlb::products_of_pairs(ctx, vlb::kPairPoly, set, count, split)) return rc;
+    ex = en;
+  }
+  return VLB_Success;
+}
+
+bool overlap(void const* p, size_t n, void const* q, size_t m) { return (char const*)p < (char const*)q + m && (char const*)q < (char const*)p + n; }
+
+// Whether what one of them writes is anything of the other's.
+bool overlap(vlb_muon_param const& a, vlb_muon_param const& b)
+{
+  size_t const n = sizeof(float) * (size_t)a.rows * a.cols, m = sizeof(float) * (size_t)b.rows * b.cols;
+  for (void const* p : {(void const*)a.W, (void const*)a.S1})
+    for (void const* q : {(void const*)b.W, (void const*)b.S1, (void const*)b.G})
+      if (overlap(p, n, q, m)) return true;
+  return overlap(b.W, m, a.G, n) || overlap(b.S1, m, a.G, n);
+}
+
 }  // namespace
 
 extern "C" {
@@ -62,6 +299,17 @@ int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, doubl
     most = std::max(most, 2 * (size_t)u[i].rows * u[i].cols + 2 * m * m);
   }
   if (count == 0) return VLB_Success;
+  if (ctx->precision != VLB_PRECISION_FP32) {
+    for (int first = 0, end; first < count; first = end) {
+      for (end = first + 1; end < count && end - first < kMost; ++end) {
+        bool apart = true;
+        for (int i = first; apart && i < end; ++i) apart = !overlap(u[i], u[end]);
+        if (!apart) break;
+      }
+      if (int const rc = update_on_pairs(ctx, end - first, u + first, gradMult, o)) return vlb::pass_error(ctx, rc, "vlb_muon_update_many");
+    }
+    return vlb::check_launch(ctx, "vlb_muon_update_many");
+  }
   double* const parts = (double*)vlb::workspace(ctx, sizeof(double) * kMaxParts + sizeof(float) * most);
   if (!parts) return vlb::pass_error(ctx, ctx->lastError, "vlb_muon_update_many");
   for (int i = 0; i < count; ++i) {
@@ -73,7 +321,7 @@ int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, doubl
                 (float)o->momentum, o->nesterov, parts);
     vlb::launch(ctx->stream, normalise_kernel, grid, kThreads, 0, x, n, parts, (int)grid, o->epsilon);
     for (int k = 0; k < o->steps; ++k) {
-      vlb::Operand const byRow = {x, cols, 1}, byCol = {x, 1, cols};
+      vlb::Strided const byRow = {x, cols, 1}, byCol = {x, 1, cols};
       if (rows <= cols) vlb::products_exact(ctx, a, m, m, m, cols, byRow, byRow, 1.f, 0.f, nullptr, nullptr);
       else              vlb::products_exact(ctx, a, m, m, m, rows, byCol, byCol, 1.f, 0.f, nullptr, nullptr);
       vlb::products_exact(ctx, q, m, m, m, m, {a, m, 1}, {a, m, 1}, (float)o->c, (float)o->b, a, nullptr);

@@ -1,0 +1,737 @@
+// Products of matrices held as pairs of halves, on tcgen05 / TMEM with operands delivered by tensor-map copies.
+//
+// D[i][j] = sum over k of A(i, k) * B(j, k), where A and B are row-major matrices of halves, hi and lo (pairs.cuh), either of which may be read along its rows or
+// along its columns: the tensor core takes K-major and MN-major tiles alike, so no operand is ever transposed.  A product of two values is three products of
+// halves, lo*hi + hi*lo + hi*hi (lo*lo, 2^-22, is dropped); every k-block of 64 is an accumulation chain of its own in tensor memory, small terms first, then
+// hi*hi on the accumulator scaled by 2^-11, and is added to the tile's single-precision running sum, which eight drain warps hold in registers: the tensor
+// core truncates when it adds, and twelve additions have no time to pile up.
+//
+// A tile is 256 x 256 on a pair of CTAs (cta_group::2: each loads 128 rows of A and 128 of B and holds 128 rows of the accumulator) or 128 x 128 on one.
+// Roles of a CTA's warps: 0-7 drain (warp w: TMEM lanes 32 (w % 4), half w / 4 of the columns), 8 loads, 9 issues the MMAs (of the pair's first CTA), 10 and
+// 11 complete the warpgroup that gives registers to the drain warps (setmaxnreg moves them by whole warpgroups; a pair's drain threads hold 128 sums each).
+// Persistent: CTAs walk the work (product, tile, range of the reduction) with a stride; pipeline indices run through, so a tile's epilogue overlaps the next
+// tile's first chains.  A reduction that is cut leaves its partial sums in scratch; the drain warps that take a tile's last ticket add them up in the order of
+// the ranges, so results do not depend on timing.
+#include "pairs.cuh"
+#include "tc_common.cuh"
+#include <math.h>
+
+namespace {
+
+using vlb::PairEpilogue; using vlb::PairKind; using vlb::PairProduct; using vlb::Pair;
+using vlb::kPairOut; using vlb::kPairSeen; using vlb::kPairGrad; using vlb::kPairPoly;
+using vlb::pow2; using vlb::exp_of; using vlb::load32; using vlb::store_pair16;
+
+constexpr int kThreads = 384, kDrainWarps = 8;
+constexpr int kLaunchRegs = 168, kDrainRegs = 224, kOtherRegs = 56;     // registers per thread: 8 * 224 + 4 * 56 = 12 * 168
+constexpr int kDepth = 64;                       // halves of a k-block: 128 bytes, a row of the swizzle
+constexpr int kHalfTile = 128 * kDepth * 2;      // bytes of one operand's hi or lo part of a stage
+constexpr int kStageBytes = 4 * kHalfTile, kStages = 3;
+constexpr int kRing = 8;                         // barriers of finished k-blocks; more than a waiter can fall behind (3 stages, 4 accumulators)
+constexpr int kPatch = 32 * 33;                  // floats of a warp's transposition patch
+constexpr size_t kSmem = (size_t)kStages * kStageBytes + kDrainWarps * kPatch * sizeof(float) + 1024;
+
+struct Product {
+  int M, N, kBlocks, tilesM, tilesN, splits, work;      // work: items in front of and including this product's
+  int byColsA, byColsB, symmetric;
+  int slot0; long long part0;                           // tickets and partial results in front of this product's, per CTA of a pair
+  PairEpilogue e;
+};
+
+template <int kMax> struct Batch {
+  CUtensorMap map[4 * kMax];                            // a.hi, a.lo, b.hi, b.lo of each product
+  Product p[kMax];
+  int count, work, three;
+  float* split;
+  int* tickets;
+  int* status;
+};
+
+struct Item { int prod, tile, tm, tn, split, kb0, kb1; };
+
+template <int kMax>
+__device__ __forceinline__ Item item_of(Batch<kMax> const& b, int w)
+{
+  Item t;
+  t.prod = 0;
+  while (kMax > 1 && w >= b.p[t.prod].work) ++t.prod;
+  Product const& p = b.p[t.prod];
+  if (t.prod) w -= b.p[t.prod - 1].work;
+  t.tile = w / p.splits;
+  t.split = w - t.tile * p.splits;
+  t.kb0 = (int)((long long)p.kBlocks * t.split / p.splits);
+  t.kb1 = (int)((long long)p.kBlocks * (t.split + 1) / p.splits);
+  if (p.symmetric) {
+    int i = (int)((sqrtf(8.f * t.tile + 1.f) - 1.f) * 0.5f);
+    while (i * (i + 1) / 2 > t.tile) --i;
+    while ((i + 1) * (i + 2) / 2 <= t.tile) ++i;
+    t.tm = i; t.tn = t.tile - i * (i + 1) / 2;
+  } else {
+    // groups of eight row tiles, column by column: what runs at one time reads few different tiles
+    int const per = 8 * p.tilesN, g = t.tile / per, r = t.tile - g * per, rows = min(8, p.tilesM - 8 * g);
+    t.tn = r / rows; t.tm = 8 * g + r - t.tn * rows;
+  }
+  return t;
+}
+
+// ------------------------------------------------------------------ PTX
+__device__ __forceinline__ uint32_t rank_in_cluster() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync()
+{ asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// the same shared-memory place in the cluster's first CTA
+__device__ __forceinline__ uint32_t in_first(uint32_t addr)
+{ uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr)); return r; }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar)
+{ asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+
+template <int kCtas>
+__device__ __forceinline__ void load_box(uint32_t dst, CUtensorMap const* map, int x, int y, uint32_t bar)
+{
+  if (kCtas == 2)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+
+template <int kCtas>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+  if (kCtas == 2)
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// d = a*b + d * 2^-11
+template <int kCtas>
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc)
+{
+  if (kCtas == 2)
+    asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, %3, %3;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, 11;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+  else
+    asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, %3, %3;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+}
+// arrives on the barrier of each CTA of the pair when the MMAs issued so far are through
+template <int kCtas>
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+  if (kCtas == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    umma_commit(bar);
+}
+// the end of all MMAs issued so far; bounded like every wait
+template <int kCtas>
+__device__ __forceinline__ void finish_mma(uint32_t bar) { commit<kCtas>(bar); mbar_wait(bar, 0u, kWaitCycles); }
+template <int kCtas>
+__device__ __forceinline__ void alloc_tmem(uint32_t dst)
+{
+  if (kCtas == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, 512);
+  }
+}
+template <int kCtas>
+__device__ __forceinline__ void free_tmem(uint32_t t)
+{
+  if (kCtas == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(t) : "memory");
+  else            tmem_dealloc(t, 512);
+}
+// A prediction's exponential below the largest of its row: exp(-inf - -inf) and exp(inf - inf) count as 1.
+__device__ __forceinline__ float exp_below(float z, float top) { return z == top ? 1.f : expf(z - top); }
+
+// ------------------------------------------------------------------ epilogues
+// acc: kCols columns from col0 on of row `row` (a lane's), the same columns of the rows row0 + 0 .. 31 in the warp.
+template <int kCols>
+__device__ __forceinline__ void finish_out(Product const& p, float (&acc)[kCols], int row0, int col0, float* patch)
+{
+  PairEpilogue const& e = p.e;
+  int const lane = threadIdx.x & 31;
+  float const fa = pow2(-exp_of(e.ea)), fb = pow2(-exp_of(e.eb)), alpha = e.alpha;
+  int const rows = min(32, p.M - row0);
+#pragma unroll
+  for (int g = 0; g < kCols / 32; ++g) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = acc[g * 32 + i];
+    __syncwarp();
+    int const c = col0 + g * 32 + lane;
+    if (c < p.N) {
+      float* const o = e.out + (long long)row0 * e.ldc + c;
+      if (e.beta != 0.f) {
+        for (int r = 0; r < rows; r += 8) {
+          float old[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (r + i < rows) old[i] = o[(r + i) * e.ldc];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (r + i < rows) o[(r + i) * e.ldc] = patch[(r + i) * 33 + lane] * fa * fb * alpha + old[i];
+        }
+      } else {
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) o[r * e.ldc] = patch[r * 33 + lane] * fa * fb * alpha;
+      }
+    }
+    __syncwarp();
+  }
+}
+
+// predictions = product + bias in place, -inf beyond the last column
+template <int kCols>
+__device__ __forceinline__ void predictions(Product const& p, float (&acc)[kCols], int col0)
+{
+  PairEpilogue const& e = p.e;
+  float const fa = pow2(-exp_of(e.ea)), fb = pow2(-exp_of(e.eb));
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    float const z = acc[i] * fa * fb;
+    acc[i] = col0 + i < p.N ? (e.bias ? z + __ldg(e.bias + col0 + i) : z) : -INFINITY;
+  }
+}
+
+template <int kCols>
+__device__ __forceinline__ void finish_seen(Product const& p, float (&acc)[kCols], int row, int col0)
+{
+  PairEpilogue const& e = p.e;
+  predictions(p, acc, col0);
+  if (row >= p.M) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) top = fmaxf(top, acc[i]);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) if (col0 + i < p.N) sum += exp_below(acc[i], top);
+  e.parts[(long long)(col0 / kCols) * p.M + row] = make_float2(top, sum);
+  int const at = min(max((int)__ldg(e.labels + row) - 1, 0), e.classes - 1) - e.firstClass - col0;
+  if (at >= 0 && at < kCols && col0 + at < p.N) {
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) if (i == at) z = acc[i];
+    e.label[row] = z;
+  }
+}
+
+// Sums over the 32 lanes of 32 values each: afterwards lane l holds the sum of v[l] in v[0].
+__device__ __forceinline__ float lane_sums(float (&v)[32])
+{
+  int const lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    bool const up = lane & s;
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      float const send = up ? v[i] : v[i + s], keep = up ? v[i + s] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
+    }
+  }
+  return v[0];
+}
+
+template <int kCols>
+__device__ __forceinline__ void finish_grad(Product const& p, float (&acc)[kCols], int row0, int row, int col0)
+{
+  PairEpilogue const& e = p.e;
+  predictions(p, acc, col0);
+  bool const in = row < p.M;
+  float const l = in ? __ldg(e.labels + row) : 0.f, lse = in ? __ldg(e.lse + row) : 0.f;
+  bool const real = l > 0.f && l <= (float)e.classes;
+  if (l > (float)e.classes && e.status) atomicExch(e.status, kStatusBadLabel);
+  int const at = min(max((int)l - 1, 0), e.classes - 1) - e.firstClass - col0;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    float const v = expf(acc[i] - lse) - (i == at ? 1.f : 0.f);
+    acc[i] = real && col0 + i < p.N ? v : 0.f;
+  }
+  if (e.db) {
+#pragma unroll
+    for (int g = 0; g < kCols / 32; ++g) {
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = acc[g * 32 + i];
+      float const s = lane_sums(v);
+      int const c = col0 + g * 32 + (threadIdx.x & 31);
+      if (row0 < p.M && c < p.N) e.db[(long long)(row0 / 32) * e.to.ld + c] = s;
+    }
+  }
+  float const f = pow2(e.toExp);
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) acc[i] *= f;
+  if (!in) return;
+#pragma unroll
+  for (int i = 0; i < kCols; i += 16)
+    if (col0 + i < e.to.ld) store_pair16(e.to, row, col0 + i, &acc[i]);
+}
+
+template <int kCols>
+__device__ __forceinline__ void finish_poly(Product const& p, float (&acc)[kCols], int row0, int row, int col0, bool mirror, float* patch)
+{
+  PairEpilogue const& e = p.e;
+  bool const in = row < p.M;
+  float const f = e.alpha * pow2(-exp_of(e.ea)) * pow2(-exp_of(e.eb));
+  if (e.beta != 0.f) {
+    float const fadd = e.beta * pow2(-e.addExp);
+#pragma unroll
+    for (int i = 0; i < kCols; i += 16) {
+      uint32_t hi[8] = {}, lo[8] = {};
+      if (in && col0 + i < e.add.ld) {
+        load32(e.add.hi + row * e.add.ld + col0 + i, hi);
+        load32(e.add.lo + row * e.add.ld + col0 + i, lo);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        __half const h = __ushort_as_half((unsigned short)(hi[j / 2] >> (j % 2 * 16))), l = __ushort_as_half((unsigned short)(lo[j / 2] >> (j % 2 * 16)));
+        acc[i + j] = f * acc[i + j] + fadd * vlb::pair_value(h, l);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) acc[i] *= f;
+  }
+  if (e.out) {
+    int const lane = threadIdx.x & 31, rows = min(32, p.M - row0);
+#pragma unroll
+    for (int g = 0; g < kCols / 32; ++g) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = acc[g * 32 + i];
+      __syncwarp();
+      int const c = col0 + g * 32 + lane;
+      if (c < p.N) {
+        float* const o = e.out + (long long)row0 * e.ldc + c;
+        for (int r = 0; r < rows; r += 8) {
+          float old[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (r + i < rows) old[i] = o[(r + i) * e.ldc];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (r + i < rows) o[(r + i) * e.ldc] = old[i] - e.rate * patch[(r + i) * 33 + lane];
+        }
+      }
+      __syncwarp();
+    }
+    return;
+  }
+  float const ft = pow2(e.toExp);
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) acc[i] *= ft;
+  if (!in) return;
+#pragma unroll
+  for (int i = 0; i < kCols; i += 16)
+    if (col0 + i < e.to.ld) store_pair16(e.to, row, col0 + i, &acc[i]);
+  if (mirror) {
+    // 32 lanes, 32 neighbouring elements of a row of the mirror image
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) {
+      __half h, l;
+      vlb::pair_of(acc[i], h, l);
+      if (col0 + i < p.N) {
+        e.to.hi[(col0 + i) * e.to.ld + row] = h;
+        e.to.lo[(col0 + i) * e.to.ld + row] = l;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the kernel
+template <int kKind, int kMax, int kCtas>
+__global__ void __launch_bounds__(kThreads, 1)
+pairs_kernel(const __grid_constant__ Batch<kMax> batch)
+{
+  constexpr int kTileRows = 128 * kCtas, kTileCols = 128 * kCtas, kCols = kTileCols / 2, kAcc = 512 / kTileCols;
+  extern __shared__ char raw[];
+  __shared__ __align__(8) uint64_t full[kStages], done[kRing], empty[kAcc], last;
+  __shared__ uint32_t tmemAt;
+  __shared__ int ticket;
+  uint32_t const base = (smem_u32(raw) + 1023u) & ~1023u;
+  int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t const rank = kCtas == 2 ? rank_in_cluster() : 0u;
+  int const first = (int)blockIdx.x / kCtas, stride = (int)gridDim.x / kCtas;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&full[i]), 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(smem_u32(&done[i]), 1);
+    for (int i = 0; i < kAcc; ++i) mbar_init(smem_u32(&empty[i]), kDrainWarps * kCtas);
+    mbar_init(smem_u32(&last), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) alloc_tmem<kCtas>(smem_u32(&tmemAt));
+  tc_fence_before();
+  __syncthreads();
+  if (kCtas == 2) cluster_sync();
+  tc_fence_after();
+  uint32_t const tmem = tmemAt;
+  vlb::pdl_wait();
+
+  bool dead = false;                 // a wait ran out: nothing is waited for any more, the work is walked through to the end
+  if (warp < kDrainWarps) {
+    // (a single CTA's drain threads hold 64 sums and do with what they have)
+    if (kCtas == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kDrainRegs));
+    int const quarter = warp & 3, half = warp >> 2;
+    float* const patch = (float*)(raw + (base - smem_u32(raw)) + kStages * kStageBytes) + warp * kPatch;
+    uint32_t const lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kCols);
+    int j = 0;
+    for (int w = first; w < batch.work; w += stride) {
+      Item const t = item_of(batch, w);
+      Product const& p = batch.p[t.prod];
+      float acc[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+      for (int kb = t.kb0; kb < t.kb1; ++kb, ++j) {
+        if (!dead && !mbar_wait(smem_u32(&done[j % kRing]), (uint32_t)(j / kRing) & 1u)) dead = true;
+        if (dead) continue;
+        tc_fence_after();
+        int const buf = j % kAcc;
+        uint32_t const at = lanes + (uint32_t)(buf * kTileCols);
+        uint32_t r[2][16];
+        tmem_ld16_issue(at, r[0]);
+#pragma unroll
+        for (int g = 0; g < kCols / 16; ++g) {
+          tmem_ld_wait();
+          if (g + 1 < kCols / 16) tmem_ld16_issue(at + 16u * (g + 1), r[(g + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[g * 16 + i] += __uint_as_float(r[g & 1][i]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kCtas == 2) mbar_arrive_cluster(in_first(smem_u32(&empty[buf])));
+          else            mbar_arrive(smem_u32(&empty[buf]));
+        }
+      }
+      if (p.splits > 1) {
+        // a tile's partial sums: [tile and CTA][range][column / 4][drain thread]
+        int const slot = (p.slot0 + t.tile) * kCtas + (int)rank;
+        float4* const all = (float4*)batch.split + (p.part0 * kCtas + (long long)(t.tile * kCtas + (int)rank) * p.splits) * (kCols / 4) * 256 + threadIdx.x;
+        float4* const mine = all + (long long)t.split * (kCols / 4) * 256;
+#pragma unroll
+        for (int i = 0; i < kCols / 4; ++i) mine[i * 256] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+        __threadfence();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (threadIdx.x == 0) ticket = atomicAdd(batch.tickets + slot, 1);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (ticket != p.splits - 1) continue;
+        __threadfence();
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+        for (int s = 0; s < p.splits; ++s) {
+#pragma unroll
+          for (int i = 0; i < kCols / 4; ++i) {
+            float4 const v = __ldcg(all + (long long)(s * (kCols / 4) + i) * 256);
+            acc[4 * i] += v.x; acc[4 * i + 1] += v.y; acc[4 * i + 2] += v.z; acc[4 * i + 3] += v.w;
+          }
+        }
+        if (threadIdx.x == 0) batch.tickets[slot] = 0;
+      }
+      int const row0 = t.tm * kTileRows + (int)rank * 128 + quarter * 32, col0 = t.tn * kTileCols + half * kCols;
+      if (kKind == kPairOut)  finish_out(p, acc, row0, col0, patch);
+      if (kKind == kPairSeen) finish_seen(p, acc, row0 + lane, col0);
+      if (kKind == kPairGrad) finish_grad(p, acc, row0, row0 + lane, col0);
+      if (kKind == kPairPoly) finish_poly(p, acc, row0, row0 + lane, col0, p.symmetric && t.tn < t.tm, patch);
+    }
+    if (dead && lane == 0) atomicCAS(batch.status, 0, 42);
+  } else {
+    if (kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      if (lane == 0) {
+        int it = 0;
+        uint32_t const bytes = (batch.three ? 4u : 2u) * kHalfTile;
+        for (int w = first; w < batch.work && !dead; w += stride) {
+          Item const t = item_of(batch, w);
+          Product const& p = batch.p[t.prod];
+          CUtensorMap const* const map = batch.map + 4 * t.prod;
+          int const a0 = t.tm * kTileRows + (int)rank * 128, b0 = t.tn * kTileCols + (int)rank * 128;
+          for (int kb = t.kb0; kb < t.kb1 && !dead; ++kb, ++it) {
+            int const s = it % kStages, before = it - kStages;
+            if (before >= 0 && !mbar_wait(smem_u32(&done[before % kRing]), (uint32_t)(before / kRing) & 1u)) { dead = true; break; }
+            uint32_t const mine = smem_u32(&full[s]), bar = kCtas == 2 ? in_first(mine) : mine;
+            if (rank == 0) mbar_arrive_expect_tx(mine, bytes * kCtas);
+            uint32_t const dst = base + (uint32_t)s * kStageBytes;
+  #pragma unroll
+            for (int part = 0; part < 4; ++part) {
+              if ((part & 1) && !batch.three) continue;
+              uint32_t const to = dst + (uint32_t)part * kHalfTile;
+              int const r0 = part < 2 ? a0 : b0;
+              if (part < 2 ? p.byColsA : p.byColsB) {
+                load_box<kCtas>(to, map + part, r0, kb * kDepth, bar);
+                load_box<kCtas>(to + kHalfTile / 2, map + part, r0 + 64, kb * kDepth, bar);
+              } else {
+                load_box<kCtas>(to, map + part, kb * kDepth, r0, bar);
+              }
+            }
+          }
+        }
+        if (dead) atomicCAS(batch.status, 0, 40);
+        // copies still on their way when a wait ran out land before the block ends
+        if (dead && rank == 0)
+          for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(smem_u32(&full[j % kStages]), (uint32_t)(j / kStages) & 1u, kWaitCycles);
+      }
+    } else if (warp == 9) {
+      if (lane == 0 && rank == 0) {
+        int j = 0;
+        for (int w = first; w < batch.work && !dead; w += stride) {
+          Item const t = item_of(batch, w);
+          Product const& p = batch.p[t.prod];
+          uint32_t const idesc = (1u << 4) | (p.byColsA ? 1u << 15 : 0u) | (p.byColsB ? 1u << 16 : 0u) | ((uint32_t)(kTileCols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+          uint32_t const lboA = p.byColsA ? kHalfTile / 2 : 16, lboB = p.byColsB ? kHalfTile / 2 : 16;
+          uint64_t const stepA = (p.byColsA ? 2048u : 32u) >> 4, stepB = (p.byColsB ? 2048u : 32u) >> 4;
+          for (int kb = t.kb0; kb < t.kb1; ++kb, ++j) {
+            int const s = j % kStages, acc = j % kAcc;
+            if (!mbar_wait(smem_u32(&full[s]), (uint32_t)(j / kStages) & 1u)) { dead = true; break; }
+            if (j >= kAcc && !mbar_wait(smem_u32(&empty[acc]), (uint32_t)(j / kAcc - 1) & 1u)) { dead = true; break; }
+            tc_fence_after();
+            uint32_t const st = base + (uint32_t)s * kStageBytes, d = tmem + (uint32_t)(acc * kTileCols);
+            uint64_t const aH = make_desc(st, lboA, 1024), aL = make_desc(st + kHalfTile, lboA, 1024);
+            uint64_t const bH = make_desc(st + 2 * kHalfTile, lboB, 1024), bL = make_desc(st + 3 * kHalfTile, lboB, 1024);
+            if (batch.three) {
+  #pragma unroll
+              for (int k = 0; k < kDepth / 16; ++k) {
+                mma<kCtas>(d, aL + stepA * k, bH + stepB * k, idesc, k > 0 ? 1u : 0u);
+                mma<kCtas>(d, aH + stepA * k, bL + stepB * k, idesc, 1u);
+              }
+              mma_scaled<kCtas>(d, aH, bH, idesc);
+  #pragma unroll
+              for (int k = 1; k < kDepth / 16; ++k) mma<kCtas>(d, aH + stepA * k, bH + stepB * k, idesc, 1u);
+            } else {
+  #pragma unroll
+              for (int k = 0; k < kDepth / 16; ++k) mma<kCtas>(d, aH + stepA * k, bH + stepB * k, idesc, k > 0 ? 1u : 0u);
+            }
+            commit<kCtas>(smem_u32(&done[j % kRing]));
+          }
+        }
+        if (dead) atomicCAS(batch.status, 0, 41);
+        // tensor memory is given back only when nothing writes to it any more
+        finish_mma<kCtas>(smem_u32(&last));
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (kCtas == 2) cluster_sync();
+  tc_fence_after();
+  if (warp == 9) free_tmem<kCtas>(tmem);
+}
+
+// ------------------------------------------------------------------ pairs of single-precision matrices
+__device__ __forceinline__ bool is_real(float const* labels, long long row, int classes)
+{
+  if (!labels) return true;
+  float const l = __ldg(labels + row);
+  return l > 0.f && l <= (float)classes;
+}
+__device__ __forceinline__ unsigned finite_bits(float v)
+{
+  unsigned const b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+constexpr int kSplitThreads = 256;
+
+// Rows in turn to the grid's warps.
+__global__ void __launch_bounds__(kSplitThreads)
+largest_kernel(unsigned* largest, float const* __restrict__ x, int rows, int cols, float const* __restrict__ labels, int classes, bool vec)
+{
+  vlb::pdl_wait();
+  int const lane = threadIdx.x & 31, warps = (int)gridDim.x * (kSplitThreads / 32);
+  unsigned m = 0;
+  if (!labels && vec) {                                       // one run of floats
+    long long const n = (long long)rows * cols / 4, step = (long long)gridDim.x * kSplitThreads;
+    float4 const* const v = (float4 const*)x;
+    for (long long i = (long long)blockIdx.x * kSplitThreads + threadIdx.x; i < n; i += 4 * step) {
+      float4 q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] = __ldg(v + min(i + k * step, n - 1));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = max(max(m, max(finite_bits(q[k].x), finite_bits(q[k].y))), max(finite_bits(q[k].z), finite_bits(q[k].w)));
+    }
+  } else {
+    for (int r = (int)blockIdx.x * (kSplitThreads / 32) + (int)(threadIdx.x >> 5); r < rows; r += warps) {
+      if (!is_real(labels, r, classes)) continue;
+      float const* const row = x + (long long)r * cols;
+#pragma unroll 4
+      for (int c = lane; c < cols; c += 32) m = max(m, finite_bits(__ldg(row + c)));
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  __shared__ unsigned all[kSplitThreads / 32];
+  if (lane == 0) all[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kSplitThreads / 32; ++i) m = max(m, all[i]);
+    if (m) atomicMax(largest, m);                             // (the largest does not depend on the order)
+  }
+}
+
+// A block takes rowsPer rows, a thread sixteen neighbouring columns at a time.
+__global__ void __launch_bounds__(kSplitThreads)
+make_pair_kernel(Pair to, float const* __restrict__ x, unsigned const* __restrict__ largest, float const* __restrict__ labels, int classes, int rowsPer,
+                 vlb::FastDiv perRow, bool vec)
+{
+  vlb::pdl_wait();
+  float const f = pow2(vlb::pair_exp(__uint_as_float(__ldg(largest))));
+  int const groups = (int)(to.ld / 16);
+  for (int t = threadIdx.x; t < rowsPer * groups; t += kSplitThreads) {
+    int const r = perRow(t), c = (t - r * groups) * 16;
+    long long const row = (long long)blockIdx.x * rowsPer + r;
+    if (row >= to.rows) break;
+    float v[16];
+    bool const real = is_real(labels, row, classes);
+    float const* const p = x + row * to.cols + c;
+    if (vec && c + 16 <= to.cols) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4 const q = __ldg((float4 const*)p + i);
+        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = c + i < to.cols ? __ldg(p + i) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = real ? v[i] * f : 0.f;
+    store_pair16(to, row, c, v);
+  }
+}
+
+// ------------------------------------------------------------------ host
+bool encode_side(CUtensorMap* hi, CUtensorMap* lo, vlb::PairSide const& s)
+{
+  EncodeTiledFn const encode = encode_tiled();
+  if (!encode) return false;
+  cuuint64_t const dims[2] = {(cuuint64_t)s.m.cols, (cuuint64_t)s.m.rows}, strides[1] = {(cuuint64_t)s.m.ld * 2};
+  cuuint32_t const box[2] = {64, s.byCols ? 64u : 128u}, one[2] = {1, 1};
+  for (int part = 0; part < 2; ++part)
+    if (encode(part ? lo : hi, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, part ? s.m.lo : s.m.hi, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  return true;
+}
+
+int tiles_of(PairProduct const& p, int tile)
+{
+  int const m = vlb::ceil_div(p.M, tile), n = vlb::ceil_div(p.N, tile);
+  return p.symmetric ? m * (m + 1) / 2 : m * n;
+}
+
+template <int kKind, int kMax, int kCtas>
+int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
+{
+  constexpr int kTile = 128 * kCtas;
+  Batch<kMax> b;
+  int const clusters = ctx->smCount / kCtas;
+  long long tiles = 0, blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    int const t = tiles_of(p[i], kTile);
+    tiles += t;
+    blocks += (long long)t * vlb::ceil_div(p[i].K, kDepth);
+  }
+  // Fewer tiles than places to run them: reductions are cut into ranges of about the same length that fill the places, of eight k-blocks at least
+  long long const range = std::max<long long>(8, (blocks + clusters - 1) / clusters);
+  size_t const partBytes = sizeof(float) * 128 * kTile;
+  int slot = 0;
+  long long part = 0, work = 0;
+  for (int i = 0; i < count; ++i) {
+    PairProduct const& q = p[i];
+    Product& d = b.p[i];
+    d.M = q.M; d.N = q.N; d.kBlocks = vlb::ceil_div(q.K, kDepth);
+    d.tilesM = vlb::ceil_div(q.M, kTile); d.tilesN = vlb::ceil_div(q.N, kTile);
+    int const t = tiles_of(q, kTile);
+    d.splits = 1;
+    if (tiles < clusters) {
+      int const s = (int)std::min<long long>((d.kBlocks + range - 1) / range, 64);
+      if (s > 1 && (slot + t) * kCtas <= 4096 && (size_t)((part + (long long)t * s) * kCtas) * partBytes <= vlb::kPairSplitBytes) d.splits = s;
+    }
+    d.slot0 = slot; d.part0 = part;
+    if (d.splits > 1) { slot += t; part += (long long)t * d.splits; }
+    work += (long long)t * d.splits;
+    d.work = (int)work;
+    d.byColsA = q.a.byCols; d.byColsB = q.b.byCols; d.symmetric = q.symmetric;
+    d.e = q.e;
+    if (!encode_side(&b.map[4 * i], &b.map[4 * i + 1], q.a) || !encode_side(&b.map[4 * i + 2], &b.map[4 * i + 3], q.b))
+      return vlb::set_error(ctx, VLB_Cuda, "a tensor map could not be made");
+  }
+  if (work > INT32_MAX) return vlb::set_error(ctx, VLB_IllegalArgument, "the matrices are too large");
+  b.count = count; b.work = (int)work; b.three = ctx->precision != VLB_PRECISION_TF32;
+  b.split = (float*)split;
+  b.tickets = ctx->deviceStatus + 64;
+  b.status = ctx->deviceStatus;
+  auto const kernel = pairs_kernel<kKind, kMax, kCtas>;
+  static bool ready[64];
+  if (!ready[ctx->device & 63]) {
+    cudaError_t const e = vlb::allow_max_dynamic_smem(kernel);
+    if (e != cudaSuccess) return vlb::set_error(ctx, VLB_Cuda, cudaGetErrorString(e));
+    cudaFuncAttributes a;
+    if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess || (kCtas == 2 && a.numRegs != kLaunchRegs))        // the drain warps would wait for registers for ever
+      return vlb::set_error(ctx, VLB_Cuda, "products_of_pairs: the kernel was built with another number of registers");
+    ready[ctx->device & 63] = true;
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kCtas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<long long>(clusters, work) * kCtas)); cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem; cfg.stream = ctx->stream; cfg.attrs = attr; cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kernel, b);
+  VLB_LAUNCHED(ctx, 1);
+  return vlb::check_launch(ctx, "products_of_pairs");
+}
+
+// Whether pairs of CTAs take less time, by k-blocks through the tensor core: 1536 cycles for 256 x 256 on two SMs, 768 for 128 x 128 on one, and a hand-over
+// between k-blocks that a pair's longer ones hide.
+bool pairs_pay(vlb_ctx* ctx, PairProduct const* p, int count)
+{
+  double two = 0, one = 0;
+  for (int i = 0; i < count; ++i) {
+    double const kb = vlb::ceil_div(p[i].K, kDepth);
+    two += tiles_of(p[i], 256) * kb;
+    one += tiles_of(p[i], 128) * kb;
+  }
+  return two / (ctx->smCount / 2) * 1600. <= one / ctx->smCount * 950.;
+}
+
+template <int kKind, int kMax>
+int run_kind(vlb_ctx* ctx, PairProduct const* p, int count, void* split, int* parts)
+{
+  bool const two = pairs_pay(ctx, p, count);
+  if (parts) *parts = 2 * vlb::ceil_div(p->N, two ? 256 : 128);
+  return two ? run<kKind, kMax, 2>(ctx, p, count, split) : run<kKind, kMax, 1>(ctx, p, count, split);
+}
+
+}  // namespace
+
+namespace vlb {
+
+void largest_of(vlb_ctx* ctx, unsigned* largest, float const* x, int rows, int cols, float const* labels, int classes)
+{
+  bool const vec = ((uintptr_t)x & 15) == 0 && (long long)rows * cols % 4 == 0;
+  unsigned const grid = grid_for(!labels && vec ? (size_t)rows * cols / 16 + 1 : (size_t)rows * 32, kSplitThreads, ctx->smCount * 8);
+  launch(ctx->stream, largest_kernel, grid, kSplitThreads, 0, largest, x, rows, cols, labels, classes, vec);
+  VLB_LAUNCHED(ctx, 1);
+}
+
+void make_pair(vlb_ctx* ctx, Pair to, float const* x, unsigned const* largest, float const* labels, int classes)
+{
+  int const groups = (int)(to.ld / 16), rowsPer = std::max(1, 512 / groups);
+  bool const vec = ((uintptr_t)x & 15) == 0 && to.cols % 4 == 0;
+  launch(ctx->stream, make_pair_kernel, (unsigned)ceil_div(to.rows, rowsPer), kSplitThreads, 0, to, x, largest, labels, classes, rowsPer, FastDiv(groups), vec);
+  VLB_LAUNCHED(ctx, 1);
+}
+
+int products_of_pairs(vlb_ctx* ctx, PairKind kind, PairProduct const* p, int count, void* split, int* parts)
+{
+  switch (kind) {
+    case kPairOut:  return run_kind<kPairOut, 2>(ctx, p, count, split, parts);
+    case kPairSeen: return run_kind<kPairSeen, 1>(ctx, p, count, split, parts);
+    case kPairGrad: return run_kind<kPairGrad, 1>(ctx, p, count, split, parts);
+    default:        return count > 1 ? run_kind<kPairPoly, kMaxPairProducts>(ctx, p, count, split, parts) : run_kind<kPairPoly, 1>(ctx, p, count, split, parts);
+  }
+}
+
+cudaError_t pairs_set_wait_limit(long long cycles, cudaStream_t stream)
+{
+  long long const v = cycles == 0 ? kWaitCycles : cycles;
+  return cudaMemcpyToSymbolAsync(gWaitCycles, &v, sizeof(v), 0, cudaMemcpyHostToDevice, stream);
+}
+
+}  // namespace vlb

@@ -3,12 +3,12 @@
 
 namespace {
 
-using vlb::Operand;
+using vlb::Strided;
 
 constexpr int kTile = 64, kDepth = 16;
 
 __global__ void __launch_bounds__(256)
-products_exact_kernel(float* __restrict__ C, long long ldc, int M, int N, int K, int tilesM, Operand a, Operand b, float alpha, float beta,
+products_exact_kernel(float* __restrict__ C, long long ldc, int M, int N, int K, int tilesM, Strided a, Strided b, float alpha, float beta,
                       float const* D, float const* __restrict__ bias)
 {
   vlb::pdl_wait();
@@ -54,7 +54,7 @@ products_exact_kernel(float* __restrict__ C, long long ldc, int M, int N, int K,
 
 namespace vlb {
 
-void products_exact(vlb_ctx* ctx, float* C, long long ldc, int M, int N, int K, Operand a, Operand b, float alpha, float beta, float const* D,
+void products_exact(vlb_ctx* ctx, float* C, long long ldc, int M, int N, int K, Strided a, Strided b, float alpha, float beta, float const* D,
                     float const* bias)
 {
   int const tm = ceil_div(M, kTile), tn = ceil_div(N, kTile);
