@@ -119,8 +119,8 @@ struct Part { float top, sum; };
 
 __device__ __forceinline__ Part together(Part a, Part b)
 {
-  float const top = fmaxf(a.top, b.top);
-  return {top, a.sum * exp_below(a.top, top) + b.sum * exp_below(b.top, top)};
+  float const top = fmaxf(a.top, b.top), base = isinf(top) ? 0.f : top;      // (as where the parts come from)
+  return {top, a.sum * expf(a.top - base) + b.sum * expf(b.top - base)};
 }
 
 // lse of 32 images per block from the parts of their predictions, and the loss by the block that is through last, which adds the blocks' sums in their order.
@@ -204,7 +204,7 @@ struct Plan {
     x = take(vlb::pair_bytes(images, D));
     f = take(vlb::pair_bytes(piece, D));
     split = take(vlb::kPairSplitBytes);
-    parts = (float2*)take(sizeof(float2) * (size_t)images * vlb::pair_parts(piece) * pieces);
+    parts = (float2*)take(sizeof(float2) * (size_t)images * vlb::pair_parts(piece, 128) * pieces);
     label = (float*)take(sizeof(float) * (size_t)images);
     lse = (float*)take(sizeof(float) * (size_t)images);
     sums = (double*)take(sizeof(double) * (size_t)vlb::ceil_div(N, 32));
@@ -254,7 +254,7 @@ vlb::Pair images(Problem const& q, Plan const& plan, int n0, int rows)
 vlb::PairProduct predictions(Problem const& q, Plan const& plan, vlb::Pair x, vlb::Pair f, int n0, int k0)
 {
   vlb::PairProduct p = {};
-  p.a = {x, false}; p.b = {f, false};
+  p.a = {x, false, false}; p.b = {f, false, false};
   p.M = x.rows; p.N = f.rows; p.K = q.D;
   p.e.ea.largest = plan.largest; p.e.eb.largest = plan.largest + 1;
   p.e.bias = q.b ? q.b + k0 : nullptr;
@@ -271,9 +271,9 @@ int seen(Problem const& q, Plan const& plan, vlb::Pair x, int n0, float* lse, fl
     vlb::Pair const f = filters(q, plan, k0, std::min(plan.piece, q.K - k0));
     vlb::PairProduct p = predictions(q, plan, x, f, n0, k0);
     p.e.parts = plan.parts + (size_t)count * x.rows; p.e.label = plan.label;
-    int n = 0;
-    if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairSeen, &p, 1, plan.split, &n)) return rc;
-    count += n;
+    int const tile = vlb::pair_tile(q.ctx, &p, 1);
+    if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairSeen, &p, 1, plan.split, tile)) return rc;
+    count += vlb::pair_parts(f.rows, tile);
   }
   vlb::launch(q.ctx->stream, lse_kernel, (unsigned)vlb::ceil_div(x.rows, 32), 1024, 0, loss, lse, plan.parts, count, plan.label, q.labels + n0, x.rows, n0,
               q.N, q.K, plan.sums, vlb::ceil_div(q.N, 32), q.ctx->deviceStatus + 64 + 4095, status);
@@ -311,7 +311,7 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
       p.e.lse = lse ? lse + n0 : plan.lse;
       p.e.to = dz; p.e.toExp = kDzExp; p.e.db = db ? plan.db : nullptr;
       p.e.status = q.ctx->deviceStatus;
-      if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairGrad, &p, 1, plan.split)) return rc;
+      if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairGrad, &p, 1, plan.split, vlb::pair_tile(q.ctx, &p, 1))) return rc;
       if (db) {
         vlb::launch(q.ctx->stream, db_parts_kernel, (unsigned)vlb::ceil_div(cols, kThreads), kThreads, 0, db + k0, plan.db, dz.ld, cols,
                     vlb::ceil_div(x.rows, 32), scale, n0 > 0);
@@ -322,14 +322,14 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
       int count = 0;
       if (dX) {
         vlb::PairProduct& d = two[count++];
-        d.a = {dz, false}; d.b = {f, true};
+        d.a = {dz, false, false}; d.b = {f, true, false};
         d.M = x.rows; d.N = q.D; d.K = cols;
         d.e.eb.largest = plan.largest + 1;
         d.e.out = dX + (size_t)n0 * q.D; d.e.beta = k0 ? 1.f : 0.f;
       }
       if (dF) {
         vlb::PairProduct& d = two[count++];
-        d.a = {dz, true}; d.b = {x, true};
+        d.a = {dz, true, false}; d.b = {x, true, false};
         d.M = cols; d.N = q.D; d.K = x.rows;
         d.e.eb.largest = plan.largest;
         d.e.out = dF + (size_t)k0 * q.D; d.e.beta = n0 ? 1.f : 0.f;
@@ -337,7 +337,7 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
       for (int i = 0; i < count; ++i) { two[i].e.ea.value = kDzExp; two[i].e.alpha = scale; two[i].e.ldc = q.D; }
       if (count == 2 && two[1].K > two[0].K) std::swap(two[0], two[1]);
       if (count)
-        if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairOut, two, count, plan.split)) return rc;
+        if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairOut, two, count, plan.split, vlb::pair_tile(q.ctx, two, count))) return rc;
     }
   }
   return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_backward");

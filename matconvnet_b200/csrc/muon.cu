@@ -182,7 +182,8 @@ int exp_below_half(double m)
 int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* o)
 {
   Jobs jobs = {};
-  vlb::PairProduct gram[kMost] = {}, poly[kMost] = {}, next[kMost] = {};
+  vlb::PairProduct step[3 * kMost] = {};
+  vlb::PairProduct *const gram = step, *const poly = step + count, *const next = step + 2 * count;
   vlb::Pair x[2][kMost], a[kMost], q[kMost];
   size_t bytes = 0;
   char* at = nullptr;
@@ -247,24 +248,25 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
       bool const tall = rows > cols;
       vlb::Pair const& xi = x[k & 1][i];
       vlb::PairProduct &g = gram[i], &p = poly[i], &n = next[i];
-      g.a = g.b = {xi, tall};
+      g.a = g.b = {xi, tall, false};
       g.M = g.N = m; g.K = std::max(rows, cols);
       g.symmetric = true;
       g.e.ea.value = g.e.eb.value = ex; g.e.alpha = 1.f; g.e.to = a[i]; g.e.toExp = ea;
-      p.a = p.b = {a[i], false};
+      p.a = p.b = {a[i], false, true};
       p.M = p.N = p.K = m;
       p.symmetric = true;
       p.e.ea.value = p.e.eb.value = ea; p.e.alpha = (float)o->c; p.e.beta = (float)o->b; p.e.add = a[i]; p.e.addExp = ea; p.e.to = q[i]; p.e.toExp = eq;
-      n.a = tall ? vlb::PairSide{xi, false} : vlb::PairSide{q[i], false};
-      n.b = tall ? vlb::PairSide{q[i], false} : vlb::PairSide{xi, true};
+      n.a = tall ? vlb::PairSide{xi, false, false} : vlb::PairSide{q[i], false, true};
+      n.b = tall ? vlb::PairSide{q[i], false, true} : vlb::PairSide{xi, true, false};
       n.M = rows; n.N = cols; n.K = m;
       n.e.ea.value = tall ? ex : eq; n.e.eb.value = tall ? eq : ex;
       n.e.alpha = 1.f; n.e.beta = (float)o->a; n.e.add = xi; n.e.addExp = ex;
       if (k + 1 < o->steps) { n.e.to = x[(k + 1) & 1][i]; n.e.toExp = en; }
       else                  { n.e.out = u[i].W; n.e.ldc = cols; n.e.rate = jobs.j[i].rate; }
     }
-    for (auto const* set : {gram, poly, next})
-      if (int const rc = vlb::products_of_pairs(ctx, vlb::kPairPoly, set, count, split)) return rc;
+    int const tile = vlb::pair_tile(ctx, step, 3 * count);          // (one for all: what one product leaves of a symmetric matrix the next one reads)
+    for (int set = 0; set < 3; ++set)
+      if (int const rc = vlb::products_of_pairs(ctx, vlb::kPairPoly, step + set * count, count, split, tile)) return rc;
     ex = en;
   }
   return VLB_Success;

@@ -1,14 +1,15 @@
 // Products of matrices held as pairs of halves, on tcgen05 / TMEM with operands delivered by tensor-map copies.
 //
 // D[i][j] = sum over k of A(i, k) * B(j, k), where A and B are row-major matrices of halves, hi and lo (pairs.cuh), either of which may be read along its rows or
-// along its columns: the tensor core takes K-major and MN-major tiles alike, so no operand is ever transposed.  A product of two values is three products of
+// along its columns: the tensor core takes K-major and MN-major tiles alike, so no operand is ever transposed, and of a symmetric matrix only the tiles on and
+// under the diagonal are made and kept: what lies above is read along the other index.  A product of two values is three products of
 // halves, lo*hi + hi*lo + hi*hi (lo*lo, 2^-22, is dropped); every k-block of 64 is an accumulation chain of its own in tensor memory, small terms first, then
 // hi*hi on the accumulator scaled by 2^-11, and is added to the tile's single-precision running sum, which eight drain warps hold in registers: the tensor
 // core truncates when it adds, and twelve additions have no time to pile up.
 //
 // A tile is 256 x 256 on a pair of CTAs (cta_group::2: each loads 128 rows of A and 128 of B and holds 128 rows of the accumulator) or 128 x 128 on one.
-// Roles of a CTA's warps: 0-7 drain (warp w: TMEM lanes 32 (w % 4), half w / 4 of the columns), 8 loads, 9 issues the MMAs (of the pair's first CTA), 10 and
-// 11 complete the warpgroup that gives registers to the drain warps (setmaxnreg moves them by whole warpgroups; a pair's drain threads hold 128 sums each).
+// Roles of a CTA's warps: 0-7 drain (warp w: TMEM lanes 32 (w % 4), half w / 4 of the columns), 8 loads A, 10 loads B, 9 issues the MMAs (of the pair's first
+// CTA), 11 completes the warpgroup that gives registers to the drain warps (setmaxnreg moves them by whole warpgroups; a pair's drain threads hold 128 sums each).
 // Persistent: CTAs walk the work (product, tile, range of the reduction) with a stride; pipeline indices run through, so a tile's epilogue overlaps the next
 // tile's first chains.  A reduction that is cut leaves its partial sums in scratch; the drain warps that take a tile's last ticket add them up in the order of
 // the ranges, so results do not depend on timing.
@@ -20,26 +21,26 @@ namespace {
 
 using vlb::PairEpilogue; using vlb::PairKind; using vlb::PairProduct; using vlb::Pair;
 using vlb::kPairOut; using vlb::kPairSeen; using vlb::kPairGrad; using vlb::kPairPoly;
-using vlb::pow2; using vlb::exp_of; using vlb::load32; using vlb::store_pair16;
+using vlb::pow2; using vlb::exp_of; using vlb::store_pair16;
 
 constexpr int kThreads = 384, kDrainWarps = 8;
 constexpr int kLaunchRegs = 168, kDrainRegs = 224, kOtherRegs = 56;     // registers per thread: 8 * 224 + 4 * 56 = 12 * 168
 constexpr int kDepth = 64;                       // halves of a k-block: 128 bytes, a row of the swizzle
-constexpr int kHalfTile = 128 * kDepth * 2;      // bytes of one operand's hi or lo part of a stage
+constexpr int kHalfTile = 128 * kDepth * 2;      // bytes of one operand's hi or lo part of a stage.  Along the rows: hi, lo; along the columns: hi and lo of 64 rows, twice
 constexpr int kStageBytes = 4 * kHalfTile, kStages = 3;
 constexpr int kRing = 8;                         // barriers of finished k-blocks; more than a waiter can fall behind (3 stages, 4 accumulators)
-constexpr int kPatch = 32 * 33;                  // floats of a warp's transposition patch
-constexpr size_t kSmem = (size_t)kStages * kStageBytes + kDrainWarps * kPatch * sizeof(float) + 1024;
+constexpr int kPatch = 32 * 33;                  // floats of a warp's patch
+constexpr size_t kSmem = (size_t)kStages * kStageBytes + kDrainWarps * kPatch * sizeof(float) + 1024;       // (the stages begin at a multiple of 1024)
 
 struct Product {
   int M, N, kBlocks, tilesM, tilesN, splits, work;      // work: items in front of and including this product's
-  int byColsA, byColsB, symmetric;
+  int byColsA, byColsB, lowerA, lowerB, symmetric;
   int slot0; long long part0;                           // tickets and partial results in front of this product's, per CTA of a pair
   PairEpilogue e;
 };
 
 template <int kMax> struct Batch {
-  CUtensorMap map[4 * kMax];                            // a.hi, a.lo, b.hi, b.lo of each product
+  CUtensorMap map[4 * kMax];                            // of each product A along its rows, along its columns, B likewise; those that are used
   Product p[kMax];
   int count, work, three;
   float* split;
@@ -74,6 +75,9 @@ __device__ __forceinline__ Item item_of(Batch<kMax> const& b, int w)
   return t;
 }
 
+// Whether k-block kb of a side's tile t is read along the columns.
+__device__ __forceinline__ bool along_cols(int byCols, int lower, int t, int tile, int kb) { return byCols || (lower && kb * kDepth >= (t + 1) * tile); }
+
 // ------------------------------------------------------------------ PTX
 __device__ __forceinline__ uint32_t rank_in_cluster() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync()
@@ -81,18 +85,19 @@ __device__ __forceinline__ void cluster_sync()
 // the same shared-memory place in the cluster's first CTA
 __device__ __forceinline__ uint32_t in_first(uint32_t addr)
 { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr)); return r; }
+// Relaxed: what it tells of are loads from tensor memory that have been waited for.  (With release semantics in the cluster the arrival waits for the whole
+// of the tensor core's work under way: 2200 cycles per k-block of a pair instead of 1800.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar)
-{ asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+{ asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 template <int kCtas>
 __device__ __forceinline__ void load_box(uint32_t dst, CUtensorMap const* map, int x, int y, uint32_t bar)
 {
   if (kCtas == 2)
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar) : "memory");
   else
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    tma_load_3d(dst, map, x, y, 0, bar);
 }
 
 template <int kCtas>
@@ -140,75 +145,144 @@ __device__ __forceinline__ void free_tmem(uint32_t t)
   if (kCtas == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(t) : "memory");
   else            tmem_dealloc(t, 512);
 }
-// A prediction's exponential below the largest of its row: exp(-inf - -inf) and exp(inf - inf) count as 1.
-__device__ __forceinline__ float exp_below(float z, float top) { return z == top ? 1.f : expf(z - top); }
-
 // ------------------------------------------------------------------ epilogues
-// acc: kCols columns from col0 on of row `row` (a lane's), the same columns of the rows row0 + 0 .. 31 in the warp.
+// acc: kCols columns from col0 on of row `row` (a lane's); the warp has the same columns of the rows row0 + 0 .. 31.  Global memory is read and written by rows
+// of 128 bytes, eight lanes each, and turned into a row per lane in the warp's patch: 32 rows of eight 16-byte places, place c of row r at c ^ (r % 8), so
+// that both ways are free of conflicts.
+__device__ __forceinline__ uint4& patch_at(float* patch, int row, int place) { return ((uint4*)patch)[row * 8 + (place ^ (row & 7))]; }
+
+// Rows of 64 halves or 32 floats, `pitch` bytes apart, into or out of a lane's eight uint4; rows: those that exist.
+__device__ __forceinline__ void load_rows(uint4 (&v)[8], char const* from, long long pitch, int rows, float* patch)
+{
+  int const lane = threadIdx.x & 31, r0 = lane >> 3, c = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = r0 + 4 * i < rows ? *(uint4 const*)(from + (r0 + 4 * i) * pitch + 16 * c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) patch_at(patch, r0 + 4 * i, c) = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = patch_at(patch, lane, i);
+  __syncwarp();
+}
+__device__ __forceinline__ void store_rows(uint4 const (&v)[8], char* to, long long pitch, int rows, float* patch)
+{
+  int const lane = threadIdx.x & 31, r0 = lane >> 3, c = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) patch_at(patch, lane, i) = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint4 const q = patch_at(patch, r0 + 4 * i, c);
+    if (r0 + 4 * i < rows) *(uint4*)(to + (r0 + 4 * i) * pitch + 16 * c) = q;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ uint32_t two_halves(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16); }
+
+// 64 neighbouring values of a row per lane, scaled, into a pair.
+__device__ __forceinline__ void store_pair64(Pair const& to, int row0, int col, int rows, float const* v, float* patch)
+{
+  uint4 hi[8], lo[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    __half h[8], l[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) vlb::pair_of(v[8 * i + k], h[k], l[k]);
+    hi[i] = make_uint4(two_halves(h[0], h[1]), two_halves(h[2], h[3]), two_halves(h[4], h[5]), two_halves(h[6], h[7]));
+    lo[i] = make_uint4(two_halves(l[0], l[1]), two_halves(l[2], l[3]), two_halves(l[4], l[5]), two_halves(l[6], l[7]));
+  }
+  store_rows(hi, (char*)(to.hi + row0 * to.ld + col), to.ld * 2, rows, patch);
+  store_rows(lo, (char*)(to.lo + row0 * to.ld + col), to.ld * 2, rows, patch);
+}
+
+// out = combine(out or 0, value) for the columns of a tile, whatever the alignment of out.
+template <int kCols, class F>
+__device__ __forceinline__ void update_rows(float* out, long long ldc, int M, int N, bool readOld, float const (&acc)[kCols], int row0, int col0, float* patch, F combine)
+{
+  int const lane = threadIdx.x & 31, rows = min(32, M - row0);
+  bool const vec = ((uintptr_t)out & 15) == 0 && (ldc & 3) == 0;
+#pragma unroll
+  for (int g = 0; g < kCols / 32; ++g) {
+    int const c0 = col0 + g * 32;
+    float* const o = out + row0 * ldc + c0;
+    if (vec && c0 + 32 <= N) {
+      uint4 q[8];
+      if (readOld) load_rows(q, (char const*)o, ldc * 4, rows, patch);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        auto one = [&](uint32_t old, int k) { return __float_as_uint(combine(readOld ? __uint_as_float(old) : 0.f, acc[g * 32 + 4 * i + k])); };
+        q[i] = make_uint4(one(q[i].x, 0), one(q[i].y, 1), one(q[i].z, 2), one(q[i].w, 3));
+      }
+      store_rows(q, (char*)o, ldc * 4, rows, patch);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = acc[g * 32 + i];
+      __syncwarp();
+      if (c0 + lane < N)
+        for (int r = 0; r < rows; r += 8) {
+          float old[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) old[i] = readOld && r + i < rows ? o[(r + i) * ldc + lane] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) if (r + i < rows) o[(r + i) * ldc + lane] = combine(old[i], patch[(r + i) * 33 + lane]);
+        }
+      __syncwarp();
+    }
+  }
+}
+
 template <int kCols>
 __device__ __forceinline__ void finish_out(Product const& p, float (&acc)[kCols], int row0, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  int const lane = threadIdx.x & 31;
   float const fa = pow2(-exp_of(e.ea)), fb = pow2(-exp_of(e.eb)), alpha = e.alpha;
-  int const rows = min(32, p.M - row0);
-#pragma unroll
-  for (int g = 0; g < kCols / 32; ++g) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = acc[g * 32 + i];
-    __syncwarp();
-    int const c = col0 + g * 32 + lane;
-    if (c < p.N) {
-      float* const o = e.out + (long long)row0 * e.ldc + c;
-      if (e.beta != 0.f) {
-        for (int r = 0; r < rows; r += 8) {
-          float old[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) if (r + i < rows) old[i] = o[(r + i) * e.ldc];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) if (r + i < rows) o[(r + i) * e.ldc] = patch[(r + i) * 33 + lane] * fa * fb * alpha + old[i];
-        }
-      } else {
-#pragma unroll 8
-        for (int r = 0; r < rows; ++r) o[r * e.ldc] = patch[r * 33 + lane] * fa * fb * alpha;
-      }
-    }
-    __syncwarp();
-  }
+  update_rows(e.out, e.ldc, p.M, p.N, e.beta != 0.f, acc, row0, col0, patch, [&](float old, float v) { return v * fa * fb * alpha + old; });
 }
 
-// predictions = product + bias in place, -inf beyond the last column
+// predictions = product + bias in place, -inf beyond the last column.  The columns' biases go through the warp's patch: loaded side by side, read by all lanes.
 template <int kCols>
-__device__ __forceinline__ void predictions(Product const& p, float (&acc)[kCols], int col0)
+__device__ __forceinline__ void predictions(Product const& p, float (&acc)[kCols], int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
   float const fa = pow2(-exp_of(e.ea)), fb = pow2(-exp_of(e.eb));
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    float const z = acc[i] * fa * fb;
-    acc[i] = col0 + i < p.N ? (e.bias ? z + __ldg(e.bias + col0 + i) : z) : -INFINITY;
+  for (int i = 0; i < kCols; i += 32) {
+    int const c = col0 + i + (int)(threadIdx.x & 31);
+    patch[i + (threadIdx.x & 31)] = c < p.N ? (e.bias ? __ldg(e.bias + c) : 0.f) : -INFINITY;
   }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kCols; i += 4) {
+    float4 const b = *(float4 const*)(patch + i);
+    acc[i] = fmaf(acc[i] * fa, fb, b.x); acc[i + 1] = fmaf(acc[i + 1] * fa, fb, b.y);
+    acc[i + 2] = fmaf(acc[i + 2] * fa, fb, b.z); acc[i + 3] = fmaf(acc[i + 3] * fa, fb, b.w);
+  }
+  __syncwarp();
 }
 
 template <int kCols>
-__device__ __forceinline__ void finish_seen(Product const& p, float (&acc)[kCols], int row, int col0)
+__device__ __forceinline__ void finish_seen(Product const& p, float (&acc)[kCols], int row, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  predictions(p, acc, col0);
-  if (row >= p.M) return;
+  predictions(p, acc, col0, patch);
+  bool const in = row < p.M;
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kCols; ++i) top = fmaxf(top, acc[i]);
+  // an infinite largest value is none to subtract: the exponentials below it are then 0 or infinite, as the definition has them
+  float const base = isinf(top) ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) if (col0 + i < p.N) sum += exp_below(acc[i], top);
-  e.parts[(long long)(col0 / kCols) * p.M + row] = make_float2(top, sum);
-  int const at = min(max((int)__ldg(e.labels + row) - 1, 0), e.classes - 1) - e.firstClass - col0;
-  if (at >= 0 && at < kCols && col0 + at < p.N) {
+  for (int i = 0; i < kCols; ++i) sum += __expf(acc[i] - base);
+  if (in) e.parts[(long long)(col0 / kCols) * p.M + row] = make_float2(top, sum);
+  int const at = in ? min(max((int)__ldg(e.labels + row) - 1, 0), e.classes - 1) - e.firstClass - col0 : -1;
+  bool const here = at >= 0 && at < kCols && col0 + at < p.N;
+  if (__any_sync(0xffffffffu, here)) {
     float z = 0.f;
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) if (i == at) z = acc[i];
-    e.label[row] = z;
+    for (int i = 0; i < kCols; ++i) z = i == at ? acc[i] : z;
+    if (here) e.label[row] = z;
   }
 }
 
@@ -229,19 +303,20 @@ __device__ __forceinline__ float lane_sums(float (&v)[32])
 }
 
 template <int kCols>
-__device__ __forceinline__ void finish_grad(Product const& p, float (&acc)[kCols], int row0, int row, int col0)
+__device__ __forceinline__ void finish_grad(Product const& p, float (&acc)[kCols], int row0, int row, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  predictions(p, acc, col0);
+  predictions(p, acc, col0, patch);
   bool const in = row < p.M;
   float const l = in ? __ldg(e.labels + row) : 0.f, lse = in ? __ldg(e.lse + row) : 0.f;
   bool const real = l > 0.f && l <= (float)e.classes;
   if (l > (float)e.classes && e.status) atomicExch(e.status, kStatusBadLabel);
   int const at = min(max((int)l - 1, 0), e.classes - 1) - e.firstClass - col0;
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    float const v = expf(acc[i] - lse) - (i == at ? 1.f : 0.f);
-    acc[i] = real && col0 + i < p.N ? v : 0.f;
+  for (int i = 0; i < kCols; ++i) acc[i] = real ? __expf(acc[i] - lse) : 0.f;
+  if (__any_sync(0xffffffffu, real && at >= 0 && at < kCols)) {
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) acc[i] -= real && i == at ? 1.f : 0.f;
   }
   if (e.db) {
 #pragma unroll
@@ -257,78 +332,51 @@ __device__ __forceinline__ void finish_grad(Product const& p, float (&acc)[kCols
   float const f = pow2(e.toExp);
 #pragma unroll
   for (int i = 0; i < kCols; ++i) acc[i] *= f;
-  if (!in) return;
 #pragma unroll
-  for (int i = 0; i < kCols; i += 16)
-    if (col0 + i < e.to.ld) store_pair16(e.to, row, col0 + i, &acc[i]);
+  for (int i = 0; i < kCols; i += 64)
+    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, min(32, p.M - row0), &acc[i], patch);
 }
 
 template <int kCols>
-__device__ __forceinline__ void finish_poly(Product const& p, float (&acc)[kCols], int row0, int row, int col0, bool mirror, float* patch)
+__device__ __forceinline__ void finish_poly(Product const& p, float (&acc)[kCols], int row0, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  bool const in = row < p.M;
+  int const rows = min(32, p.M - row0);
   float const f = e.alpha * pow2(-exp_of(e.ea)) * pow2(-exp_of(e.eb));
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) acc[i] *= f;
   if (e.beta != 0.f) {
-    float const fadd = e.beta * pow2(-e.addExp);
+    float const fh = e.beta * pow2(-e.addExp), fl = fh * (1.f / 2048.f);
+    auto two = [&](uint32_t w, float k, float& a, float& b) {
+      float2 const v = __half22float2(*(__half2 const*)&w);
+      a = fmaf(v.x, k, a); b = fmaf(v.y, k, b);
+    };
 #pragma unroll
-    for (int i = 0; i < kCols; i += 16) {
-      uint32_t hi[8] = {}, lo[8] = {};
-      if (in && col0 + i < e.add.ld) {
-        load32(e.add.hi + row * e.add.ld + col0 + i, hi);
-        load32(e.add.lo + row * e.add.ld + col0 + i, lo);
-      }
+    for (int i = 0; i < kCols; i += 64) {
+      if (col0 + i >= e.add.ld) continue;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        __half const h = __ushort_as_half((unsigned short)(hi[j / 2] >> (j % 2 * 16))), l = __ushort_as_half((unsigned short)(lo[j / 2] >> (j % 2 * 16)));
-        acc[i + j] = f * acc[i + j] + fadd * vlb::pair_value(h, l);
-      }
-    }
-  } else {
+      for (int part = 0; part < 2; ++part) {
+        uint4 q[8];
+        load_rows(q, (char const*)((part ? e.add.lo : e.add.hi) + row0 * e.add.ld + col0 + i), e.add.ld * 2, rows, patch);
+        float const k = part ? fl : fh;
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) acc[i] *= f;
-  }
-  if (e.out) {
-    int const lane = threadIdx.x & 31, rows = min(32, p.M - row0);
-#pragma unroll
-    for (int g = 0; g < kCols / 32; ++g) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) patch[lane * 33 + i] = acc[g * 32 + i];
-      __syncwarp();
-      int const c = col0 + g * 32 + lane;
-      if (c < p.N) {
-        float* const o = e.out + (long long)row0 * e.ldc + c;
-        for (int r = 0; r < rows; r += 8) {
-          float old[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) if (r + i < rows) old[i] = o[(r + i) * e.ldc];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) if (r + i < rows) o[(r + i) * e.ldc] = old[i] - e.rate * patch[(r + i) * 33 + lane];
+        for (int c = 0; c < 8; ++c) {
+          two(q[c].x, k, acc[i + 8 * c], acc[i + 8 * c + 1]); two(q[c].y, k, acc[i + 8 * c + 2], acc[i + 8 * c + 3]);
+          two(q[c].z, k, acc[i + 8 * c + 4], acc[i + 8 * c + 5]); two(q[c].w, k, acc[i + 8 * c + 6], acc[i + 8 * c + 7]);
         }
       }
-      __syncwarp();
     }
+  }
+  if (e.out) {
+    update_rows(e.out, e.ldc, p.M, p.N, true, acc, row0, col0, patch, [&](float old, float v) { return old - e.rate * v; });
     return;
   }
   float const ft = pow2(e.toExp);
 #pragma unroll
   for (int i = 0; i < kCols; ++i) acc[i] *= ft;
-  if (!in) return;
 #pragma unroll
-  for (int i = 0; i < kCols; i += 16)
-    if (col0 + i < e.to.ld) store_pair16(e.to, row, col0 + i, &acc[i]);
-  if (mirror) {
-    // 32 lanes, 32 neighbouring elements of a row of the mirror image
-#pragma unroll
-    for (int i = 0; i < kCols; ++i) {
-      __half h, l;
-      vlb::pair_of(acc[i], h, l);
-      if (col0 + i < p.N) {
-        e.to.hi[(col0 + i) * e.to.ld + row] = h;
-        e.to.lo[(col0 + i) * e.to.ld + row] = l;
-      }
-    }
-  }
+  for (int i = 0; i < kCols; i += 64)
+    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, rows, &acc[i], patch);
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -347,7 +395,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
   int const first = (int)blockIdx.x / kCtas, stride = (int)gridDim.x / kCtas;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&full[i]), 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&full[i]), 2);
     for (int i = 0; i < kRing; ++i) mbar_init(smem_u32(&done[i]), 1);
     for (int i = 0; i < kAcc; ++i) mbar_init(smem_u32(&empty[i]), kDrainWarps * kCtas);
     mbar_init(smem_u32(&last), 1);
@@ -423,39 +471,34 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
       }
       int const row0 = t.tm * kTileRows + (int)rank * 128 + quarter * 32, col0 = t.tn * kTileCols + half * kCols;
       if (kKind == kPairOut)  finish_out(p, acc, row0, col0, patch);
-      if (kKind == kPairSeen) finish_seen(p, acc, row0 + lane, col0);
-      if (kKind == kPairGrad) finish_grad(p, acc, row0, row0 + lane, col0);
-      if (kKind == kPairPoly) finish_poly(p, acc, row0, row0 + lane, col0, p.symmetric && t.tn < t.tm, patch);
+      if (kKind == kPairSeen) finish_seen(p, acc, row0 + lane, col0, patch);
+      if (kKind == kPairGrad) finish_grad(p, acc, row0, row0 + lane, col0, patch);
+      if (kKind == kPairPoly) finish_poly(p, acc, row0, col0, patch);
     }
     if (dead && lane == 0) atomicCAS(batch.status, 0, 42);
   } else {
     if (kCtas == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 8) {
+    if (warp == 8 || warp == 10) {
       if (lane == 0) {
+        bool const isA = warp == 8;
         int it = 0;
-        uint32_t const bytes = (batch.three ? 4u : 2u) * kHalfTile;
+        uint32_t const bytes = (batch.three ? 2u : 1u) * kHalfTile;
         for (int w = first; w < batch.work && !dead; w += stride) {
           Item const t = item_of(batch, w);
           Product const& p = batch.p[t.prod];
-          CUtensorMap const* const map = batch.map + 4 * t.prod;
-          int const a0 = t.tm * kTileRows + (int)rank * 128, b0 = t.tn * kTileCols + (int)rank * 128;
-          for (int kb = t.kb0; kb < t.kb1 && !dead; ++kb, ++it) {
+          int const tile = isA ? t.tm : t.tn, byCols = isA ? p.byColsA : p.byColsB, lower = isA ? p.lowerA : p.lowerB, r0 = tile * kTileRows + (int)rank * 128;
+          CUtensorMap const* const map = batch.map + 4 * t.prod + (isA ? 0 : 2);
+          for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
             int const s = it % kStages, before = it - kStages;
             if (before >= 0 && !mbar_wait(smem_u32(&done[before % kRing]), (uint32_t)(before / kRing) & 1u)) { dead = true; break; }
             uint32_t const mine = smem_u32(&full[s]), bar = kCtas == 2 ? in_first(mine) : mine;
             if (rank == 0) mbar_arrive_expect_tx(mine, bytes * kCtas);
-            uint32_t const dst = base + (uint32_t)s * kStageBytes;
-  #pragma unroll
-            for (int part = 0; part < 4; ++part) {
-              if ((part & 1) && !batch.three) continue;
-              uint32_t const to = dst + (uint32_t)part * kHalfTile;
-              int const r0 = part < 2 ? a0 : b0;
-              if (part < 2 ? p.byColsA : p.byColsB) {
-                load_box<kCtas>(to, map + part, r0, kb * kDepth, bar);
-                load_box<kCtas>(to + kHalfTile / 2, map + part, r0 + 64, kb * kDepth, bar);
-              } else {
-                load_box<kCtas>(to, map + part, kb * kDepth, r0, bar);
-              }
+            uint32_t const to = base + (uint32_t)s * kStageBytes + (isA ? 0u : 2u * kHalfTile);
+            if (along_cols(byCols, lower, tile, kTileRows, kb)) {
+              load_box<kCtas>(to, map + 1, r0, kb * kDepth, bar);
+              load_box<kCtas>(to + kHalfTile, map + 1, r0 + 64, kb * kDepth, bar);
+            } else {
+              load_box<kCtas>(to, map, kb * kDepth, r0, bar);
             }
           }
         }
@@ -466,33 +509,43 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
       }
     } else if (warp == 9) {
       if (lane == 0 && rank == 0) {
+        // k-block j has its operands and an accumulator
+        auto ready = [&](int j) {
+          return mbar_wait(smem_u32(&full[j % kStages]), (uint32_t)(j / kStages) & 1u) &&
+                 (j < kAcc || mbar_wait(smem_u32(&empty[j % kAcc]), (uint32_t)(j / kAcc - 1) & 1u));
+        };
         int j = 0;
+        if (first < batch.work) dead = !ready(0);
         for (int w = first; w < batch.work && !dead; w += stride) {
           Item const t = item_of(batch, w);
           Product const& p = batch.p[t.prod];
-          uint32_t const idesc = (1u << 4) | (p.byColsA ? 1u << 15 : 0u) | (p.byColsB ? 1u << 16 : 0u) | ((uint32_t)(kTileCols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
-          uint32_t const lboA = p.byColsA ? kHalfTile / 2 : 16, lboB = p.byColsB ? kHalfTile / 2 : 16;
-          uint64_t const stepA = (p.byColsA ? 2048u : 32u) >> 4, stepB = (p.byColsB ? 2048u : 32u) >> 4;
-          for (int kb = t.kb0; kb < t.kb1; ++kb, ++j) {
+          for (int kb = t.kb0; kb < t.kb1 && !dead; ++kb, ++j) {
             int const s = j % kStages, acc = j % kAcc;
-            if (!mbar_wait(smem_u32(&full[s]), (uint32_t)(j / kStages) & 1u)) { dead = true; break; }
-            if (j >= kAcc && !mbar_wait(smem_u32(&empty[acc]), (uint32_t)(j / kAcc - 1) & 1u)) { dead = true; break; }
+            // the next k-block is waited for when the tensor core still has the end of this one to work on: 250 cycles per k-block
+            bool const more = kb + 1 < t.kb1 || w + stride < batch.work;
             tc_fence_after();
             uint32_t const st = base + (uint32_t)s * kStageBytes, d = tmem + (uint32_t)(acc * kTileCols);
-            uint64_t const aH = make_desc(st, lboA, 1024), aL = make_desc(st + kHalfTile, lboA, 1024);
-            uint64_t const bH = make_desc(st + 2 * kHalfTile, lboB, 1024), bL = make_desc(st + 3 * kHalfTile, lboB, 1024);
+            bool const ca = along_cols(p.byColsA, p.lowerA, t.tm, kTileRows, kb), cb = along_cols(p.byColsB, p.lowerB, t.tn, kTileCols, kb);
+            uint32_t const idesc = (1u << 4) | (ca ? 1u << 15 : 0u) | (cb ? 1u << 16 : 0u) | ((uint32_t)(kTileCols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
+            uint64_t const stepA = (ca ? 2048u : 32u) >> 4, stepB = (cb ? 2048u : 32u) >> 4;
+            uint64_t const aH = make_desc(st, kHalfTile, 1024), aL = aH + ((ca ? kHalfTile / 2 : kHalfTile) >> 4);
+            uint64_t const bH = make_desc(st + 2 * kHalfTile, kHalfTile, 1024), bL = bH + ((cb ? kHalfTile / 2 : kHalfTile) >> 4);
             if (batch.three) {
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < kDepth / 16; ++k) {
                 mma<kCtas>(d, aL + stepA * k, bH + stepB * k, idesc, k > 0 ? 1u : 0u);
                 mma<kCtas>(d, aH + stepA * k, bL + stepB * k, idesc, 1u);
               }
               mma_scaled<kCtas>(d, aH, bH, idesc);
-  #pragma unroll
+              if (more) dead = !ready(j + 1);
+#pragma unroll
               for (int k = 1; k < kDepth / 16; ++k) mma<kCtas>(d, aH + stepA * k, bH + stepB * k, idesc, 1u);
             } else {
-  #pragma unroll
-              for (int k = 0; k < kDepth / 16; ++k) mma<kCtas>(d, aH + stepA * k, bH + stepB * k, idesc, k > 0 ? 1u : 0u);
+#pragma unroll
+              for (int k = 0; k < kDepth / 16; ++k) {
+                mma<kCtas>(d, aH + stepA * k, bH + stepB * k, idesc, k > 0 ? 1u : 0u);
+                if (k == 0 && more) dead = !ready(j + 1);
+              }
             }
             commit<kCtas>(smem_u32(&done[j % kRing]));
           }
@@ -593,16 +646,21 @@ make_pair_kernel(Pair to, float const* __restrict__ x, unsigned const* __restric
 }
 
 // ------------------------------------------------------------------ host
-bool encode_side(CUtensorMap* hi, CUtensorMap* lo, vlb::PairSide const& s)
+// The maps of a side, along its rows and along its columns: hi and lo (or hi alone) in one copy.
+bool encode_side(CUtensorMap* map, vlb::PairSide const& s, bool three)
 {
   EncodeTiledFn const encode = encode_tiled();
   if (!encode) return false;
-  cuuint64_t const dims[2] = {(cuuint64_t)s.m.cols, (cuuint64_t)s.m.rows}, strides[1] = {(cuuint64_t)s.m.ld * 2};
-  cuuint32_t const box[2] = {64, s.byCols ? 64u : 128u}, one[2] = {1, 1};
-  for (int part = 0; part < 2; ++part)
-    if (encode(part ? lo : hi, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, part ? s.m.lo : s.m.hi, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t const dims[3] = {(cuuint64_t)s.m.cols, (cuuint64_t)s.m.rows, 2};
+  cuuint64_t const strides[2] = {(cuuint64_t)s.m.ld * 2, (cuuint64_t)((char*)s.m.lo - (char*)s.m.hi)};
+  cuuint32_t const one[3] = {1, 1, 1};
+  for (int along = 0; along < 2; ++along) {
+    if (!(along ? s.byCols || s.lower : !s.byCols)) continue;
+    cuuint32_t const box[3] = {64, along ? 64u : 128u, three ? 2u : 1u};
+    if (encode(map + along, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, s.m.hi, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return false;
+  }
   return true;
 }
 
@@ -617,6 +675,7 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
 {
   constexpr int kTile = 128 * kCtas;
   Batch<kMax> b;
+  b.three = ctx->precision != VLB_PRECISION_TF32;
   int const clusters = ctx->smCount / kCtas;
   long long tiles = 0, blocks = 0;
   for (int i = 0; i < count; ++i) {
@@ -644,13 +703,13 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
     if (d.splits > 1) { slot += t; part += (long long)t * d.splits; }
     work += (long long)t * d.splits;
     d.work = (int)work;
-    d.byColsA = q.a.byCols; d.byColsB = q.b.byCols; d.symmetric = q.symmetric;
+    d.byColsA = q.a.byCols; d.byColsB = q.b.byCols; d.lowerA = q.a.lower; d.lowerB = q.b.lower; d.symmetric = q.symmetric;
     d.e = q.e;
-    if (!encode_side(&b.map[4 * i], &b.map[4 * i + 1], q.a) || !encode_side(&b.map[4 * i + 2], &b.map[4 * i + 3], q.b))
+    if (!encode_side(&b.map[4 * i], q.a, b.three) || !encode_side(&b.map[4 * i + 2], q.b, b.three))
       return vlb::set_error(ctx, VLB_Cuda, "a tensor map could not be made");
   }
   if (work > INT32_MAX) return vlb::set_error(ctx, VLB_IllegalArgument, "the matrices are too large");
-  b.count = count; b.work = (int)work; b.three = ctx->precision != VLB_PRECISION_TF32;
+  b.count = count; b.work = (int)work;
   b.split = (float*)split;
   b.tickets = ctx->deviceStatus + 64;
   b.status = ctx->deviceStatus;
@@ -677,25 +736,10 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
   return vlb::check_launch(ctx, "products_of_pairs");
 }
 
-// Whether pairs of CTAs take less time, by k-blocks through the tensor core: 1536 cycles for 256 x 256 on two SMs, 768 for 128 x 128 on one, and a hand-over
-// between k-blocks that a pair's longer ones hide.
-bool pairs_pay(vlb_ctx* ctx, PairProduct const* p, int count)
-{
-  double two = 0, one = 0;
-  for (int i = 0; i < count; ++i) {
-    double const kb = vlb::ceil_div(p[i].K, kDepth);
-    two += tiles_of(p[i], 256) * kb;
-    one += tiles_of(p[i], 128) * kb;
-  }
-  return two / (ctx->smCount / 2) * 1600. <= one / ctx->smCount * 950.;
-}
-
 template <int kKind, int kMax>
-int run_kind(vlb_ctx* ctx, PairProduct const* p, int count, void* split, int* parts)
+int run_kind(vlb_ctx* ctx, PairProduct const* p, int count, void* split, int tile)
 {
-  bool const two = pairs_pay(ctx, p, count);
-  if (parts) *parts = 2 * vlb::ceil_div(p->N, two ? 256 : 128);
-  return two ? run<kKind, kMax, 2>(ctx, p, count, split) : run<kKind, kMax, 1>(ctx, p, count, split);
+  return tile == 256 ? run<kKind, kMax, 2>(ctx, p, count, split) : run<kKind, kMax, 1>(ctx, p, count, split);
 }
 
 }  // namespace
@@ -718,13 +762,26 @@ void make_pair(vlb_ctx* ctx, Pair to, float const* x, unsigned const* largest, f
   VLB_LAUNCHED(ctx, 1);
 }
 
-int products_of_pairs(vlb_ctx* ctx, PairKind kind, PairProduct const* p, int count, void* split, int* parts)
+// By k-blocks through the tensor core: 1536 cycles for 256 x 256 on two SMs, 768 for 128 x 128 on one, and a hand-over between k-blocks that a pair's longer
+// ones hide.
+int pair_tile(vlb_ctx* ctx, PairProduct const* p, int count)
+{
+  double two = 0, one = 0;
+  for (int i = 0; i < count; ++i) {
+    double const kb = ceil_div(p[i].K, kDepth);
+    two += tiles_of(p[i], 256) * kb;
+    one += tiles_of(p[i], 128) * kb;
+  }
+  return two / (ctx->smCount / 2) * 1600. <= one / ctx->smCount * 950. ? 256 : 128;
+}
+
+int products_of_pairs(vlb_ctx* ctx, PairKind kind, PairProduct const* p, int count, void* split, int tile)
 {
   switch (kind) {
-    case kPairOut:  return run_kind<kPairOut, 2>(ctx, p, count, split, parts);
-    case kPairSeen: return run_kind<kPairSeen, 1>(ctx, p, count, split, parts);
-    case kPairGrad: return run_kind<kPairGrad, 1>(ctx, p, count, split, parts);
-    default:        return count > 1 ? run_kind<kPairPoly, kMaxPairProducts>(ctx, p, count, split, parts) : run_kind<kPairPoly, 1>(ctx, p, count, split, parts);
+    case kPairOut:  return run_kind<kPairOut, 2>(ctx, p, count, split, tile);
+    case kPairSeen: return run_kind<kPairSeen, 1>(ctx, p, count, split, tile);
+    case kPairGrad: return run_kind<kPairGrad, 1>(ctx, p, count, split, tile);
+    default:        return count > 1 ? run_kind<kPairPoly, kMaxPairProducts>(ctx, p, count, split, tile) : run_kind<kPairPoly, 1>(ctx, p, count, split, tile);
   }
 }
 

@@ -22,8 +22,9 @@ inline Pair pair_at(void* p, int rows, int cols)
   return {(__half*)p, (__half*)p + (size_t)rows * ld, rows, cols, ld};
 }
 
-// A side of a product: its rows are the matrix's rows and the reduction runs along the columns, or (byCols) the other way round.
-struct PairSide { Pair m; bool byCols; };
+// A side of a product: its rows are the matrix's rows and the reduction runs along the columns, or (byCols) the other way round.  lower: of a symmetric
+// matrix only the tiles on and under the diagonal are there, as a symmetric product with the same tiles left them.
+struct PairSide { Pair m; bool byCols, lower; };
 
 // The exponent e of a pair: that of the largest magnitude, whose bits are in a word on the device, or a number.
 struct PairExp { unsigned const* largest; int value; };
@@ -51,26 +52,28 @@ struct PairEpilogue {
 struct PairProduct {
   PairSide a, b;
   int M, N, K;
-  bool symmetric;                   // kPairPoly: the product is symmetric; tiles right of the diagonal are written from their mirror images
+  bool symmetric;                   // the product is symmetric: only the tiles on and under the diagonal are made
   PairEpilogue e;
 };
 
 constexpr int kMaxPairProducts = 16;
-constexpr int kPairTile = 256;      // columns of kPairSeen's parts: two parts for each 256 or, with small tiles, each 128 of them
 
 // Scratch for the partial results of reductions that are cut, at most.
 constexpr size_t kPairSplitBytes = 64u << 20;
 
-// What kPairSeen writes per row: parts of products of N columns, at most.
-inline int pair_parts(int N) { return 2 * ceil_div(N, 128); }
+// Parts per row that kPairSeen writes of N columns.
+inline int pair_parts(int N, int tile) { return 2 * ceil_div(N, tile); }
 
 // The largest finite magnitude of rows x cols floats one after the other, as bits, into *largest, which holds zero or an earlier result; and that matrix as
 // a pair with the exponent of *largest.  labels (or NULL): rows whose label is not in 1 ... classes count as zeros, whatever they hold.
 void largest_of(vlb_ctx* ctx, unsigned* largest, float const* x, int rows, int cols, float const* labels, int classes);
 void make_pair(vlb_ctx* ctx, Pair to, float const* x, unsigned const* largest, float const* labels, int classes);
 
-// All products of one kind in one launch.  split: kPairSplitBytes of scratch, 16-byte aligned.  parts, where given, gets the number of parts per row of kPairSeen.
-int products_of_pairs(vlb_ctx* ctx, PairKind kind, PairProduct const* p, int count, void* split, int* parts = nullptr);
+// The tiles, 256 x 256 or 128 x 128, that take less time for these products, all of them together.
+int pair_tile(vlb_ctx* ctx, PairProduct const* p, int count);
+
+// All products of one kind in one launch, with tiles of `tile` rows and columns.  split: kPairSplitBytes of scratch, 16-byte aligned.
+int products_of_pairs(vlb_ctx* ctx, PairKind kind, PairProduct const* p, int count, void* split, int tile);
 
 #ifdef __CUDACC__
 // 32 bytes at once, 32-byte aligned
@@ -78,11 +81,6 @@ __device__ __forceinline__ void store32(void* p, uint32_t const (&v)[8])
 {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-__device__ __forceinline__ void load32(void const* p, uint32_t (&v)[8])
-{
-  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p) : "memory");
-}
-
 // The exponent that brings the magnitude m into [2^14, 2^15); at most 116, so that 2^e and its inverse are normal numbers.
 __device__ __forceinline__ int pair_exp(float m) { return m > 0.f ? min(141 - (int)(__float_as_uint(m) >> 23), 116) : 0; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }        // -126 <= e <= 127
@@ -111,7 +109,6 @@ __device__ __forceinline__ void store_pair16(Pair const& to, long long row, int 
   store32(to.hi + row * to.ld + col, hi);
   store32(to.lo + row * to.ld + col, lo);
 }
-__device__ __forceinline__ float pair_value(__half hi, __half lo) { return fmaf(__half2float(lo), 1.f / 2048.f, __half2float(hi)); }
 #endif
 
 }  // namespace vlb
