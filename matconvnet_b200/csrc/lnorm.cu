@@ -1,85 +1,471 @@
-// Layer normalisation over the channels of a position (include/vlb.h has the formulas).
+// Layer normalisation over the channels of a position (include/vlb.h has the formulas) -- HBM bound: 8 bytes per value forward, 12 backward.
+//
+// A position's values are read once and held in registers through all passes over them: the mean, then the sum of squared differences from it (backward
+// together with the two sums of the derivative), then the result.  One position per image (tokens; P = 1): a position is a run of C floats and belongs to a warp or
+// a block.  Maps (P > 1): values of a position lie P floats apart, so that 32 neighbouring positions belong to a block, one per lane, and its warps share the
+// channels.  Both count positions through the batch.  What does not fit the registers is read again for each pass, from L2.
+//
+// The sums over positions (dG, dB) are kept per channel by the threads that see it; each block leaves its part, and a second kernel adds the parts in order.
 #include "common.cuh"
+#include <algorithm>
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMaxParts = 148 * 4;      // blocks of a backward pass, at most
 
-// Sum of a and of b over the block, in every thread; red: 2 * 32 floats of shared memory.
-__device__ __forceinline__ float2 block_sum2(float a, float b, float2* red)
+__device__ __forceinline__ float warp_sum(float v)
 {
-  for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(a, b);
-  __syncthreads();
-  float2 s = make_float2(0.f, 0.f);
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) { s.x += red[i].x; s.y += red[i].y; }
-  return s;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-struct Moments { float mean, r; };
-
-__device__ __forceinline__ Moments moments_of(float const* x, size_t P, int C, float eps, float2* red)
+// Sums over the kThreads threads of a row, in each of them; red: [kCount][32] floats, not in use by an earlier call's readers any more.
+template <int kThreads, int kCount>
+__device__ __forceinline__ void row_sums(float (&v)[kCount], float (*red)[32])
 {
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) v[k] = warp_sum(v[k]);
+  if (kThreads == 32) return;
+  int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) {
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) red[k][warp] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) v[k] = warp_sum(lane < kThreads / 32 ? red[k][lane] : 0.f);
+}
+
+// ------------------------------------------------------------------ positions that are rows
+// A row belongs to kThreads threads, each with kVec times four neighbouring channels (kWide) or 4 kVec channels kThreads apart.
+template <int kThreads, int kVec, bool kWide>
+struct Row {
+  static constexpr int kValues = 4 * kVec;
+  static __device__ __forceinline__ int channel(int i)
+  {
+    int const t = threadIdx.x % kThreads;
+    return kWide ? 4 * (t + kThreads * (i / 4)) + i % 4 : t + kThreads * i;
+  }
+  static __device__ __forceinline__ void load(float (&v)[kValues], float const* __restrict__ p, int C)
+  {
+    if (kWide) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        float4 const q = channel(4 * i) < C ? __ldg((float4 const*)(p + channel(4 * i))) : make_float4(0, 0, 0, 0);
+        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) v[i] = channel(i) < C ? __ldg(p + channel(i)) : 0.f;
+    }
+  }
+  static __device__ __forceinline__ void store(float* __restrict__ p, float const (&v)[kValues], int C)
+  {
+    if (kWide) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (channel(4 * i) < C) *(float4*)(p + channel(4 * i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) if (channel(i) < C) p[channel(i)] = v[i];
+    }
+  }
+};
+
+constexpr int block_of(int rowThreads) { return rowThreads < 128 ? 128 : rowThreads; }
+
+template <int kThreads, int kVec, bool kWide>
+__global__ void __launch_bounds__(block_of(kThreads))
+rows_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, int rows, int C, float eps)
+{
+  using R = Row<kThreads, kVec, kWide>;
+  vlb::pdl_wait();
+  __shared__ float red[2][1][32];
+  int const row = (int)blockIdx.x * (block_of(kThreads) / kThreads) + (int)threadIdx.x / kThreads;
+  if (kThreads == 32 && row >= rows) return;
+  float v[R::kValues];
+  R::load(v, x + (size_t)row * C, C);
+  float s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < R::kValues; ++i) s[0] += v[i];
+  row_sums<kThreads>(s, red[0]);
+  float const mean = s[0] / (float)C;
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < R::kValues; ++i) { v[i] -= mean; s[0] += R::channel(i) < C ? v[i] * v[i] : 0.f; }
+  row_sums<kThreads>(s, red[1]);
+  float const r = 1.f / sqrtf(s[0] / (float)C + eps);
+  float gv[R::kValues], bv[R::kValues];
+  R::load(gv, g, C);
+  R::load(bv, b, C);
+#pragma unroll
+  for (int i = 0; i < R::kValues; ++i) v[i] = fmaf(gv[i], v[i] * r, bv[i]);
+  R::store(y + (size_t)row * C, v, C);
+}
+
+// Rows in turn to the blocks (or, kThreads == 32, to the warps).  parts: [block][2][C], dG then dB.
+template <int kThreads, int kVec, bool kWide>
+__global__ void __launch_bounds__(block_of(kThreads))
+rows_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
+                int rows, int C, float eps)
+{
+  using R = Row<kThreads, kVec, kWide>;
+  constexpr int kRows = block_of(kThreads) / kThreads;
+  vlb::pdl_wait();
+  __shared__ float red[2][4][32];
+  __shared__ float other[kRows > 1 ? (kRows - 1) * 2 * 32 * R::kValues : 1];
+  float gv[R::kValues], dg[R::kValues] = {}, db[R::kValues] = {};
+  R::load(gv, g, C);
+  float const n = (float)C;
+  int even = 0;
+  for (int row = (int)blockIdx.x * kRows + (int)threadIdx.x / kThreads; row < rows; row += (int)gridDim.x * kRows, even ^= 1) {
+    float v[R::kValues], d[R::kValues];
+    R::load(v, x + (size_t)row * C, C);
+    R::load(d, dy + (size_t)row * C, C);
+    float m[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < R::kValues; ++i) m[0] += v[i];
+    row_sums<kThreads>(m, red[even] + 3);
+    float const mean = m[0] / n;
+    float s[3] = {};
+#pragma unroll
+    for (int i = 0; i < R::kValues; ++i) {
+      v[i] = R::channel(i) < C ? v[i] - mean : 0.f;
+      float const gd = gv[i] * d[i];
+      s[0] += v[i] * v[i]; s[1] += gd; s[2] += gd * v[i];
+    }
+    row_sums<kThreads>(s, red[even]);
+    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+#pragma unroll
+    for (int i = 0; i < R::kValues; ++i) {
+      float const xh = v[i] * r;
+      dg[i] += d[i] * xh; db[i] += d[i];
+      v[i] = r * (gv[i] * d[i] - m1 - xh * m2);
+    }
+    if (dx) R::store(dx + (size_t)row * C, v, C);
+  }
+  if (!parts) return;
+  if (kRows > 1) {
+    // the block's warps, added in order
+    int const w = (int)threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (w) {
+#pragma unroll
+      for (int i = 0; i < R::kValues; ++i) {
+        other[((w - 1) * 2 * R::kValues + i) * 32 + lane] = dg[i];
+        other[((w - 1) * 2 * R::kValues + R::kValues + i) * 32 + lane] = db[i];
+      }
+    }
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int i = 0; i < R::kValues; ++i)
+      for (int k = 0; k < kRows - 1; ++k) {
+        dg[i] += other[(k * 2 * R::kValues + i) * 32 + lane];
+        db[i] += other[(k * 2 * R::kValues + R::kValues + i) * 32 + lane];
+      }
+  }
+  float* const p = parts + (size_t)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int i = 0; i < R::kValues; ++i)
+    if (R::channel(i) < C) { p[R::channel(i)] = dg[i]; p[C + R::channel(i)] = db[i]; }
+}
+
+// Rows of any length, a block per row: the values are read again for each pass, the block's sums over rows are kept in parts themselves.
+__global__ void __launch_bounds__(1024)
+rows_fwd_long_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, int C, float eps)
+{
+  vlb::pdl_wait();
+  __shared__ float red[2][1][32];
+  float const* const xp = x + (size_t)blockIdx.x * C;
+  float s[1] = {0.f};
+#pragma unroll 8
+  for (int c = threadIdx.x; c < C; c += 1024) s[0] += __ldg(xp + c);
+  row_sums<1024>(s, red[0]);
+  float const mean = s[0] / (float)C;
+  s[0] = 0.f;
+#pragma unroll 8
+  for (int c = threadIdx.x; c < C; c += 1024) { float const d = __ldg(xp + c) - mean; s[0] += d * d; }
+  row_sums<1024>(s, red[1]);
+  float const r = 1.f / sqrtf(s[0] / (float)C + eps);
+#pragma unroll 4
+  for (int c = threadIdx.x; c < C; c += 1024) y[(size_t)blockIdx.x * C + c] = fmaf(__ldg(g + c), (__ldg(xp + c) - mean) * r, __ldg(b + c));
+}
+
+__global__ void __launch_bounds__(1024)
+rows_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
+                     int rows, int C, float eps)
+{
+  vlb::pdl_wait();
+  __shared__ float red[2][4][32];
+  float const n = (float)C;
+  float* const own = parts ? parts + (size_t)blockIdx.x * 2 * C : nullptr;
+  int even = 0;
+  for (int row = blockIdx.x; row < rows; row += gridDim.x, even ^= 1) {
+    bool const first = row == (int)blockIdx.x;
+    float const *const xp = x + (size_t)row * C, *const dp = dy + (size_t)row * C;
+    float m[1] = {0.f};
+#pragma unroll 8
+    for (int c = threadIdx.x; c < C; c += 1024) m[0] += __ldg(xp + c);
+    row_sums<1024>(m, red[even] + 3);
+    float const mean = m[0] / n;
+    float s[3] = {};
+#pragma unroll 4
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      float const v = __ldg(xp + c) - mean, gd = __ldg(g + c) * __ldg(dp + c);
+      s[0] += v * v; s[1] += gd; s[2] += gd * v;
+    }
+    row_sums<1024>(s, red[even]);
+    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < C; c += 1024) {
+      float const xh = (__ldg(xp + c) - mean) * r, d = __ldg(dp + c);
+      if (dx) dx[(size_t)row * C + c] = r * (__ldg(g + c) * d - m1 - xh * m2);
+      if (own) {
+        own[c] = first ? d * xh : own[c] + d * xh;
+        own[C + c] = first ? d : own[C + c] + d;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ positions of maps
+// A block of kWarps warps takes 32 positions, a lane's is `q` of the batch; warp w has the channels w, w + kWarps, ..., kValues of them in registers (0: read
+// again for every pass).
+struct Place { size_t at; bool in; };
+
+__device__ __forceinline__ Place place_of(long long q, long long positions, int P, int C)
+{
+  bool const in = q < positions;
+  long long const t = in ? q : positions - 1, n = t / P;
+  return {(size_t)(n * P * C + (t - n * P)), in};
+}
+
+// Sums over the block's warps, lane by lane.
+template <int kWarps, int kCount>
+__device__ __forceinline__ void lane_totals(float (&v)[kCount], float (*red)[kWarps][32])
+{
+  int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) red[k][warp][lane] = v[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kCount; ++k) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += red[k][w][lane];
+    v[k] = s;
+  }
+}
+
+template <int kWarps, int kValues>
+__global__ void __launch_bounds__(kWarps * 32)
+maps_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, long long positions, int P, int C,
+                float eps)
+{
+  vlb::pdl_wait();
+  __shared__ float red[2][1][kWarps][32];
+  int const warp = threadIdx.x >> 5;
+  Place const at = place_of(blockIdx.x * 32ll + (threadIdx.x & 31), positions, P, C);
+  float const* const xp = x + at.at;
+  float* const yp = y + at.at;
+  float v[kValues > 0 ? kValues : 1], s[1] = {0.f};
+  if (kValues) {
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) { int const c = warp + kWarps * i; v[i] = c < C ? __ldg(xp + (size_t)P * c) : 0.f; }
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) s[0] += v[i];
+  } else {
+#pragma unroll 8
+    for (int c = warp; c < C; c += kWarps) s[0] += __ldg(xp + (size_t)P * c);
+  }
+  lane_totals<kWarps>(s, red[0]);
+  float const mean = s[0] / (float)C;
+  s[0] = 0.f;
+  if (kValues) {
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) { v[i] -= mean; s[0] += warp + kWarps * i < C ? v[i] * v[i] : 0.f; }
+  } else {
+#pragma unroll 8
+    for (int c = warp; c < C; c += kWarps) { float const d = __ldg(xp + (size_t)P * c) - mean; s[0] += d * d; }
+  }
+  lane_totals<kWarps>(s, red[1]);
+  float const r = 1.f / sqrtf(s[0] / (float)C + eps);
+  if (!at.in) return;
+  if (kValues) {
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) {
+      int const c = warp + kWarps * i;
+      if (c < C) yp[(size_t)P * c] = fmaf(__ldg(g + c), v[i] * r, __ldg(b + c));
+    }
+  } else {
+#pragma unroll 8
+    for (int c = warp; c < C; c += kWarps) yp[(size_t)P * c] = fmaf(__ldg(g + c), (__ldg(xp + (size_t)P * c) - mean) * r, __ldg(b + c));
+  }
+}
+
+// Sums over the lanes of kCount values (a power of two up to 32): lane l ends with the total of v[l % kCount].
+template <int kCount>
+__device__ __forceinline__ float lane_sums(float (&v)[kCount])
+{
+  int const lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = kCount / 2; s > 0; s >>= 1) {
+    bool const up = lane & s;
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      float const send = up ? v[i] : v[i + s], keep = up ? v[i + s] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
+    }
+  }
+  float t = v[0];
+#pragma unroll
+  for (int s = kCount; s < 32; s <<= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
+  return t;
+}
+
+// Tiles of 32 positions in turn to the blocks.  parts: [block][2][C].
+template <int kWarps, int kValues>
+__global__ void __launch_bounds__(kWarps * 32)
+maps_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
+                long long positions, int tiles, int P, int C, float eps)
+{
+  vlb::pdl_wait();
+  __shared__ float red[2][4][kWarps][32];
+  int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float const n = (float)C;
+  float sum = 0.f;                       // lane l: the block's dG (l < kValues) or dB of channel warp + kWarps * (l % kValues)
+  int even = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, even ^= 1) {
+    Place const at = place_of(tile * 32ll + lane, positions, P, C);
+    float const *const xp = x + at.at, *const dp = dy + at.at;
+    float v[kValues], d[kValues], m[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) { int const c = warp + kWarps * i; v[i] = c < C ? __ldg(xp + (size_t)P * c) : 0.f; }
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) { int const c = warp + kWarps * i; d[i] = c < C ? __ldg(dp + (size_t)P * c) : 0.f; }
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) m[0] += v[i];
+    lane_totals<kWarps>(m, red[even] + 3);
+    float const mean = m[0] / n;
+    float s[3] = {};
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) {
+      int const c = warp + kWarps * i;
+      v[i] = c < C ? v[i] - mean : 0.f;
+      float const gd = c < C ? __ldg(g + c) * d[i] : 0.f;
+      s[0] += v[i] * v[i]; s[1] += gd; s[2] += gd * v[i];
+    }
+    lane_totals<kWarps>(s, red[even]);
+    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+    if (parts) {
+      float t[2 * kValues];
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) { t[i] = at.in ? d[i] * (v[i] * r) : 0.f; t[kValues + i] = at.in ? d[i] : 0.f; }
+      sum += lane_sums(t);
+    }
+    if (dx && at.in) {
+#pragma unroll
+      for (int i = 0; i < kValues; ++i) {
+        int const c = warp + kWarps * i;
+        if (c < C) dx[at.at + (size_t)P * c] = r * (__ldg(g + c) * d[i] - m1 - v[i] * r * m2);
+      }
+    }
+  }
+  if (!parts) return;
+  int const c = warp + kWarps * (lane % kValues);
+  if (c < C && lane < 2 * kValues) parts[(size_t)blockIdx.x * 2 * C + (lane < kValues ? 0 : C) + c] = sum;
+}
+
+// Any number of channels: the values are read again for each pass, the block's sums over positions are kept in parts themselves.
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * 32)
+maps_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
+                     long long positions, int tiles, int P, int C, float eps)
+{
+  vlb::pdl_wait();
+  __shared__ float red[2][4][kWarps][32];
+  int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float const n = (float)C;
+  float* const own = parts ? parts + (size_t)blockIdx.x * 2 * C : nullptr;
+  int even = 0;
+  bool first = true;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, even ^= 1, first = false) {
+    Place const at = place_of(tile * 32ll + lane, positions, P, C);
+    float const *const xp = x + at.at, *const dp = dy + at.at;
+    float m[1] = {0.f};
+#pragma unroll 8
+    for (int c = warp; c < C; c += kWarps) m[0] += __ldg(xp + (size_t)P * c);
+    lane_totals<kWarps>(m, red[even] + 3);
+    float const mean = m[0] / n;
+    float s[3] = {};
+#pragma unroll 4
+    for (int c = warp; c < C; c += kWarps) {
+      float const v = __ldg(xp + (size_t)P * c) - mean, gd = __ldg(g + c) * __ldg(dp + (size_t)P * c);
+      s[0] += v * v; s[1] += gd; s[2] += gd * v;
+    }
+    lane_totals<kWarps>(s, red[even]);
+    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+    for (int c0 = warp; c0 < C; c0 += kWarps * 16) {
+      float t[32];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        int const c = c0 + kWarps * i;
+        float const xh = c < C ? (__ldg(xp + (size_t)P * c) - mean) * r : 0.f, d = c < C ? __ldg(dp + (size_t)P * c) : 0.f;
+        if (dx && at.in && c < C) dx[at.at + (size_t)P * c] = r * (__ldg(g + c) * d - m1 - xh * m2);
+        t[i] = at.in ? d * xh : 0.f; t[16 + i] = at.in ? d : 0.f;
+      }
+      if (own) {
+        float const sum = lane_sums(t);
+        int const c = c0 + kWarps * (lane % 16);
+        float* const p = own + (lane < 16 ? 0 : C) + c;
+        if (c < C) *p = first ? sum : *p + sum;
+      }
+    }
+  }
+}
+
+// dG and dB from the parts of `count` blocks, 32 columns per block, in a fixed order.
+__global__ void __launch_bounds__(1024)
+sum_blocks_kernel(float* __restrict__ dg, float* __restrict__ db, float const* __restrict__ parts, int count, int C)
+{
+  vlb::pdl_wait();
+  __shared__ float all[32][33];
+  int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + tx;
   float s = 0.f;
-  for (int c = threadIdx.x; c < C; c += blockDim.x) s += x[P * c];
-  float const mean = block_sum2(s, 0.f, red).x / (float)C;
-  float v = 0.f;
-  for (int c = threadIdx.x; c < C; c += blockDim.x) { float const d = x[P * c] - mean; v += d * d; }
-  return {mean, 1.f / sqrtf(block_sum2(v, 0.f, red).x / (float)C + eps)};
+  if (c < 2 * C) {
+#pragma unroll 4
+    for (int i = ty; i < count; i += 32) s += __ldg(parts + (size_t)i * 2 * C + c);
+  }
+  all[ty][tx] = s;
+  __syncthreads();
+  if (ty) return;
+  for (int i = 1; i < 32; ++i) s += all[i][tx];
+  if (c < C) { if (dg) dg[c] = s; }
+  else if (c < 2 * C) { if (db) db[c - C] = s; }
 }
 
-// A block per position: P positions of an image, values of a position P floats apart.
-__global__ void lnorm_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b,
-                                 int P, int C, float eps)
+bool bad_shape(int H, int W, int C, int N) { return H <= 0 || W <= 0 || C <= 0 || N <= 0 || (long long)H * W * N > INT32_MAX - 64; }
+
+bool wide(int C, std::initializer_list<void const*> ps)
 {
-  vlb::pdl_wait();
-  __shared__ float2 red[32];
-  size_t const at = blockIdx.x / P * ((size_t)P * C) + blockIdx.x % P;
-  Moments const m = moments_of(x + at, P, C, eps, red);
-  for (int c = threadIdx.x; c < C; c += blockDim.x) y[at + (size_t)P * c] = g[c] * ((x[at + (size_t)P * c] - m.mean) * m.r) + b[c];
+  uintptr_t all = 0;
+  for (void const* p : ps) all |= (uintptr_t)p;
+  return C % 4 == 0 && (all & 15) == 0;
 }
 
-__global__ void lnorm_dx_kernel(float* __restrict__ dx, Moments* __restrict__ moments, float const* __restrict__ x, float const* __restrict__ g,
-                                float const* __restrict__ dy, int P, int C, float eps)
+// Threads per row: as few as hold it with sixteen values each.  f(threads, vec) for the smallest that do; false for rows that are too long.
+template <class F>
+bool with_row(int C, F f)
 {
-  vlb::pdl_wait();
-  __shared__ float2 red[32];
-  size_t const at = blockIdx.x / P * ((size_t)P * C) + blockIdx.x % P;
-  Moments const m = moments_of(x + at, P, C, eps, red);
-  if (threadIdx.x == 0) moments[blockIdx.x] = m;
-  if (!dx) return;
-  float s = 0.f, sx = 0.f;
-  for (int c = threadIdx.x; c < C; c += blockDim.x) {
-    float const gd = g[c] * dy[at + (size_t)P * c];
-    s += gd; sx += gd * ((x[at + (size_t)P * c] - m.mean) * m.r);
-  }
-  float2 const t = block_sum2(s, sx, red);
-  for (int c = threadIdx.x; c < C; c += blockDim.x) {
-    size_t const i = at + (size_t)P * c;
-    dx[i] = m.r * (g[c] * dy[i] - t.x / (float)C - (x[i] - m.mean) * m.r * (t.y / (float)C));
-  }
+  if (C <= 128)   { f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{}); return true; }
+  if (C <= 256)   { f(std::integral_constant<int, 32>{}, std::integral_constant<int, 2>{}); return true; }
+  if (C <= 512)   { f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{}); return true; }
+  if (C <= 1024)  { f(std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{}); return true; }
+  if (C <= 2048)  { f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{}); return true; }
+  if (C <= 4096)  { f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{}); return true; }
+  if (C <= 8192)  { f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{}); return true; }
+  return false;
 }
-
-// A block per channel.
-__global__ void lnorm_dparam_kernel(float* __restrict__ dg, float* __restrict__ db, Moments const* __restrict__ moments, float const* __restrict__ x,
-                                    float const* __restrict__ dy, int P, int C, int positions)
-{
-  vlb::pdl_wait();
-  __shared__ float2 red[32];
-  float s = 0.f, sx = 0.f;
-  for (int p = threadIdx.x; p < positions; p += blockDim.x) {
-    size_t const i = p / P * ((size_t)P * C) + p % P + (size_t)P * blockIdx.x;
-    s += dy[i]; sx += dy[i] * ((x[i] - moments[p].mean) * moments[p].r);
-  }
-  float2 const t = block_sum2(s, sx, red);
-  if (threadIdx.x == 0) {
-    if (dg) dg[blockIdx.x] = t.y;
-    if (db) db[blockIdx.x] = t.x;
-  }
-}
-
-bool bad_shape(int H, int W, int C, int N) { return H <= 0 || W <= 0 || C <= 0 || N <= 0 || (long long)H * W * N > INT32_MAX; }
 
 }  // namespace
 
@@ -91,7 +477,28 @@ int vlb_lnorm_forward(vlb_ctx* ctx, float* Y, float const* X, float const* g, fl
   VLB_REQUIRE(ctx, !bad_shape(H, W, C, N), "lnorm_forward: bad shape");
   VLB_REQUIRE(ctx, Y && X && g && b, "lnorm_forward: null tensor");
   VLB_REQUIRE(ctx, eps >= 0, "lnorm_forward: epsilon is negative");
-  vlb::launch(ctx->stream, lnorm_fwd_kernel, (unsigned)(H * W * N), kThreads, 0, Y, X, g, b, H * W, C, (float)eps);
+  int const P = H * W, positions = P * N;
+  bool done = false;
+  if (P == 1) {
+    bool const vec = wide(C, {Y, X, g, b});
+    done = with_row(C, [&](auto threads, auto count) {
+      constexpr int kThreads = decltype(threads)::value, kVec = decltype(count)::value, kRows = block_of(kThreads) / kThreads;
+      auto const kernel = vec ? rows_fwd_kernel<kThreads, kVec, true> : rows_fwd_kernel<kThreads, kVec, false>;
+      vlb::launch(ctx->stream, kernel, (unsigned)vlb::ceil_div(N, kRows), block_of(kThreads), 0, Y, X, g, b, N, C, (float)eps);
+    });
+    if (!done) vlb::launch(ctx->stream, rows_fwd_long_kernel, (unsigned)N, 1024, 0, Y, X, g, b, C, (float)eps);
+    done = true;
+  }
+  if (!done) {
+    unsigned const grid = (unsigned)vlb::ceil_div(positions, 32);
+    auto run = [&](auto kernel, int warps) { vlb::launch(ctx->stream, kernel, grid, warps * 32, 0, Y, X, g, b, (long long)positions, P, C, (float)eps); };
+    if (C <= 32)        run(maps_fwd_kernel<8, 4>, 8);
+    else if (C <= 128)  run(maps_fwd_kernel<8, 16>, 8);
+    else if (C <= 256)  run(maps_fwd_kernel<16, 16>, 16);
+    else if (C <= 512)  run(maps_fwd_kernel<16, 32>, 16);
+    else if (C <= 1024) run(maps_fwd_kernel<32, 32>, 32);
+    else                run(maps_fwd_kernel<32, 0>, 32);
+  }
   VLB_LAUNCHED(ctx, 1);
   return vlb::check_launch(ctx, "vlb_lnorm_forward");
 }
@@ -103,12 +510,46 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
   VLB_REQUIRE(ctx, !bad_shape(H, W, C, N), "lnorm_backward: bad shape");
   VLB_REQUIRE(ctx, X && g && dY, "lnorm_backward: null tensor");
   VLB_REQUIRE(ctx, eps >= 0, "lnorm_backward: epsilon is negative");
-  int const positions = H * W * N;
-  Moments* const m = (Moments*)vlb::workspace(ctx, sizeof(Moments) * (size_t)positions);
-  if (!m) return vlb::pass_error(ctx, ctx->lastError, "vlb_lnorm_backward");
-  vlb::launch(ctx->stream, lnorm_dx_kernel, (unsigned)positions, kThreads, 0, dX, m, X, g, dY, H * W, C, (float)eps);
-  if (dG || dB) vlb::launch(ctx->stream, lnorm_dparam_kernel, (unsigned)C, kThreads, 0, dG, dB, m, X, dY, H * W, C, positions);
-  VLB_LAUNCHED(ctx, dG || dB ? 2 : 1);
+  if (!dX && !dG && !dB) return VLB_Success;
+  int const P = H * W, positions = P * N;
+  float* parts = nullptr;
+  if (dG || dB) {
+    parts = (float*)vlb::workspace(ctx, sizeof(float) * 2 * (size_t)C * kMaxParts);
+    if (!parts) return vlb::pass_error(ctx, ctx->lastError, "vlb_lnorm_backward");
+  }
+  int blocks = 0;
+  if (P == 1) {
+    bool const vec = wide(C, {dX, X, g, dY});
+    with_row(C, [&](auto threads, auto count) {
+      constexpr int kThreads = decltype(threads)::value, kVec = decltype(count)::value, kRows = block_of(kThreads) / kThreads;
+      // as many blocks as fit the device at once: half of its threads with sixteen values each of three tensors in registers
+      int const perSm = std::max(1, std::min(4, 512 / block_of(kThreads)));
+      blocks = std::min(vlb::ceil_div(N, kRows), std::min(kMaxParts, ctx->smCount * perSm));
+      auto const kernel = vec ? rows_bwd_kernel<kThreads, kVec, true> : rows_bwd_kernel<kThreads, kVec, false>;
+      vlb::launch(ctx->stream, kernel, (unsigned)blocks, block_of(kThreads), 0, dX, parts, X, g, dY, N, C, (float)eps);
+    });
+    if (!blocks) {
+      blocks = std::min(N, ctx->smCount * 2);
+      vlb::launch(ctx->stream, rows_bwd_long_kernel, (unsigned)blocks, 1024, 0, dX, parts, X, g, dY, N, C, (float)eps);
+    }
+  }
+  if (!blocks) {
+    int const tiles = vlb::ceil_div(positions, 32);
+    auto run = [&](auto kernel, int warps) {
+      blocks = std::min(tiles, std::min(kMaxParts, ctx->smCount * std::max(1, std::min(4, 32 / warps))));
+      vlb::launch(ctx->stream, kernel, (unsigned)blocks, warps * 32, 0, dX, parts, X, g, dY, (long long)positions, tiles, P, C, (float)eps);
+    };
+    if (C <= 32)       run(maps_bwd_kernel<8, 4>, 8);
+    else if (C <= 128) run(maps_bwd_kernel<8, 16>, 8);
+    else if (C <= 256) run(maps_bwd_kernel<16, 16>, 16);
+    else if (C <= 512) run(maps_bwd_kernel<32, 16>, 32);
+    else               run(maps_bwd_long_kernel<16>, 16);
+  }
+  VLB_LAUNCHED(ctx, 1);
+  if (parts) {
+    vlb::launch(ctx->stream, sum_blocks_kernel, (unsigned)vlb::ceil_div(2ll * C, 32), 1024, 0, dG, dB, parts, blocks, C);
+    VLB_LAUNCHED(ctx, 1);
+  }
   return vlb::check_launch(ctx, "vlb_lnorm_backward");
 }
 
