@@ -343,6 +343,293 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
   return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_backward");
 }
 
+// ------------------------------------------------------------------ few images: on CUDA cores, bound by reading F
+// Up to sixteen images: F is read as it is, once forward and twice backward (and its derivative written); with the images in shared memory a class costs as
+// many multiplications as there are images, exact ones, which the cores do in the time that its row takes to arrive.
+constexpr int kFew = 16;
+constexpr int kFewFloats = 49152;             // images that fit shared memory: 192 KB
+constexpr int kFewWarps = 16;
+
+bool few_images(int N, long long D) { return N <= kFew && N * D <= kFewFloats; }
+
+struct FewArgs {
+  float const *x, *f, *b, *labels, *lse;
+  int N, D, K;
+  int* status;
+  float2* parts; float* label;                // forward: parts[block * N + n]
+  float *dz, *db; float scale;                // backward: dz[class * kImages + n]
+};
+
+// Predictions, kRows classes at a time to the warps of all blocks in turn (neighbouring ones to different blocks); forward their largest and sum of exponentials, backward the derivatives.
+template <int kImages, int kRows, bool kBack, bool kWide>
+__global__ void __launch_bounds__(kFewWarps * 32, 1)
+few_predict_kernel(FewArgs a)
+{
+  vlb::pdl_wait();
+  extern __shared__ __align__(16) float xs[];               // [n][D rounded up to a multiple of 128]
+  __shared__ float info[2][kFew];                           // label + 1, or 0 for an image that is skipped; lse
+  int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ld = (a.D + 127) / 128 * 128;
+  if (threadIdx.x < a.N) {
+    Label const l = label_of(a.labels, threadIdx.x, a.K, blockIdx.x == 0 ? a.status : nullptr);
+    info[0][threadIdx.x] = l.real ? (float)(l.at + 1) : 0.f;
+    info[1][threadIdx.x] = kBack ? a.lse[threadIdx.x] : 0.f;
+  }
+  __syncthreads();
+  for (int n = 0; n < a.N; ++n) {
+    bool const real = info[0][n] > 0.f;                     // (what a skipped image holds is not looked at)
+    for (int d = threadIdx.x; d < ld; d += kFewWarps * 32) xs[n * ld + d] = real && d < a.D ? a.x[(size_t)n * a.D + d] : 0.f;
+  }
+  __syncthreads();
+  int const n = lane % kImages, k1 = a.K;
+  int const at = n < a.N ? (int)info[0][n] - 1 : -1;        // the label's class, -1: skipped
+  float const lse = n < a.N ? info[1][n] : 0.f;
+  float top = -INFINITY, sum = 0.f;
+  for (int k = (warp * (int)gridDim.x + (int)blockIdx.x) * kRows; k < k1; k += kFewWarps * (int)gridDim.x * kRows) {
+    float acc[kRows * kImages] = {};
+    float const* f[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) f[r] = a.f + (size_t)min(k + r, k1 - 1) * a.D;
+#pragma unroll 4
+    for (int d = 4 * lane; d < ld; d += 128) {
+      float4 w[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        if (kWide) {
+          w[r] = d < a.D ? __ldg((float4 const*)(f[r] + d)) : make_float4(0, 0, 0, 0);
+        } else {
+          w[r].x = d < a.D ? __ldg(f[r] + d) : 0.f; w[r].y = d + 1 < a.D ? __ldg(f[r] + d + 1) : 0.f;
+          w[r].z = d + 2 < a.D ? __ldg(f[r] + d + 2) : 0.f; w[r].w = d + 3 < a.D ? __ldg(f[r] + d + 3) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kImages; ++i) {
+        if (kImages > 1 && i >= a.N) break;
+        float4 const q = *(float4 const*)(xs + i * ld + d);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          acc[r * kImages + i] = fmaf(w[r].x, q.x, fmaf(w[r].y, q.y, fmaf(w[r].z, q.z, fmaf(w[r].w, q.w, acc[r * kImages + i]))));
+      }
+    }
+    // lane l: class k + l / kImages % kRows of image l % kImages
+    constexpr int kCount = kRows * kImages;
+#pragma unroll
+    for (int s = kCount / 2; s > 0; s >>= 1) {
+      bool const up = lane & s;
+#pragma unroll
+      for (int i = 0; i < s; ++i) {
+        float const send = up ? acc[i] : acc[i + s], keep = up ? acc[i + s] : acc[i];
+        acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
+      }
+    }
+#pragma unroll
+    for (int s = kCount; s < 32; s <<= 1) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], s);
+    int const c = k + lane / kImages % kRows;
+    bool const mine = c < k1 && n < a.N && lane < kCount;
+    float const z = acc[0] + (a.b && c < k1 ? __ldg(a.b + c) : 0.f);
+    if (!kBack) {
+      if (mine) {
+        float const t = fmaxf(top, z), base = isinf(t) ? 0.f : t;
+        sum = sum * __expf(top - base) + __expf(z - base);
+        top = t;
+        if (c == at) a.label[n] = z;
+      }
+    } else {
+      float v = mine && at >= 0 ? (__expf(z - lse) - (c == at ? 1.f : 0.f)) * a.scale : 0.f;
+      if (c < k1 && lane < kCount) a.dz[(size_t)c * kImages + n] = v;
+      if (a.db) {
+#pragma unroll
+        for (int s = 1; s < kImages; s <<= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+        if (n == 0 && c < k1 && lane < kCount) a.db[c] = v;
+      }
+    }
+  }
+  if (kBack) return;
+  // lanes of one image, then the block's warps
+  Part p = {top, sum};
+#pragma unroll
+  for (int s = kImages; s < 32; s <<= 1) {
+    Part const q = {__shfl_xor_sync(0xffffffffu, p.top, s), __shfl_xor_sync(0xffffffffu, p.sum, s)};
+    p = lane & s ? together(q, p) : together(p, q);          // (in the lanes' order, so that all of them hold the same)
+  }
+  __shared__ Part all[kFewWarps][kFew];
+  if (lane < kImages) all[warp][lane] = p;
+  __syncthreads();
+  if (threadIdx.x < a.N) {
+    p = all[0][threadIdx.x];
+    for (int w = 1; w < kFewWarps; ++w) p = together(p, all[w][threadIdx.x]);
+    a.parts[blockIdx.x * a.N + threadIdx.x] = make_float2(p.top, p.sum);
+  }
+}
+
+// dF of the block's classes, and the block's part of dX: parts[block][n][D].  A thread has four neighbouring columns (kWide) or four kFewThreads apart.
+constexpr int kFewThreads = 128;
+
+template <int kImages, bool kWide>
+__global__ void __launch_bounds__(kFewThreads)
+few_derivatives_kernel(float* __restrict__ dF, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ f, float const* __restrict__ dz,
+                       float const* __restrict__ labels, int N, int D, int K, int perBlock)
+{
+  vlb::pdl_wait();
+  int const c0 = (int)blockIdx.y * 4 * kFewThreads + (kWide ? 4 : 1) * (int)threadIdx.x, k0 = (int)blockIdx.x * perBlock, k1 = min(k0 + perBlock, K);
+  auto col = [&](int i) { return kWide ? c0 + i : c0 + kFewThreads * i; };
+  float xv[kImages][4] = {}, acc[kImages][4] = {};
+#pragma unroll
+  for (int n = 0; n < kImages; ++n)
+    if (n < N && label_of(labels, n, K, nullptr).real)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) if (col(i) < D) xv[n][i] = __ldg(x + (size_t)n * D + col(i));
+#pragma unroll 4
+  for (int k = k0; k < k1; ++k) {
+    float w[4] = {}, o[4] = {}, g[kImages];
+    if (parts) {
+      if (kWide) {
+        float4 const q = col(0) < D ? __ldg((float4 const*)(f + (size_t)k * D + col(0))) : make_float4(0, 0, 0, 0);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = col(i) < D ? __ldg(f + (size_t)k * D + col(i)) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kImages; ++n) g[n] = __ldg(dz + (size_t)k * kImages + n);
+#pragma unroll
+    for (int n = 0; n < kImages; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { acc[n][i] = fmaf(g[n], w[i], acc[n][i]); o[i] = fmaf(g[n], xv[n][i], o[i]); }
+    if (dF) {
+      if (kWide) {
+        if (col(0) < D) *(float4*)(dF + (size_t)k * D + col(0)) = make_float4(o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (col(i) < D) dF[(size_t)k * D + col(i)] = o[i];
+      }
+    }
+  }
+  if (!parts) return;
+#pragma unroll
+  for (int n = 0; n < kImages; ++n)
+    if (n < N)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) if (col(i) < D) parts[((size_t)blockIdx.x * N + n) * D + col(i)] = acc[n][i];
+}
+
+// dX = the sum of the blocks' parts, in order: 32 elements to a block.
+__global__ void __launch_bounds__(512)
+few_sum_kernel(float* __restrict__ dX, float const* __restrict__ parts, int count, int n)
+{
+  vlb::pdl_wait();
+  __shared__ float all[16][33];
+  int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, at = (int)blockIdx.x * 32 + tx;
+  float s = 0.f;
+  if (at < n) {
+#pragma unroll 4
+    for (int i = ty; i < count; i += 16) s += __ldg(parts + (size_t)i * n + at);
+  }
+  all[ty][tx] = s;
+  __syncthreads();
+  if (ty) return;
+  for (int i = 1; i < 16; ++i) s += all[i][tx];
+  if (at < n) dX[at] = s;
+}
+
+// f(images, rows): the smallest number of images, a power of two, that holds N, and the classes that a warp takes at a time.
+template <class F>
+void with_images(int N, F f)
+{
+  using std::integral_constant;
+  if (N == 1)      f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  else if (N == 2) f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+  else if (N <= 4) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  else if (N <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  else             f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+}
+
+bool aligned(int D, void const* f) { return D % 4 == 0 && ((uintptr_t)f & 15) == 0; }
+
+template <bool kBack>
+int few_predict(Problem const& q, FewArgs a, int& blocks)
+{
+  int rc = VLB_Success;
+  with_images(q.N, [&](auto images, auto rows) {
+    constexpr int kImages = decltype(images)::value, kRows = decltype(rows)::value;
+    blocks = std::min(q.ctx->smCount, vlb::ceil_div(q.K, kRows));
+    auto const kernel = aligned(q.D, q.F) ? few_predict_kernel<kImages, kRows, kBack, true> : few_predict_kernel<kImages, kRows, kBack, false>;
+    size_t const smem = sizeof(float) * (size_t)q.N * vlb::ceil_div(q.D, 128) * 128;
+    static bool ready[64][2];
+    bool& r = ready[q.ctx->device & 63][aligned(q.D, q.F)];
+    if (smem > 32 * 1024 && !r) {
+      cudaError_t const e = vlb::allow_max_dynamic_smem(kernel);
+      if (e != cudaSuccess) { rc = vlb::set_error(q.ctx, VLB_Cuda, cudaGetErrorString(e)); return; }
+      r = true;
+    }
+    vlb::launch(q.ctx->stream, kernel, (unsigned)blocks, kFewWarps * 32, smem, a);
+    VLB_LAUNCHED(q.ctx, 1);
+  });
+  return rc;
+}
+
+FewArgs few_args(Problem const& q)
+{
+  FewArgs a = {};
+  a.x = q.X; a.f = q.F; a.b = q.b; a.labels = q.labels;
+  a.N = q.N; a.D = q.D; a.K = q.K;
+  return a;
+}
+
+// lse and loss (either may be null); scratch: few_scratch(q) bytes.
+size_t few_scratch(Problem const& q) { return (sizeof(float2) * q.ctx->smCount + 2 * sizeof(float)) * kFew + 64; }
+
+int few_seen(Problem const& q, float* loss, float* lse, char* scratch, int* status)
+{
+  FewArgs a = few_args(q);
+  a.parts = (float2*)scratch;
+  a.label = (float*)(a.parts + (size_t)q.ctx->smCount * kFew);
+  double* const sums = (double*)(a.label + kFew);
+  int blocks = 0;
+  if (int const rc = few_predict<false>(q, a, blocks)) return rc;
+  vlb::launch(q.ctx->stream, lse_kernel, 1, 1024, 0, loss, lse, a.parts, blocks, a.label, q.labels, q.N, 0, q.N, q.K, sums, 1,
+              q.ctx->deviceStatus + 64 + 4095, status);
+  VLB_LAUNCHED(q.ctx, 1);
+  return VLB_Success;
+}
+
+int forward_few(Problem const& q, float* loss, float* lse)
+{
+  char* const scratch = (char*)vlb::workspace(q.ctx, few_scratch(q));
+  if (!scratch) return q.ctx->lastError;
+  if (int const rc = few_seen(q, loss, lse, scratch, q.ctx->deviceStatus)) return rc;
+  return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_forward");
+}
+
+int backward_few(Problem const& q, float* dX, float* dF, float* db, float const* lse, float scale)
+{
+  int const columns = vlb::ceil_div(q.D, 4 * kFewThreads), chunks = std::min(q.K, std::max(1, 4 * q.ctx->smCount / columns)), per = vlb::ceil_div(q.K, chunks);
+  int const count = vlb::ceil_div(q.K, per);
+  size_t const seen = (few_scratch(q) + 255) / 256 * 256, dzBytes = (sizeof(float) * (size_t)q.K * kFew + 255) / 256 * 256;
+  char* const scratch = (char*)vlb::workspace(q.ctx, seen + 256 + dzBytes + (dX ? sizeof(float) * (size_t)count * q.N * q.D : 0));
+  if (!scratch) return q.ctx->lastError;
+  float *const own = (float*)(scratch + seen), *const dz = (float*)(scratch + seen + 256), *const parts = dX ? (float*)(scratch + seen + 256 + dzBytes) : nullptr;
+  if (!lse)
+    if (int const rc = few_seen(q, nullptr, own, scratch, nullptr)) return rc;
+  FewArgs a = few_args(q);
+  a.lse = lse ? lse : own; a.dz = dz; a.db = db; a.scale = scale; a.status = q.ctx->deviceStatus;
+  int blocks = 0;
+  if (int const rc = few_predict<true>(q, a, blocks)) return rc;
+  if (dX || dF)
+    with_images(q.N, [&](auto images, auto) {
+      constexpr int kImages = decltype(images)::value;
+      bool const wide = aligned(q.D, q.F) && (!dF || aligned(q.D, dF));
+      vlb::launch(q.ctx->stream, wide ? few_derivatives_kernel<kImages, true> : few_derivatives_kernel<kImages, false>, dim3((unsigned)count, (unsigned)columns),
+                  kFewThreads, 0, dF, parts, q.X, q.F, dz, q.labels, q.N, q.D, q.K, per);
+      VLB_LAUNCHED(q.ctx, 1);
+    });
+  if (dX) {
+    vlb::launch(q.ctx->stream, few_sum_kernel, (unsigned)vlb::ceil_div((long long)q.N * q.D, 32), 512, 0, dX, parts, count, q.N * q.D);
+    VLB_LAUNCHED(q.ctx, 1);
+  }
+  return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_backward");
+}
+
 // Classes per piece: predictions of a piece up to 64 MB.
 int piece_of(int N, int K) { return (int)std::min<long long>(K, std::max<long long>(64, (16ll << 20) / N / 64 * 64)); }
 
@@ -356,9 +643,11 @@ int vlb_fc_softmaxloss_forward(vlb_ctx* ctx, float* loss, float* lse, float cons
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W * C <= INT32_MAX, "fc_softmaxloss_forward: bad shape");
   VLB_REQUIRE(ctx, loss && X && F && labels, "fc_softmaxloss_forward: null tensor");
+  int const D = H * W * C;
+  if (few_images(N, D)) return vlb::pass_error(ctx, forward_few({ctx, X, F, b, labels, N, D, K}, loss, lse), "vlb_fc_softmaxloss_forward");
   if (ctx->precision != VLB_PRECISION_FP32)
-    return vlb::pass_error(ctx, forward_on_pairs({ctx, X, F, b, labels, N, H * W * C, K}, loss, lse), "vlb_fc_softmaxloss_forward");
-  int const D = H * W * C, piece = piece_of(N, K);
+    return vlb::pass_error(ctx, forward_on_pairs({ctx, X, F, b, labels, N, D, K}, loss, lse), "vlb_fc_softmaxloss_forward");
+  int const piece = piece_of(N, K);
   char* const ws = (char*)vlb::workspace(ctx, sizeof(float) * (size_t)N * piece + sizeof(Seen) * (size_t)N);
   if (!ws) return vlb::pass_error(ctx, ctx->lastError, "vlb_fc_softmaxloss_forward");
   float* const z = (float*)ws;
@@ -380,9 +669,12 @@ int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, f
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W * C <= INT32_MAX, "fc_softmaxloss_backward: bad shape");
   VLB_REQUIRE(ctx, X && F && labels, "fc_softmaxloss_backward: null tensor");
+  int const D = H * W * C;
+  if (few_images(N, D))
+    return vlb::pass_error(ctx, backward_few({ctx, X, F, b, labels, N, D, K}, dX, dF, db, lse, (float)(dzdy / N)), "vlb_fc_softmaxloss_backward");
   if (ctx->precision != VLB_PRECISION_FP32)
-    return vlb::pass_error(ctx, backward_on_pairs({ctx, X, F, b, labels, N, H * W * C, K}, dX, dF, db, lse, (float)(dzdy / N)), "vlb_fc_softmaxloss_backward");
-  int const D = H * W * C, piece = piece_of(N, K);
+    return vlb::pass_error(ctx, backward_on_pairs({ctx, X, F, b, labels, N, D, K}, dX, dF, db, lse, (float)(dzdy / N)), "vlb_fc_softmaxloss_backward");
+  int const piece = piece_of(N, K);
   size_t const ND = (size_t)N * D;
   float* const z = (float*)vlb::workspace(ctx, sizeof(float) * ((size_t)N * piece + N + ND) + sizeof(Seen) * (size_t)N);
   if (!z) return vlb::pass_error(ctx, ctx->lastError, "vlb_fc_softmaxloss_backward");

@@ -6,7 +6,7 @@
 // channels.  Both count positions through the batch.  What does not fit the registers is read again for each pass, from L2.
 //
 // The sums over positions (dG, dB) are kept per channel by the threads that see it; each block leaves its part, and a second kernel adds the parts in order.
-#include "common.cuh"
+#include "tc_common.cuh"
 #include <algorithm>
 
 namespace {
@@ -103,47 +103,98 @@ rows_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const*
   R::store(y + (size_t)row * C, v, C);
 }
 
-// Rows in turn to the blocks (or, kThreads == 32, to the warps).  parts: [block][2][C], dG then dB.
+// Groups of neighbouring rows in turn to the blocks, `per` rows to a row's threads.  kWide: they come by bulk copies, kStages groups on their way or in use, so that
+// the reductions of one row (half of the time otherwise) do not keep the memory waiting: 16384 x 4096 175 -> 126 us, the copy rate.  Without 16-byte alignment every thread loads
+// its own values.  parts: [block][2][C], dG then dB.
+constexpr int kStages = 3;
+
 template <int kThreads, int kVec, bool kWide>
 __global__ void __launch_bounds__(block_of(kThreads))
 rows_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
-                int rows, int C, float eps)
+                int rows, int C, int per, float eps, int* status)
 {
   using R = Row<kThreads, kVec, kWide>;
-  constexpr int kRows = block_of(kThreads) / kThreads;
-  vlb::pdl_wait();
+  constexpr int kRows = block_of(kThreads) / kThreads, kWarps = block_of(kThreads) / 32;
+  extern __shared__ __align__(128) float staged[];         // [stage][x or dy][per * kRows rows]
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
   __shared__ float red[2][4][32];
   __shared__ float other[kRows > 1 ? (kRows - 1) * 2 * 32 * R::kValues : 1];
+  int const group = per * kRows, groups = (rows + group - 1) / group, mine = ((int)blockIdx.x < groups) ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  if (kWide) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kStages; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), kWarps); }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+  }
+  vlb::pdl_wait();
+  bool dead = false;                                       // a wait ran out: nothing is waited for any more
+  auto fetch = [&](int it) {                               // by one thread
+    int const st = it % kStages, row0 = ((int)blockIdx.x + it * (int)gridDim.x) * group, count = min(group, rows - row0);
+    if (it >= kStages && !dead && !mbar_wait(smem_u32(&empty[st]), (uint32_t)(it / kStages - 1) & 1u)) dead = true;
+    if (dead) return;
+    uint32_t const bytes = (uint32_t)count * C * 4, to = smem_u32(staged + (size_t)st * 2 * group * C);
+    mbar_arrive_expect_tx(smem_u32(&full[st]), 2 * bytes);
+    bulk_copy_g2s(to, x + (size_t)row0 * C, bytes, smem_u32(&full[st]));
+    bulk_copy_g2s(to + (uint32_t)group * C * 4, dy + (size_t)row0 * C, bytes, smem_u32(&full[st]));
+  };
+  if (kWide && threadIdx.x == 0)
+    for (int it = 0; it < min(mine, kStages - 1); ++it) fetch(it);
   float gv[R::kValues], dg[R::kValues] = {}, db[R::kValues] = {};
   R::load(gv, g, C);
   float const n = (float)C;
   int even = 0;
-  for (int row = (int)blockIdx.x * kRows + (int)threadIdx.x / kThreads; row < rows; row += (int)gridDim.x * kRows, even ^= 1) {
-    float v[R::kValues], d[R::kValues];
-    R::load(v, x + (size_t)row * C, C);
-    R::load(d, dy + (size_t)row * C, C);
-    float m[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < R::kValues; ++i) m[0] += v[i];
-    row_sums<kThreads>(m, red[even] + 3);
-    float const mean = m[0] / n;
-    float s[3] = {};
-#pragma unroll
-    for (int i = 0; i < R::kValues; ++i) {
-      v[i] = R::channel(i) < C ? v[i] - mean : 0.f;
-      float const gd = gv[i] * d[i];
-      s[0] += v[i] * v[i]; s[1] += gd; s[2] += gd * v[i];
+  for (int it = 0; it < mine; ++it) {
+    int const st = it % kStages, row0 = ((int)blockIdx.x + it * (int)gridDim.x) * group;
+    if (kWide) {
+      if (threadIdx.x == 0 && it + kStages - 1 < mine) fetch(it + kStages - 1);
+      if (!dead && !mbar_wait(smem_u32(&full[st]), (uint32_t)(it / kStages) & 1u)) dead = true;
     }
-    row_sums<kThreads>(s, red[even]);
-    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+    for (int k = 0; k < per; ++k, even ^= 1) {
+      int const local = k * kRows + (int)threadIdx.x / kThreads, row = row0 + local;
+      if (row >= rows) break;                              // (a block has one row at a time where its threads meet at barriers)
+      float v[R::kValues], d[R::kValues];
+      if (kWide) {
+        float const* const from = staged + ((size_t)st * 2 * group + local) * C;
 #pragma unroll
-    for (int i = 0; i < R::kValues; ++i) {
-      float const xh = v[i] * r;
-      dg[i] += d[i] * xh; db[i] += d[i];
-      v[i] = r * (gv[i] * d[i] - m1 - xh * m2);
+        for (int i = 0; i < kVec; ++i) {
+          int const c = R::channel(4 * i);
+          float4 const p = c < C ? *(float4 const*)(from + c) : make_float4(0, 0, 0, 0), q = c < C ? *(float4 const*)(from + (size_t)group * C + c) : make_float4(0, 0, 0, 0);
+          v[4 * i] = p.x; v[4 * i + 1] = p.y; v[4 * i + 2] = p.z; v[4 * i + 3] = p.w;
+          d[4 * i] = q.x; d[4 * i + 1] = q.y; d[4 * i + 2] = q.z; d[4 * i + 3] = q.w;
+        }
+      } else {
+        R::load(v, x + (size_t)row * C, C);
+        R::load(d, dy + (size_t)row * C, C);
+      }
+      float m[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < R::kValues; ++i) m[0] += v[i];
+      row_sums<kThreads>(m, red[even] + 3);
+      float const mean = m[0] / n;
+      float s[3] = {};
+#pragma unroll
+      for (int i = 0; i < R::kValues; ++i) {
+        v[i] = R::channel(i) < C ? v[i] - mean : 0.f;
+        float const gd = gv[i] * d[i];
+        s[0] += v[i] * v[i]; s[1] += gd; s[2] += gd * v[i];
+      }
+      row_sums<kThreads>(s, red[even]);
+      float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+#pragma unroll
+      for (int i = 0; i < R::kValues; ++i) {
+        float const xh = v[i] * r;
+        dg[i] += d[i] * xh; db[i] += d[i];
+        v[i] = r * (gv[i] * d[i] - m1 - xh * m2);
+      }
+      if (dx) R::store(dx + (size_t)row * C, v, C);
     }
-    if (dx) R::store(dx + (size_t)row * C, v, C);
+    if (kWide) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&empty[st]));
+    }
   }
+  if (dead) atomicCAS(status, 0, 43);
   if (!parts) return;
   if (kRows > 1) {
     // the block's warps, added in order
@@ -229,8 +280,8 @@ rows_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
 }
 
 // ------------------------------------------------------------------ positions of maps
-// A block of kWarps warps takes 32 positions, a lane's is `q` of the batch; warp w has the channels w, w + kWarps, ..., kValues of them in registers (0: read
-// again for every pass).
+// A block of kWarps warps takes 32 positions, kPos neighbouring ones to a lane: 1, or 4 by 16-byte loads where planes and tensors allow it; a warp's lanes then have
+// kPos channels at a time.  28 x 28 x 512 x 64 forward with kPos 1 / 4: 52 / 49 us.  A lane has kValues of the channels in registers (0: read again for every pass).
 struct Place { size_t at; bool in; };
 
 __device__ __forceinline__ Place place_of(long long q, long long positions, int P, int C)
@@ -240,140 +291,233 @@ __device__ __forceinline__ Place place_of(long long q, long long positions, int 
   return {(size_t)(n * P * C + (t - n * P)), in};
 }
 
-// Sums over the block's warps, lane by lane.
-template <int kWarps, int kCount>
-__device__ __forceinline__ void lane_totals(float (&v)[kCount], float (*red)[kWarps][32])
-{
-  int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int k = 0; k < kCount; ++k) red[k][warp][lane] = v[k];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kCount; ++k) {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += red[k][w][lane];
-    v[k] = s;
+template <int kWarps, int kPos>
+struct Maps {
+  static constexpr int kLanes = 32 / kPos;
+  static __device__ __forceinline__ int channel(int i) { return (int)(threadIdx.x >> 5) * kPos + (int)(threadIdx.x & 31) / kLanes + kWarps * kPos * i; }
+  // the first of the lane's positions; those behind the batch's last (all kPos of them) repeat earlier ones
+  static __device__ __forceinline__ Place place(int tile, long long positions, int P, int C)
+  {
+    long long const q = tile * 32ll + (threadIdx.x & 31) % kLanes * kPos;
+    Place const p = place_of(min(q, positions - kPos), positions, P, C);
+    return {p.at, q < positions};
   }
-}
+  static __device__ __forceinline__ void load(float (&v)[kPos], float const* __restrict__ p)
+  {
+    if (kPos == 4) { float4 const q = __ldg((float4 const*)p); v[0] = q.x; v[1 % kPos] = q.y; v[2 % kPos] = q.z; v[3 % kPos] = q.w; }
+    else v[0] = __ldg(p);
+  }
+  static __device__ __forceinline__ void store(float* __restrict__ p, float const (&v)[kPos])
+  {
+    if (kPos == 4) *(float4*)p = make_float4(v[0], v[1 % kPos], v[2 % kPos], v[3 % kPos]);
+    else *p = v[0];
+  }
+  // sums over the block's channels, position by position
+  template <int kCount>
+  static __device__ __forceinline__ void totals(float (&v)[kCount][kPos], float (*red)[kWarps][32])
+  {
+    int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane % kLanes * kPos;
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+#pragma unroll
+      for (int p = 0; p < kPos; ++p)
+        for (int o = kLanes; o < 32; o <<= 1) v[k][p] += __shfl_xor_sync(0xffffffffu, v[k][p], o);
+      if (lane < kLanes) store(&red[k][warp][at], v[k]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      float t[kPos] = {};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (kPos == 4) {
+          float4 const q = *(float4 const*)&red[k][w][at];
+          t[0] += q.x; t[1 % kPos] += q.y; t[2 % kPos] += q.z; t[3 % kPos] += q.w;
+        } else {
+          t[0] += red[k][w][at];
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) v[k][p] = t[p];
+    }
+  }
+};
 
-template <int kWarps, int kValues>
-__global__ void __launch_bounds__(kWarps * 32)
+template <int kWarps, int kPos, int kValues>
+__global__ void __launch_bounds__(kWarps * 32, kWarps > 16 ? 1 : 32 / kWarps)
 maps_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, long long positions, int P, int C,
                 float eps)
 {
+  using M = Maps<kWarps, kPos>;
   vlb::pdl_wait();
-  __shared__ float red[2][1][kWarps][32];
-  int const warp = threadIdx.x >> 5;
-  Place const at = place_of(blockIdx.x * 32ll + (threadIdx.x & 31), positions, P, C);
+  __shared__ __align__(16) float red[2][1][kWarps][32];
+  Place const at = M::place(blockIdx.x, positions, P, C);
   float const* const xp = x + at.at;
   float* const yp = y + at.at;
-  float v[kValues > 0 ? kValues : 1], s[1] = {0.f};
+  float v[kValues > 0 ? kValues : 1][kPos], s[1][kPos] = {};
   if (kValues) {
 #pragma unroll
-    for (int i = 0; i < kValues; ++i) { int const c = warp + kWarps * i; v[i] = c < C ? __ldg(xp + (size_t)P * c) : 0.f; }
+    for (int i = 0; i < kValues; ++i) {
 #pragma unroll
-    for (int i = 0; i < kValues; ++i) s[0] += v[i];
+      for (int p = 0; p < kPos; ++p) v[i][p] = 0.f;
+      if (M::channel(i) < C) M::load(v[i], xp + (size_t)P * M::channel(i));
+    }
+#pragma unroll
+    for (int i = 0; i < kValues; ++i)
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) s[0][p] += v[i][p];
   } else {
 #pragma unroll 8
-    for (int c = warp; c < C; c += kWarps) s[0] += __ldg(xp + (size_t)P * c);
+    for (int c = M::channel(0); c < C; c += kWarps * kPos) {
+      M::load(v[0], xp + (size_t)P * c);
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) s[0][p] += v[0][p];
+    }
   }
-  lane_totals<kWarps>(s, red[0]);
-  float const mean = s[0] / (float)C;
-  s[0] = 0.f;
+  M::totals(s, red[0]);
+  float mean[kPos], r[kPos];
+#pragma unroll
+  for (int p = 0; p < kPos; ++p) { mean[p] = s[0][p] / (float)C; s[0][p] = 0.f; }
   if (kValues) {
 #pragma unroll
-    for (int i = 0; i < kValues; ++i) { v[i] -= mean; s[0] += warp + kWarps * i < C ? v[i] * v[i] : 0.f; }
+    for (int i = 0; i < kValues; ++i)
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) { v[i][p] -= mean[p]; s[0][p] += M::channel(i) < C ? v[i][p] * v[i][p] : 0.f; }
   } else {
 #pragma unroll 8
-    for (int c = warp; c < C; c += kWarps) { float const d = __ldg(xp + (size_t)P * c) - mean; s[0] += d * d; }
+    for (int c = M::channel(0); c < C; c += kWarps * kPos) {
+      M::load(v[0], xp + (size_t)P * c);
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) s[0][p] += (v[0][p] - mean[p]) * (v[0][p] - mean[p]);
+    }
   }
-  lane_totals<kWarps>(s, red[1]);
-  float const r = 1.f / sqrtf(s[0] / (float)C + eps);
+  M::totals(s, red[1]);
+#pragma unroll
+  for (int p = 0; p < kPos; ++p) r[p] = 1.f / sqrtf(s[0][p] / (float)C + eps);
   if (!at.in) return;
   if (kValues) {
 #pragma unroll
     for (int i = 0; i < kValues; ++i) {
-      int const c = warp + kWarps * i;
-      if (c < C) yp[(size_t)P * c] = fmaf(__ldg(g + c), v[i] * r, __ldg(b + c));
+      int const c = M::channel(i);
+      if (c >= C) break;
+      float const gc = __ldg(g + c), bc = __ldg(b + c);
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) v[i][p] = fmaf(gc, v[i][p] * r[p], bc);
+      M::store(yp + (size_t)P * c, v[i]);
     }
   } else {
-#pragma unroll 8
-    for (int c = warp; c < C; c += kWarps) yp[(size_t)P * c] = fmaf(__ldg(g + c), (__ldg(xp + (size_t)P * c) - mean) * r, __ldg(b + c));
+#pragma unroll 4
+    for (int c = M::channel(0); c < C; c += kWarps * kPos) {
+      float const gc = __ldg(g + c), bc = __ldg(b + c);
+      M::load(v[0], xp + (size_t)P * c);
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) v[0][p] = fmaf(gc, (v[0][p] - mean[p]) * r[p], bc);
+      M::store(yp + (size_t)P * c, v[0]);
+    }
   }
 }
 
-// Sums over the lanes of kCount values (a power of two up to 32): lane l ends with the total of v[l % kCount].
-template <int kCount>
-__device__ __forceinline__ float lane_sums(float (&v)[kCount])
+// Sums over groups of kLanes neighbouring lanes of kCount values, both powers of two: lane l ends with v[0 ...] the totals of the values
+// l % kLanes % kCount * (kCount / kLanes) ... (kCount / kLanes of them, or one).
+template <int kLanes, int kCount>
+__device__ __forceinline__ void lane_sums(float (&v)[kCount])
 {
   int const lane = threadIdx.x & 31;
+  constexpr int kFew = kCount < kLanes ? kCount : kLanes;
 #pragma unroll
-  for (int s = kCount / 2; s > 0; s >>= 1) {
+  for (int s = kFew / 2, half = kCount / 2; s > 0; s >>= 1, half >>= 1) {
     bool const up = lane & s;
 #pragma unroll
-    for (int i = 0; i < s; ++i) {
-      float const send = up ? v[i] : v[i + s], keep = up ? v[i + s] : v[i];
+    for (int i = 0; i < kCount / 2; ++i) {
+      if (i >= half) break;
+      float const send = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
       v[i] = keep + __shfl_xor_sync(0xffffffffu, send, s);
     }
   }
-  float t = v[0];
 #pragma unroll
-  for (int s = kCount; s < 32; s <<= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
-  return t;
+  for (int s = kFew; s < kLanes; s <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], s);
 }
 
 // Tiles of 32 positions in turn to the blocks.  parts: [block][2][C].
-template <int kWarps, int kValues>
+template <int kWarps, int kPos, int kValues>
 __global__ void __launch_bounds__(kWarps * 32)
 maps_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
                 long long positions, int tiles, int P, int C, float eps)
 {
+  using M = Maps<kWarps, kPos>;
+  constexpr int kSums = 2 * kValues, kOwn = kSums > M::kLanes ? kSums / M::kLanes : 1;      // dG of the lane's channels, then dB; totals that a lane ends with
   vlb::pdl_wait();
-  __shared__ float red[2][4][kWarps][32];
-  int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ __align__(16) float red[2][4][kWarps][32];
+  int const lane = threadIdx.x & 31;
   float const n = (float)C;
-  float sum = 0.f;                       // lane l: the block's dG (l < kValues) or dB of channel warp + kWarps * (l % kValues)
+  float sum[kOwn] = {};
   int even = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, even ^= 1) {
-    Place const at = place_of(tile * 32ll + lane, positions, P, C);
+    Place const at = M::place(tile, positions, P, C);
     float const *const xp = x + at.at, *const dp = dy + at.at;
-    float v[kValues], d[kValues], m[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) { int const c = warp + kWarps * i; v[i] = c < C ? __ldg(xp + (size_t)P * c) : 0.f; }
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) { int const c = warp + kWarps * i; d[i] = c < C ? __ldg(dp + (size_t)P * c) : 0.f; }
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) m[0] += v[i];
-    lane_totals<kWarps>(m, red[even] + 3);
-    float const mean = m[0] / n;
-    float s[3] = {};
+    float v[kValues][kPos], d[kValues][kPos], m[1][kPos] = {};
 #pragma unroll
     for (int i = 0; i < kValues; ++i) {
-      int const c = warp + kWarps * i;
-      v[i] = c < C ? v[i] - mean : 0.f;
-      float const gd = c < C ? __ldg(g + c) * d[i] : 0.f;
-      s[0] += v[i] * v[i]; s[1] += gd; s[2] += gd * v[i];
-    }
-    lane_totals<kWarps>(s, red[even]);
-    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
-    if (parts) {
-      float t[2 * kValues];
 #pragma unroll
-      for (int i = 0; i < kValues; ++i) { t[i] = at.in ? d[i] * (v[i] * r) : 0.f; t[kValues + i] = at.in ? d[i] : 0.f; }
-      sum += lane_sums(t);
+      for (int p = 0; p < kPos; ++p) v[i][p] = 0.f;
+      if (M::channel(i) < C) M::load(v[i], xp + (size_t)P * M::channel(i));
+    }
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) {
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) d[i][p] = 0.f;
+      if (M::channel(i) < C) M::load(d[i], dp + (size_t)P * M::channel(i));
+    }
+#pragma unroll
+    for (int i = 0; i < kValues; ++i)
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) m[0][p] += v[i][p];
+    M::totals(m, red[even] + 3);
+    float s[3][kPos] = {}, mean[kPos];
+#pragma unroll
+    for (int p = 0; p < kPos; ++p) mean[p] = m[0][p] / n;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) {
+      float const gc = M::channel(i) < C ? __ldg(g + M::channel(i)) : 0.f;
+#pragma unroll
+      for (int p = 0; p < kPos; ++p) {
+        v[i][p] = M::channel(i) < C ? v[i][p] - mean[p] : 0.f;
+        float const gd = gc * d[i][p];
+        s[0][p] += v[i][p] * v[i][p]; s[1][p] += gd; s[2][p] += gd * v[i][p];
+      }
+    }
+    M::totals(s, red[even]);
+    float r[kPos], m1[kPos], m2[kPos];
+#pragma unroll
+    for (int p = 0; p < kPos; ++p) { r[p] = 1.f / sqrtf(s[0][p] / n + eps); m1[p] = s[1][p] / n; m2[p] = s[2][p] * r[p] / n; }
+    if (parts) {
+      float t[kSums] = {};
+#pragma unroll
+      for (int i = 0; i < kValues; ++i)
+#pragma unroll
+        for (int p = 0; p < kPos; ++p) { t[i] += at.in ? d[i][p] * (v[i][p] * r[p]) : 0.f; t[kValues + i] += at.in ? d[i][p] : 0.f; }
+      lane_sums<M::kLanes>(t);
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) sum[k] += t[k];
     }
     if (dx && at.in) {
 #pragma unroll
       for (int i = 0; i < kValues; ++i) {
-        int const c = warp + kWarps * i;
-        if (c < C) dx[at.at + (size_t)P * c] = r * (__ldg(g + c) * d[i] - m1 - v[i] * r * m2);
+        int const c = M::channel(i);
+        if (c >= C) break;
+        float const gc = __ldg(g + c);
+#pragma unroll
+        for (int p = 0; p < kPos; ++p) v[i][p] = r[p] * (gc * d[i][p] - m1[p] - v[i][p] * r[p] * m2[p]);
+        M::store(dx + at.at + (size_t)P * c, v[i]);
       }
     }
   }
-  if (!parts) return;
-  int const c = warp + kWarps * (lane % kValues);
-  if (c < C && lane < 2 * kValues) parts[(size_t)blockIdx.x * 2 * C + (lane < kValues ? 0 : C) + c] = sum;
+  if (!parts || lane % M::kLanes >= kSums) return;
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    int const which = lane % M::kLanes * kOwn + k, c = M::channel(which % kValues);
+    if (c < C) parts[(size_t)blockIdx.x * 2 * C + (which < kValues ? 0 : C) + c] = sum[k];
+  }
 }
 
 // Any number of channels: the values are read again for each pass, the block's sums over positions are kept in parts themselves.
@@ -383,28 +527,29 @@ maps_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
                      long long positions, int tiles, int P, int C, float eps)
 {
   vlb::pdl_wait();
-  __shared__ float red[2][4][kWarps][32];
+  using M = Maps<kWarps, 1>;
+  __shared__ __align__(16) float red[2][4][kWarps][32];
   int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float const n = (float)C;
   float* const own = parts ? parts + (size_t)blockIdx.x * 2 * C : nullptr;
   int even = 0;
   bool first = true;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, even ^= 1, first = false) {
-    Place const at = place_of(tile * 32ll + lane, positions, P, C);
+    Place const at = M::place(tile, positions, P, C);
     float const *const xp = x + at.at, *const dp = dy + at.at;
-    float m[1] = {0.f};
+    float m[1][1] = {};
 #pragma unroll 8
-    for (int c = warp; c < C; c += kWarps) m[0] += __ldg(xp + (size_t)P * c);
-    lane_totals<kWarps>(m, red[even] + 3);
-    float const mean = m[0] / n;
-    float s[3] = {};
+    for (int c = warp; c < C; c += kWarps) m[0][0] += __ldg(xp + (size_t)P * c);
+    M::totals(m, red[even] + 3);
+    float const mean = m[0][0] / n;
+    float s[3][1] = {};
 #pragma unroll 4
     for (int c = warp; c < C; c += kWarps) {
       float const v = __ldg(xp + (size_t)P * c) - mean, gd = __ldg(g + c) * __ldg(dp + (size_t)P * c);
-      s[0] += v * v; s[1] += gd; s[2] += gd * v;
+      s[0][0] += v * v; s[1][0] += gd; s[2][0] += gd * v;
     }
-    lane_totals<kWarps>(s, red[even]);
-    float const r = 1.f / sqrtf(s[0] / n + eps), m1 = s[1] / n, m2 = s[2] * r / n;
+    M::totals(s, red[even]);
+    float const r = 1.f / sqrtf(s[0][0] / n + eps), m1 = s[1][0] / n, m2 = s[2][0] * r / n;
     for (int c0 = warp; c0 < C; c0 += kWarps * 16) {
       float t[32];
 #pragma unroll
@@ -415,7 +560,8 @@ maps_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
         t[i] = at.in ? d * xh : 0.f; t[16 + i] = at.in ? d : 0.f;
       }
       if (own) {
-        float const sum = lane_sums(t);
+        lane_sums<32>(t);
+        float const sum = t[0];
         int const c = c0 + kWarps * (lane % 16);
         float* const p = own + (lane < 16 ? 0 : C) + c;
         if (c < C) *p = first ? sum : *p + sum;
@@ -492,12 +638,20 @@ int vlb_lnorm_forward(vlb_ctx* ctx, float* Y, float const* X, float const* g, fl
   if (!done) {
     unsigned const grid = (unsigned)vlb::ceil_div(positions, 32);
     auto run = [&](auto kernel, int warps) { vlb::launch(ctx->stream, kernel, grid, warps * 32, 0, Y, X, g, b, (long long)positions, P, C, (float)eps); };
-    if (C <= 32)        run(maps_fwd_kernel<8, 4>, 8);
-    else if (C <= 128)  run(maps_fwd_kernel<8, 16>, 8);
-    else if (C <= 256)  run(maps_fwd_kernel<16, 16>, 16);
-    else if (C <= 512)  run(maps_fwd_kernel<16, 32>, 16);
-    else if (C <= 1024) run(maps_fwd_kernel<32, 32>, 32);
-    else                run(maps_fwd_kernel<32, 0>, 32);
+    if (wide(P, {Y, X})) {
+      if (C <= 32)        run(maps_fwd_kernel<8, 4, 1>, 8);
+      else if (C <= 128)  run(maps_fwd_kernel<8, 4, 4>, 8);
+      else if (C <= 256)  run(maps_fwd_kernel<8, 4, 8>, 8);
+      else if (C <= 512)  run(maps_fwd_kernel<16, 4, 8>, 16);
+      else if (C <= 1024) run(maps_fwd_kernel<32, 4, 8>, 32);
+      else                run(maps_fwd_kernel<32, 4, 0>, 32);
+    } else {
+      if (C <= 32)        run(maps_fwd_kernel<8, 1, 4>, 8);
+      else if (C <= 128)  run(maps_fwd_kernel<8, 1, 16>, 8);
+      else if (C <= 256)  run(maps_fwd_kernel<16, 1, 16>, 16);
+      else if (C <= 512)  run(maps_fwd_kernel<16, 1, 32>, 16);
+      else                run(maps_fwd_kernel<32, 1, 0>, 32);
+    }
   }
   VLB_LAUNCHED(ctx, 1);
   return vlb::check_launch(ctx, "vlb_lnorm_forward");
@@ -518,16 +672,25 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
     if (!parts) return vlb::pass_error(ctx, ctx->lastError, "vlb_lnorm_backward");
   }
   int blocks = 0;
+  cudaError_t failed = cudaSuccess;
   if (P == 1) {
     bool const vec = wide(C, {dX, X, g, dY});
     with_row(C, [&](auto threads, auto count) {
       constexpr int kThreads = decltype(threads)::value, kVec = decltype(count)::value, kRows = block_of(kThreads) / kThreads;
-      // as many blocks as fit the device at once: half of its threads with sixteen values each of three tensors in registers
-      int const perSm = std::max(1, std::min(4, 512 / block_of(kThreads)));
-      blocks = std::min(vlb::ceil_div(N, kRows), std::min(kMaxParts, ctx->smCount * perSm));
+      // as many blocks as fit the device at once: half of its threads, with sixteen values each of three tensors in registers; groups of rows of 16 KB
+      int const perSm = std::max(1, std::min(4, 512 / block_of(kThreads))), per = kThreads == 32 ? std::max(1, std::min(4096 / (C * kRows), N / (kRows * ctx->smCount * perSm))) : 1;
+      blocks = std::min(vlb::ceil_div(N, kRows * per), std::min(kMaxParts, ctx->smCount * perSm));
       auto const kernel = vec ? rows_bwd_kernel<kThreads, kVec, true> : rows_bwd_kernel<kThreads, kVec, false>;
-      vlb::launch(ctx->stream, kernel, (unsigned)blocks, block_of(kThreads), 0, dX, parts, X, g, dY, N, C, (float)eps);
+      size_t const smem = vec ? sizeof(float) * kStages * 2 * per * kRows * C : 0;
+      static bool ready[64];                               // (of this kernel and device)
+      if (smem > 32 * 1024 && !ready[ctx->device & 63]) {
+        failed = vlb::allow_max_dynamic_smem(kernel);
+        ready[ctx->device & 63] = failed == cudaSuccess;
+      }
+      if (failed == cudaSuccess)
+        vlb::launch(ctx->stream, kernel, (unsigned)blocks, block_of(kThreads), smem, dX, parts, X, g, dY, N, C, per, (float)eps, ctx->deviceStatus);
     });
+    if (failed != cudaSuccess) return vlb::set_error(ctx, VLB_Cuda, cudaGetErrorString(failed));
     if (!blocks) {
       blocks = std::min(N, ctx->smCount * 2);
       vlb::launch(ctx->stream, rows_bwd_long_kernel, (unsigned)blocks, 1024, 0, dX, parts, X, g, dY, N, C, (float)eps);
@@ -539,10 +702,11 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
       blocks = std::min(tiles, std::min(kMaxParts, ctx->smCount * std::max(1, std::min(4, 32 / warps))));
       vlb::launch(ctx->stream, kernel, (unsigned)blocks, warps * 32, 0, dX, parts, X, g, dY, (long long)positions, tiles, P, C, (float)eps);
     };
-    if (C <= 32)       run(maps_bwd_kernel<8, 4>, 8);
-    else if (C <= 128) run(maps_bwd_kernel<8, 16>, 8);
-    else if (C <= 256) run(maps_bwd_kernel<16, 16>, 16);
-    else if (C <= 512) run(maps_bwd_kernel<32, 16>, 32);
+    bool const four = wide(P, {dX, X, dY});
+    if (C <= 32)       four ? run(maps_bwd_kernel<8, 4, 1>, 8) : run(maps_bwd_kernel<8, 1, 4>, 8);
+    else if (C <= 128) four ? run(maps_bwd_kernel<8, 4, 4>, 8) : run(maps_bwd_kernel<8, 1, 16>, 8);
+    else if (C <= 256) four ? run(maps_bwd_kernel<16, 4, 4>, 16) : run(maps_bwd_kernel<16, 1, 16>, 16);
+    else if (C <= 512) four ? run(maps_bwd_kernel<32, 4, 4>, 32) : run(maps_bwd_kernel<32, 1, 16>, 32);
     else               run(maps_bwd_long_kernel<16>, 16);
   }
   VLB_LAUNCHED(ctx, 1);
