@@ -186,7 +186,7 @@ constexpr size_t kMostScratch = 1u << 30;   // what the pieces of classes may ta
 struct Plan {
   int images, piece;                        // images at a time, classes at a time
   size_t bytes;
-  unsigned* largest;                        // of X, of the piece of F
+  unsigned *largest, *partial;              // of X, of the piece of F
   char *x, *f, *dz, *split;
   float2* parts; float *label, *lse, *db;
   double* sums;
@@ -201,6 +201,7 @@ struct Plan {
     bytes = 0;
     auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
     largest = (unsigned*)take(256);
+    partial = (unsigned*)take(2 * sizeof(unsigned) * vlb::kPairPartials);
     x = take(vlb::pair_bytes(images, D));
     f = take(vlb::pair_bytes(piece, D));
     split = take(vlb::kPairSplitBytes);
@@ -230,25 +231,16 @@ struct Problem {
   int N, D, K;
 };
 
-// The pair of a piece of F.
-vlb::Pair filters(Problem const& q, Plan const& plan, int k0, int cols)
-{
-  float const* const f = q.F + (size_t)k0 * q.D;
-  vlb::Pair const to = vlb::pair_at(plan.f, cols, q.D);
-  cudaMemsetAsync(plan.largest + 1, 0, sizeof(unsigned), q.ctx->stream);
-  vlb::largest_of(q.ctx, plan.largest + 1, f, cols, q.D, nullptr, 0);
-  vlb::make_pair(q.ctx, to, f, plan.largest + 1, nullptr, 0);
-  return to;
-}
+// The pair of a piece of F, and before the first piece that of the images n0 ....
+struct Sides { vlb::Pair x, f; };
 
-vlb::Pair images(Problem const& q, Plan const& plan, int n0, int rows)
+Sides sides(Problem const& q, Plan const& plan, int n0, int k0, bool withImages)
 {
-  float const* const x = q.X + (size_t)n0 * q.D;
-  vlb::Pair const to = vlb::pair_at(plan.x, rows, q.D);
-  cudaMemsetAsync(plan.largest, 0, sizeof(unsigned), q.ctx->stream);
-  vlb::largest_of(q.ctx, plan.largest, x, rows, q.D, q.labels + n0, q.K);
-  vlb::make_pair(q.ctx, to, x, plan.largest, q.labels + n0, q.K);
-  return to;
+  int const rows = std::min(plan.images, q.N - n0), cols = std::min(plan.piece, q.K - k0);
+  Sides const s = {vlb::pair_at(plan.x, rows, q.D), vlb::pair_at(plan.f, cols, q.D)};
+  vlb::PairSource const from[2] = {{s.f, q.F + (size_t)k0 * q.D, plan.largest + 1, nullptr, 0}, {s.x, q.X + (size_t)n0 * q.D, plan.largest, q.labels + n0, q.K}};
+  vlb::make_pairs(q.ctx, from, withImages ? 2 : 1, plan.partial);
+  return s;
 }
 
 vlb::PairProduct predictions(Problem const& q, Plan const& plan, vlb::Pair x, vlb::Pair f, int n0, int k0)
@@ -263,19 +255,20 @@ vlb::PairProduct predictions(Problem const& q, Plan const& plan, vlb::Pair x, vl
   return p;
 }
 
-// lse of images n0 ... and, after the last of them, the loss (either may be null).
-int seen(Problem const& q, Plan const& plan, vlb::Pair x, int n0, float* lse, float* loss, int* status)
+// lse of images n0 ... and, after the last of them, the loss (either may be null).  The pairs of the images and of the last piece are left.
+int seen(Problem const& q, Plan const& plan, int n0, float* lse, float* loss, int* status)
 {
   int count = 0;
+  int const rows = std::min(plan.images, q.N - n0);
   for (int k0 = 0; k0 < q.K; k0 += plan.piece) {
-    vlb::Pair const f = filters(q, plan, k0, std::min(plan.piece, q.K - k0));
-    vlb::PairProduct p = predictions(q, plan, x, f, n0, k0);
-    p.e.parts = plan.parts + (size_t)count * x.rows; p.e.label = plan.label;
+    Sides const s = sides(q, plan, n0, k0, k0 == 0);
+    vlb::PairProduct p = predictions(q, plan, s.x, s.f, n0, k0);
+    p.e.parts = plan.parts + (size_t)count * rows; p.e.label = plan.label;
     int const tile = vlb::pair_tile(q.ctx, &p, 1);
     if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairSeen, &p, 1, plan.split, tile)) return rc;
-    count += vlb::pair_parts(f.rows, tile);
+    count += vlb::pair_parts(s.f.rows, tile);
   }
-  vlb::launch(q.ctx->stream, lse_kernel, (unsigned)vlb::ceil_div(x.rows, 32), 1024, 0, loss, lse, plan.parts, count, plan.label, q.labels + n0, x.rows, n0,
+  vlb::launch(q.ctx->stream, lse_kernel, (unsigned)vlb::ceil_div(rows, 32), 1024, 0, loss, lse, plan.parts, count, plan.label, q.labels + n0, rows, n0,
               q.N, q.K, plan.sums, vlb::ceil_div(q.N, 32), q.ctx->deviceStatus + 64 + 4095, status);
   VLB_LAUNCHED(q.ctx, 1);
   return VLB_Success;
@@ -287,10 +280,8 @@ int forward_on_pairs(Problem const& q, float* loss, float* lse)
   if (!plan_for(q.ctx, plan, q.N, q.D, q.K, false)) return q.ctx->lastError;
   vlb::ProfScope prof(q.ctx, vlb::kProfFc);
   prof.rec.flops = 2.0 * q.N * q.D * q.K;
-  for (int n0 = 0; n0 < q.N; n0 += plan.images) {
-    vlb::Pair const x = images(q, plan, n0, std::min(plan.images, q.N - n0));
-    if (int const rc = seen(q, plan, x, n0, lse ? lse + n0 : nullptr, loss, q.ctx->deviceStatus)) return rc;
-  }
+  for (int n0 = 0; n0 < q.N; n0 += plan.images)
+    if (int const rc = seen(q, plan, n0, lse ? lse + n0 : nullptr, loss, q.ctx->deviceStatus)) return rc;
   return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_forward");
 }
 
@@ -301,12 +292,12 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
   vlb::ProfScope prof(q.ctx, vlb::kProfFc);
   prof.rec.flops = 2.0 * q.N * q.D * q.K * ((dX ? 1 : 0) + (dF ? 1 : 0) + (lse ? 1 : 2));
   for (int n0 = 0; n0 < q.N; n0 += plan.images) {
-    vlb::Pair const x = images(q, plan, n0, std::min(plan.images, q.N - n0));
     if (!lse)
-      if (int const rc = seen(q, plan, x, n0, plan.lse, nullptr, nullptr)) return rc;
+      if (int const rc = seen(q, plan, n0, plan.lse, nullptr, nullptr)) return rc;
     for (int k0 = 0; k0 < q.K; k0 += plan.piece) {
       int const cols = std::min(plan.piece, q.K - k0);
-      vlb::Pair const f = filters(q, plan, k0, cols), dz = vlb::pair_at(plan.dz, x.rows, cols);
+      Sides const s = sides(q, plan, n0, k0, lse && k0 == 0);
+      vlb::Pair const x = s.x, f = s.f, dz = vlb::pair_at(plan.dz, x.rows, cols);
       vlb::PairProduct p = predictions(q, plan, x, f, n0, k0);
       p.e.lse = lse ? lse + n0 : plan.lse;
       p.e.to = dz; p.e.toExp = kDzExp; p.e.db = db ? plan.db : nullptr;
@@ -357,6 +348,7 @@ struct FewArgs {
   int N, D, K;
   int* status;
   float2* parts; float* label;                // forward: parts[block * N + n]
+  float *loss, *lseOut; int* ticket;          // and the results, from the block that is through last
   float *dz, *db; float scale;                // backward: dz[class * kImages + n]
 };
 
@@ -454,10 +446,41 @@ few_predict_kernel(FewArgs a)
   __shared__ Part all[kFewWarps][kFew];
   if (lane < kImages) all[warp][lane] = p;
   __syncthreads();
-  if (threadIdx.x < a.N) {
-    p = all[0][threadIdx.x];
-    for (int w = 1; w < kFewWarps; ++w) p = together(p, all[w][threadIdx.x]);
-    a.parts[blockIdx.x * a.N + threadIdx.x] = make_float2(p.top, p.sum);
+  __shared__ bool last;
+  __shared__ double term[kFew];
+  if (threadIdx.x < 32) {
+    if (lane < a.N) {
+      p = all[0][lane];
+      for (int w = 1; w < kFewWarps; ++w) p = together(p, all[w][lane]);
+      __stcg(a.parts + blockIdx.x * a.N + lane, make_float2(p.top, p.sum));
+    }
+    __threadfence();
+    __syncwarp();
+    if (lane == 0) last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  if (warp < a.N) {
+    p = {-INFINITY, 0.f};
+    for (int i = lane; i < (int)gridDim.x; i += 32) { float2 const q = __ldcg(a.parts + i * a.N + warp); p = together(p, {q.x, q.y}); }
+    for (int s = 1; s < 32; s <<= 1) {
+      Part const q = {__shfl_xor_sync(0xffffffffu, p.top, s), __shfl_xor_sync(0xffffffffu, p.sum, s)};
+      p = lane & s ? together(q, p) : together(p, q);
+    }
+    if (lane == 0) {
+      bool const real = info[0][warp] > 0.f;
+      float const v = real ? p.top + logf(p.sum) : 0.f;
+      term[warp] = real ? (double)v - __ldcg(a.label + warp) : 0.;
+      if (a.lseOut) a.lseOut[warp] = v;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double sum = 0;
+    for (int i = 0; i < a.N; ++i) sum += term[i];
+    if (a.loss) *a.loss = (float)(sum / a.N);
+    *a.ticket = 0;
   }
 }
 
@@ -577,20 +600,16 @@ FewArgs few_args(Problem const& q)
 }
 
 // lse and loss (either may be null); scratch: few_scratch(q) bytes.
-size_t few_scratch(Problem const& q) { return (sizeof(float2) * q.ctx->smCount + 2 * sizeof(float)) * kFew + 64; }
+size_t few_scratch(Problem const& q) { return (sizeof(float2) * q.ctx->smCount + sizeof(float)) * kFew; }
 
 int few_seen(Problem const& q, float* loss, float* lse, char* scratch, int* status)
 {
   FewArgs a = few_args(q);
   a.parts = (float2*)scratch;
   a.label = (float*)(a.parts + (size_t)q.ctx->smCount * kFew);
-  double* const sums = (double*)(a.label + kFew);
+  a.loss = loss; a.lseOut = lse; a.ticket = q.ctx->deviceStatus + 64 + 4095; a.status = status;
   int blocks = 0;
-  if (int const rc = few_predict<false>(q, a, blocks)) return rc;
-  vlb::launch(q.ctx->stream, lse_kernel, 1, 1024, 0, loss, lse, a.parts, blocks, a.label, q.labels, q.N, 0, q.N, q.K, sums, 1,
-              q.ctx->deviceStatus + 64 + 4095, status);
-  VLB_LAUNCHED(q.ctx, 1);
-  return VLB_Success;
+  return few_predict<false>(q, a, blocks);
 }
 
 int forward_few(Problem const& q, float* loss, float* lse)

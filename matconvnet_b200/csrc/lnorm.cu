@@ -440,7 +440,7 @@ __device__ __forceinline__ void lane_sums(float (&v)[kCount])
 
 // Tiles of 32 positions in turn to the blocks.  parts: [block][2][C].
 template <int kWarps, int kPos, int kValues>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 && kPos * kValues < 16 ? 2 : 1)
 maps_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
                 long long positions, int tiles, int P, int C, float eps)
 {
@@ -704,7 +704,7 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
     };
     bool const four = wide(P, {dX, X, dY});
     if (C <= 32)       four ? run(maps_bwd_kernel<8, 4, 1>, 8) : run(maps_bwd_kernel<8, 1, 4>, 8);
-    else if (C <= 128) four ? run(maps_bwd_kernel<8, 4, 4>, 8) : run(maps_bwd_kernel<8, 1, 16>, 8);
+    else if (C <= 128) four ? run(maps_bwd_kernel<8, 4, 4>, 8) : run(maps_bwd_kernel<16, 1, 8>, 16);
     else if (C <= 256) four ? run(maps_bwd_kernel<16, 4, 4>, 16) : run(maps_bwd_kernel<16, 1, 16>, 16);
     else if (C <= 512) four ? run(maps_bwd_kernel<32, 4, 4>, 32) : run(maps_bwd_kernel<32, 1, 16>, 32);
     else               run(maps_bwd_long_kernel<16>, 16);

@@ -43,6 +43,7 @@ template <int kMax> struct Batch {
   CUtensorMap map[4 * kMax];                            // of each product A along its rows, along its columns, B likewise; those that are used
   Product p[kMax];
   int count, work, three;
+  int early;                                            // few CTAs: the next launch may take the other SMs right away
   float* split;
   int* tickets;
   int* status;
@@ -407,6 +408,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
   if (kCtas == 2) cluster_sync();
   tc_fence_after();
   uint32_t const tmem = tmemAt;
+  if (batch.early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   vlb::pdl_wait();
 
   bool dead = false;                 // a wait ran out: nothing is waited for any more, the work is walked through to the end
@@ -578,30 +580,40 @@ __device__ __forceinline__ unsigned finite_bits(float v)
 }
 
 constexpr int kSplitThreads = 256;
+constexpr int kSegment = 1024;                // floats of a row that a warp takes at a time
 
-// Rows in turn to the grid's warps.
+struct SplitJob {
+  vlb::PairSource s;
+  unsigned* partial;                          // largest magnitude seen by each block of largest_kernel
+  int block0, blocks, segments;               // blocks of largest_kernel; segments of a row
+  int pair0, pairs, rowsPer, vec;             // blocks of make_pair_kernel, their rows at a time
+  vlb::FastDiv perRow;
+};
+struct SplitJobs { SplitJob j[2]; int count; };
+
 __global__ void __launch_bounds__(kSplitThreads)
-largest_kernel(unsigned* largest, float const* __restrict__ x, int rows, int cols, float const* __restrict__ labels, int classes, bool vec)
+largest_kernel(const __grid_constant__ SplitJobs jobs)
 {
   vlb::pdl_wait();
-  int const lane = threadIdx.x & 31, warps = (int)gridDim.x * (kSplitThreads / 32);
+  SplitJob const& j = jobs.j[jobs.count > 1 && (int)blockIdx.x >= jobs.j[1].block0];
+  int const lane = threadIdx.x & 31, block = (int)blockIdx.x - j.block0, cols = j.s.to.cols;
+  long long const units = (long long)j.s.to.rows * j.segments;
   unsigned m = 0;
-  if (!labels && vec) {                                       // one run of floats
-    long long const n = (long long)rows * cols / 4, step = (long long)gridDim.x * kSplitThreads;
-    float4 const* const v = (float4 const*)x;
-    for (long long i = (long long)blockIdx.x * kSplitThreads + threadIdx.x; i < n; i += 4 * step) {
-      float4 q[4];
+  for (long long u = (long long)block * (kSplitThreads / 32) + (threadIdx.x >> 5); u < units; u += (long long)j.blocks * (kSplitThreads / 32)) {
+    long long const row = u / j.segments;
+    int const c0 = (int)(u - row * j.segments) * kSegment, c1 = min(c0 + kSegment, cols);
+    if (!is_real(j.s.labels, row, j.s.classes)) continue;
+    float const* const x = j.s.x + row * cols;
+    if (j.vec) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) q[k] = __ldg(v + min(i + k * step, n - 1));
-#pragma unroll
-      for (int k = 0; k < 4; ++k) m = max(max(m, max(finite_bits(q[k].x), finite_bits(q[k].y))), max(finite_bits(q[k].z), finite_bits(q[k].w)));
-    }
-  } else {
-    for (int r = (int)blockIdx.x * (kSplitThreads / 32) + (int)(threadIdx.x >> 5); r < rows; r += warps) {
-      if (!is_real(labels, r, classes)) continue;
-      float const* const row = x + (long long)r * cols;
-#pragma unroll 4
-      for (int c = lane; c < cols; c += 32) m = max(m, finite_bits(__ldg(row + c)));
+      for (int i = 0; i < kSegment / 128; ++i) {
+        int const c = c0 + 4 * (lane + 32 * i);
+        float4 const q = c < c1 ? __ldg((float4 const*)(x + c)) : make_float4(0, 0, 0, 0);
+        m = max(max(m, max(finite_bits(q.x), finite_bits(q.y))), max(finite_bits(q.z), finite_bits(q.w)));
+      }
+    } else {
+#pragma unroll 8
+      for (int c = c0 + lane; c < c1; c += 32) m = max(m, finite_bits(__ldg(x + c)));
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
@@ -610,39 +622,52 @@ largest_kernel(unsigned* largest, float const* __restrict__ x, int rows, int col
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < kSplitThreads / 32; ++i) m = max(m, all[i]);
-    if (m) atomicMax(largest, m);                             // (the largest does not depend on the order)
+    j.partial[block] = m;
   }
 }
 
-// A block takes rowsPer rows, a thread sixteen neighbouring columns at a time.
+// A block takes rowsPer rows at a time, a thread sixteen neighbouring columns.
 __global__ void __launch_bounds__(kSplitThreads)
-make_pair_kernel(Pair to, float const* __restrict__ x, unsigned const* __restrict__ largest, float const* __restrict__ labels, int classes, int rowsPer,
-                 vlb::FastDiv perRow, bool vec)
+make_pair_kernel(const __grid_constant__ SplitJobs jobs)
 {
   vlb::pdl_wait();
-  float const f = pow2(vlb::pair_exp(__uint_as_float(__ldg(largest))));
+  SplitJob const& j = jobs.j[jobs.count > 1 && (int)blockIdx.x >= jobs.j[1].pair0];
+  int const block = (int)blockIdx.x - j.pair0;
+  unsigned m = 0;
+  for (int i = threadIdx.x; i < j.blocks; i += kSplitThreads) m = max(m, __ldg(j.partial + i));
+  m = __reduce_max_sync(0xffffffffu, m);
+  __shared__ unsigned all[kSplitThreads / 32];
+  if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = all[0];
+#pragma unroll
+  for (int i = 1; i < kSplitThreads / 32; ++i) m = max(m, all[i]);
+  if (block == 0 && threadIdx.x == 0) *j.s.largest = m;
+  vlb::Pair const& to = j.s.to;
+  float const f = pow2(vlb::pair_exp(__uint_as_float(m)));
   int const groups = (int)(to.ld / 16);
-  for (int t = threadIdx.x; t < rowsPer * groups; t += kSplitThreads) {
-    int const r = perRow(t), c = (t - r * groups) * 16;
-    long long const row = (long long)blockIdx.x * rowsPer + r;
-    if (row >= to.rows) break;
-    float v[16];
-    bool const real = is_real(labels, row, classes);
-    float const* const p = x + row * to.cols + c;
-    if (vec && c + 16 <= to.cols) {
+  for (long long row0 = (long long)block * j.rowsPer; row0 < to.rows; row0 += (long long)j.pairs * j.rowsPer)
+    for (int t = threadIdx.x; t < j.rowsPer * groups; t += kSplitThreads) {
+      int const r = j.perRow(t), c = (t - r * groups) * 16;
+      long long const row = row0 + r;
+      if (row >= to.rows) break;
+      float v[16];
+      bool const real = is_real(j.s.labels, row, j.s.classes);
+      float const* const p = j.s.x + row * to.cols + c;
+      if (j.vec && c + 16 <= to.cols) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float4 const q = __ldg((float4 const*)p + i);
-        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+        for (int i = 0; i < 4; ++i) {
+          float4 const q = __ldg((float4 const*)p + i);
+          v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = c + i < to.cols ? __ldg(p + i) : 0.f;
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = c + i < to.cols ? __ldg(p + i) : 0.f;
+      for (int i = 0; i < 16; ++i) v[i] = real ? v[i] * f : 0.f;
+      store_pair16(to, row, c, v);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = real ? v[i] * f : 0.f;
-    store_pair16(to, row, c, v);
-  }
 }
 
 // ------------------------------------------------------------------ host
@@ -670,6 +695,23 @@ int tiles_of(PairProduct const& p, int tile)
   return p.symmetric ? m * (m + 1) / 2 : m * n;
 }
 
+// Microseconds that a tile takes, measured: per k-block; for the hand-over of partial sums and for each of them; for its beginning and end.
+struct TileCost { double block, cut, part, ends; };
+constexpr TileCost kCost[2] = {{0.5, 3., 0.55, 4.}, {0.95, 3., 1.1, 6.}};           // 128 x 128 on one CTA, 256 x 256 on two
+
+// Ranges of a reduction of kBlocks k-blocks where there are fewer tiles than places: the number that takes least time as long as all of them run at once.
+int splits_of(int kBlocks, long long tiles, int clusters, int ctas)
+{
+  TileCost const& c = kCost[ctas - 1];
+  int best = 1;
+  double least = kBlocks * c.block;
+  for (int s = 2; s <= 64 && s * tiles <= clusters && 2 * s <= kBlocks; ++s) {
+    double const t = vlb::ceil_div(kBlocks, s) * c.block + c.cut + s * c.part;
+    if (t < least) { least = t; best = s; }
+  }
+  return best;
+}
+
 template <int kKind, int kMax, int kCtas>
 int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
 {
@@ -677,14 +719,8 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
   Batch<kMax> b;
   b.three = ctx->precision != VLB_PRECISION_TF32;
   int const clusters = ctx->smCount / kCtas;
-  long long tiles = 0, blocks = 0;
-  for (int i = 0; i < count; ++i) {
-    int const t = tiles_of(p[i], kTile);
-    tiles += t;
-    blocks += (long long)t * vlb::ceil_div(p[i].K, kDepth);
-  }
-  // Fewer tiles than places to run them: reductions are cut into ranges of about the same length that fill the places, of eight k-blocks at least
-  long long const range = std::max<long long>(8, (blocks + clusters - 1) / clusters);
+  long long tiles = 0;
+  for (int i = 0; i < count; ++i) tiles += tiles_of(p[i], kTile);
   size_t const partBytes = sizeof(float) * 128 * kTile;
   int slot = 0;
   long long part = 0, work = 0;
@@ -695,10 +731,8 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
     d.tilesM = vlb::ceil_div(q.M, kTile); d.tilesN = vlb::ceil_div(q.N, kTile);
     int const t = tiles_of(q, kTile);
     d.splits = 1;
-    if (tiles < clusters) {
-      int const s = (int)std::min<long long>((d.kBlocks + range - 1) / range, 64);
-      if (s > 1 && (slot + t) * kCtas <= 4096 && (size_t)((part + (long long)t * s) * kCtas) * partBytes <= vlb::kPairSplitBytes) d.splits = s;
-    }
+    int const t2 = splits_of(d.kBlocks, tiles, clusters, kCtas);
+    if (t2 > 1 && (slot + t) * kCtas < 4095 && (size_t)((part + (long long)t * t2) * kCtas) * partBytes <= vlb::kPairSplitBytes) d.splits = t2;
     d.slot0 = slot; d.part0 = part;
     if (d.splits > 1) { slot += t; part += (long long)t * d.splits; }
     work += (long long)t * d.splits;
@@ -710,6 +744,8 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
   }
   if (work > INT32_MAX) return vlb::set_error(ctx, VLB_IllegalArgument, "the matrices are too large");
   b.count = count; b.work = (int)work;
+  // The next launch's blocks are set up on the free SMs while this one runs, and wait there for its end (pdl_wait): Muon on one 3x3x64x64 bank EARLYFIG.
+  b.early = std::min<long long>(clusters, work) * kCtas * 2 <= ctx->smCount;
   b.split = (float*)split;
   b.tickets = ctx->deviceStatus + 64;
   b.status = ctx->deviceStatus;
@@ -746,33 +782,49 @@ int run_kind(vlb_ctx* ctx, PairProduct const* p, int count, void* split, int til
 
 namespace vlb {
 
-void largest_of(vlb_ctx* ctx, unsigned* largest, float const* x, int rows, int cols, float const* labels, int classes)
+void make_pairs(vlb_ctx* ctx, PairSource const* s, int count, unsigned* partial)
 {
-  bool const vec = ((uintptr_t)x & 15) == 0 && (long long)rows * cols % 4 == 0;
-  unsigned const grid = grid_for(!labels && vec ? (size_t)rows * cols / 16 + 1 : (size_t)rows * 32, kSplitThreads, ctx->smCount * 8);
-  launch(ctx->stream, largest_kernel, grid, kSplitThreads, 0, largest, x, rows, cols, labels, classes, vec);
-  VLB_LAUNCHED(ctx, 1);
+  SplitJobs jobs;
+  jobs.count = count;
+  int blocks = 0, pairs = 0;
+  for (int i = 0; i < count; ++i) {
+    SplitJob& j = jobs.j[i];
+    j.s = s[i];
+    j.partial = partial + i * kPairPartials;
+    j.segments = ceil_div(s[i].to.cols, kSegment);
+    j.vec = ((uintptr_t)s[i].x & 15) == 0 && s[i].to.cols % 4 == 0;
+    j.block0 = blocks;
+    j.blocks = (int)std::min<long long>(((long long)s[i].to.rows * j.segments + kSplitThreads / 32 - 1) / (kSplitThreads / 32), std::min(ctx->smCount * 6, kPairPartials));
+    int const groups = (int)(s[i].to.ld / 16);
+    j.rowsPer = std::max(1, 512 / groups);
+    j.perRow = FastDiv(groups);
+    j.pair0 = pairs;
+    j.pairs = std::min(ceil_div(s[i].to.rows, j.rowsPer), ctx->smCount * 8);
+    blocks += j.blocks; pairs += j.pairs;
+  }
+  launch(ctx->stream, largest_kernel, (unsigned)blocks, kSplitThreads, 0, jobs);
+  launch(ctx->stream, make_pair_kernel, (unsigned)pairs, kSplitThreads, 0, jobs);
+  VLB_LAUNCHED(ctx, 2);
 }
 
-void make_pair(vlb_ctx* ctx, Pair to, float const* x, unsigned const* largest, float const* labels, int classes)
-{
-  int const groups = (int)(to.ld / 16), rowsPer = std::max(1, 512 / groups);
-  bool const vec = ((uintptr_t)x & 15) == 0 && to.cols % 4 == 0;
-  launch(ctx->stream, make_pair_kernel, (unsigned)ceil_div(to.rows, rowsPer), kSplitThreads, 0, to, x, largest, labels, classes, rowsPer, FastDiv(groups), vec);
-  VLB_LAUNCHED(ctx, 1);
-}
-
-// By k-blocks through the tensor core: 1536 cycles for 256 x 256 on two SMs, 768 for 128 x 128 on one, and a hand-over between k-blocks that a pair's longer
-// ones hide.
 int pair_tile(vlb_ctx* ctx, PairProduct const* p, int count)
 {
-  double two = 0, one = 0;
-  for (int i = 0; i < count; ++i) {
-    double const kb = ceil_div(p[i].K, kDepth);
-    two += tiles_of(p[i], 256) * kb;
-    one += tiles_of(p[i], 128) * kb;
+  double time[2];
+  for (int ctas = 1; ctas <= 2; ++ctas) {
+    int const clusters = ctx->smCount / ctas;
+    TileCost const& c = kCost[ctas - 1];
+    long long tiles = 0;
+    for (int i = 0; i < count; ++i) tiles += tiles_of(p[i], 128 * ctas);
+    double sum = 0, longest = 0;
+    for (int i = 0; i < count; ++i) {
+      int const kb = ceil_div(p[i].K, kDepth), s = splits_of(kb, tiles, clusters, ctas);
+      double const t = ceil_div(kb, s) * c.block + c.ends + (s > 1 ? c.cut + s * c.part : 0);
+      sum += tiles_of(p[i], 128 * ctas) * (kb * c.block + c.ends);
+      longest = std::max(longest, t);
+    }
+    time[ctas - 1] = std::max(sum / clusters, longest);
   }
-  return two / (ctx->smCount / 2) * 1600. <= one / ctx->smCount * 950. ? 256 : 128;
+  return time[1] < time[0] ? 256 : 128;
 }
 
 int products_of_pairs(vlb_ctx* ctx, PairKind kind, PairProduct const* p, int count, void* split, int tile)

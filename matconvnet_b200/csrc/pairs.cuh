@@ -64,10 +64,13 @@ constexpr size_t kPairSplitBytes = 64u << 20;
 // Parts per row that kPairSeen writes of N columns.
 inline int pair_parts(int N, int tile) { return 2 * ceil_div(N, tile); }
 
-// The largest finite magnitude of rows x cols floats one after the other, as bits, into *largest, which holds zero or an earlier result; and that matrix as
-// a pair with the exponent of *largest.  labels (or NULL): rows whose label is not in 1 ... classes count as zeros, whatever they hold.
-void largest_of(vlb_ctx* ctx, unsigned* largest, float const* x, int rows, int cols, float const* labels, int classes);
-void make_pair(vlb_ctx* ctx, Pair to, float const* x, unsigned const* largest, float const* labels, int classes);
+// A matrix of floats, rows one after the other, to be made a pair: with the exponent of its largest finite magnitude, whose bits are left in *largest.
+// labels (or NULL): rows whose label is not in 1 ... classes count as zeros, whatever they hold.
+struct PairSource { Pair to; float const* x; unsigned* largest; float const* labels; int classes; };
+
+// One or two of them, in two launches.  partial: kPairPartials words of scratch for each.
+constexpr int kPairPartials = 1024;
+void make_pairs(vlb_ctx* ctx, PairSource const* s, int count, unsigned* partial);
 
 // The tiles, 256 x 256 or 128 x 128, that take less time for these products, all of them together.
 int pair_tile(vlb_ctx* ctx, PairProduct const* p, int count);
