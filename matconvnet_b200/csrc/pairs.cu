@@ -35,6 +35,7 @@ constexpr size_t kSmem = (size_t)kStages * kStageBytes + kDrainWarps * kPatch * 
 struct Product {
   int M, N, kBlocks, tilesM, tilesN, splits, work;      // work: items in front of and including this product's
   int byColsA, byColsB, lowerA, lowerB, symmetric;
+  int same;                                             // both sides are one matrix: a tile on the diagonal is loaded once
   int slot0; long long part0;                           // tickets and partial results in front of this product's, per CTA of a pair
   PairEpilogue e;
 };
@@ -153,11 +154,15 @@ __device__ __forceinline__ void free_tmem(uint32_t t)
 __device__ __forceinline__ uint4& patch_at(float* patch, int row, int place) { return ((uint4*)patch)[row * 8 + (place ^ (row & 7))]; }
 
 // Rows of 64 halves or 32 floats, `pitch` bytes apart, into or out of a lane's eight uint4; rows: those that exist.
-__device__ __forceinline__ void load_rows(uint4 (&v)[8], char const* from, long long pitch, int rows, float* patch)
+__device__ __forceinline__ void fetch_rows(uint4 (&v)[8], char const* from, long long pitch, int rows)
 {
   int const lane = threadIdx.x & 31, r0 = lane >> 3, c = lane & 7;
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = r0 + 4 * i < rows ? *(uint4 const*)(from + (r0 + 4 * i) * pitch + 16 * c) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void turn_rows(uint4 (&v)[8], float* patch)
+{
+  int const lane = threadIdx.x & 31, r0 = lane >> 3, c = lane & 7;
 #pragma unroll
   for (int i = 0; i < 8; ++i) patch_at(patch, r0 + 4 * i, c) = v[i];
   __syncwarp();
@@ -209,7 +214,7 @@ __device__ __forceinline__ void update_rows(float* out, long long ldc, int M, in
     float* const o = out + row0 * ldc + c0;
     if (vec && c0 + 32 <= N) {
       uint4 q[8];
-      if (readOld) load_rows(q, (char const*)o, ldc * 4, rows, patch);
+      if (readOld) { fetch_rows(q, (char const*)o, ldc * 4, rows); turn_rows(q, patch); }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         auto one = [&](uint32_t old, int k) { return __float_as_uint(combine(readOld ? __uint_as_float(old) : 0.f, acc[g * 32 + 4 * i + k])); };
@@ -355,15 +360,17 @@ __device__ __forceinline__ void finish_poly(Product const& p, float (&acc)[kCols
 #pragma unroll
     for (int i = 0; i < kCols; i += 64) {
       if (col0 + i >= e.add.ld) continue;
+      uint4 q[2][8];
+      fetch_rows(q[0], (char const*)(e.add.hi + row0 * e.add.ld + col0 + i), e.add.ld * 2, rows);
+      fetch_rows(q[1], (char const*)(e.add.lo + row0 * e.add.ld + col0 + i), e.add.ld * 2, rows);
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        uint4 q[8];
-        load_rows(q, (char const*)((part ? e.add.lo : e.add.hi) + row0 * e.add.ld + col0 + i), e.add.ld * 2, rows, patch);
+        turn_rows(q[part], patch);
         float const k = part ? fl : fh;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          two(q[c].x, k, acc[i + 8 * c], acc[i + 8 * c + 1]); two(q[c].y, k, acc[i + 8 * c + 2], acc[i + 8 * c + 3]);
-          two(q[c].z, k, acc[i + 8 * c + 4], acc[i + 8 * c + 5]); two(q[c].w, k, acc[i + 8 * c + 6], acc[i + 8 * c + 7]);
+          two(q[part][c].x, k, acc[i + 8 * c], acc[i + 8 * c + 1]); two(q[part][c].y, k, acc[i + 8 * c + 2], acc[i + 8 * c + 3]);
+          two(q[part][c].z, k, acc[i + 8 * c + 4], acc[i + 8 * c + 5]); two(q[part][c].w, k, acc[i + 8 * c + 6], acc[i + 8 * c + 7]);
         }
       }
     }
@@ -409,6 +416,11 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
   tc_fence_after();
   uint32_t const tmem = tmemAt;
   if (batch.early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 8 * 32 && first < batch.work) {       // the maps of the first item, on their way before there is anything to load
+    CUtensorMap const* const map = batch.map + 4 * item_of(batch, first).prod;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"(map + i) : "memory");
+  }
   vlb::pdl_wait();
 
   bool dead = false;                 // a wait ran out: nothing is waited for any more, the work is walked through to the end
@@ -494,6 +506,10 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
             int const s = it % kStages, before = it - kStages;
             if (before >= 0 && !mbar_wait(smem_u32(&done[before % kRing]), (uint32_t)(before / kRing) & 1u)) { dead = true; break; }
             uint32_t const mine = smem_u32(&full[s]), bar = kCtas == 2 ? in_first(mine) : mine;
+            if (!isA && p.same && t.tm == t.tn) {
+              if (rank == 0) mbar_arrive(mine);
+              continue;
+            }
             if (rank == 0) mbar_arrive_expect_tx(mine, bytes * kCtas);
             uint32_t const to = base + (uint32_t)s * kStageBytes + (isA ? 0u : 2u * kHalfTile);
             if (along_cols(byCols, lower, tile, kTileRows, kb)) {
@@ -531,7 +547,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
             uint32_t const idesc = (1u << 4) | (ca ? 1u << 15 : 0u) | (cb ? 1u << 16 : 0u) | ((uint32_t)(kTileCols >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
             uint64_t const stepA = (ca ? 2048u : 32u) >> 4, stepB = (cb ? 2048u : 32u) >> 4;
             uint64_t const aH = make_desc(st, kHalfTile, 1024), aL = aH + ((ca ? kHalfTile / 2 : kHalfTile) >> 4);
-            uint64_t const bH = make_desc(st + 2 * kHalfTile, kHalfTile, 1024), bL = bH + ((cb ? kHalfTile / 2 : kHalfTile) >> 4);
+            uint64_t const bH = p.same && t.tm == t.tn ? aH : make_desc(st + 2 * kHalfTile, kHalfTile, 1024), bL = bH + ((cb ? kHalfTile / 2 : kHalfTile) >> 4);
             if (batch.three) {
 #pragma unroll
               for (int k = 0; k < kDepth / 16; ++k) {
@@ -697,7 +713,7 @@ int tiles_of(PairProduct const& p, int tile)
 
 // Microseconds that a tile takes, measured: per k-block; for the hand-over of partial sums and for each of them; for its beginning and end.
 struct TileCost { double block, cut, part, ends; };
-constexpr TileCost kCost[2] = {{0.5, 3., 0.55, 4.}, {0.95, 3., 1.1, 6.}};           // 128 x 128 on one CTA, 256 x 256 on two
+constexpr TileCost kCost[2] = {{1., 3., 0.55, 5.}, {1., 3., 1.1, 7.}};           // 128 x 128 on one CTA, 256 x 256 on two
 
 // Ranges of a reduction of kBlocks k-blocks where there are fewer tiles than places: the number that takes least time as long as all of them run at once.
 int splits_of(int kBlocks, long long tiles, int clusters, int ctas)
@@ -738,6 +754,7 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
     work += (long long)t * d.splits;
     d.work = (int)work;
     d.byColsA = q.a.byCols; d.byColsB = q.b.byCols; d.lowerA = q.a.lower; d.lowerB = q.b.lower; d.symmetric = q.symmetric;
+    d.same = q.symmetric && q.a.m.hi == q.b.m.hi && q.a.byCols == q.b.byCols && q.a.lower == q.b.lower;
     d.e = q.e;
     if (!encode_side(&b.map[4 * i], q.a, b.three) || !encode_side(&b.map[4 * i + 2], q.b, b.three))
       return vlb::set_error(ctx, VLB_Cuda, "a tensor map could not be made");
