@@ -184,19 +184,24 @@ __device__ __forceinline__ void store_rows(uint4 const (&v)[8], char* to, long l
   __syncwarp();
 }
 
-__device__ __forceinline__ uint32_t two_halves(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16); }
+// Two values, scaled, as hi and lo: four instructions each.  An infinity leaves a not-a-number in lo (pair_of has the test that a matrix of any values needs; what
+// products and exponentials give here is finite, or has been spoilt already).
+__device__ __forceinline__ void two_pairs(float a, float b, uint32_t& hi, uint32_t& lo)
+{
+  __half2 const h = __floats2half2_rn(a, b);
+  float2 const f = __half22float2(h);
+  __half2 const l = __floats2half2_rn((a - f.x) * 2048.f, (b - f.y) * 2048.f);
+  hi = *(uint32_t const*)&h; lo = *(uint32_t const*)&l;
+}
 
-// 64 neighbouring values of a row per lane, scaled, into a pair.
-__device__ __forceinline__ void store_pair64(Pair const& to, int row0, int col, int rows, float const* v, float* patch)
+// 64 neighbouring values of a row per lane, times f, into a pair.
+__device__ __forceinline__ void store_pair64(Pair const& to, int row0, int col, int rows, float const* v, float f, float* patch)
 {
   uint4 hi[8], lo[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    __half h[8], l[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) vlb::pair_of(v[8 * i + k], h[k], l[k]);
-    hi[i] = make_uint4(two_halves(h[0], h[1]), two_halves(h[2], h[3]), two_halves(h[4], h[5]), two_halves(h[6], h[7]));
-    lo[i] = make_uint4(two_halves(l[0], l[1]), two_halves(l[2], l[3]), two_halves(l[4], l[5]), two_halves(l[6], l[7]));
+    two_pairs(v[8 * i] * f, v[8 * i + 1] * f, hi[i].x, lo[i].x); two_pairs(v[8 * i + 2] * f, v[8 * i + 3] * f, hi[i].y, lo[i].y);
+    two_pairs(v[8 * i + 4] * f, v[8 * i + 5] * f, hi[i].z, lo[i].z); two_pairs(v[8 * i + 6] * f, v[8 * i + 7] * f, hi[i].w, lo[i].w);
   }
   store_rows(hi, (char*)(to.hi + row0 * to.ld + col), to.ld * 2, rows, patch);
   store_rows(lo, (char*)(to.lo + row0 * to.ld + col), to.ld * 2, rows, patch);
@@ -238,40 +243,56 @@ __device__ __forceinline__ void update_rows(float* out, long long ldc, int M, in
   }
 }
 
-template <int kCols>
-__device__ __forceinline__ void finish_out(Product const& p, float (&acc)[kCols], int row0, int col0, float* patch)
+// What the epilogue of a tile takes from global memory, fetched before its products: the sides' scales, and for predictions the row's label and lse and, in the
+// warp's patch, the columns' biases (-inf beyond the last column).  Fetched when they are needed they cost 2 us per tile.
+struct Ahead { float fa, fb, label, lse; };
+
+template <int kKind, int kCols>
+__device__ __forceinline__ Ahead fetch_ahead(Product const& p, int row, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  float const fa = pow2(-exp_of(e.ea)), fb = pow2(-exp_of(e.eb)), alpha = e.alpha;
+  Ahead a = {pow2(-exp_of(e.ea)), pow2(-exp_of(e.eb)), 0.f, 0.f};
+  if (kKind == kPairSeen || kKind == kPairGrad) {
+    if (row < p.M) {
+      a.label = __ldg(e.labels + row);
+      if (kKind == kPairGrad) a.lse = __ldg(e.lse + row);
+    }
+#pragma unroll
+    for (int i = 0; i < kCols; i += 32) {
+      int const c = col0 + i + (int)(threadIdx.x & 31);
+      patch[i + (threadIdx.x & 31)] = c < p.N ? (e.bias ? __ldg(e.bias + c) : 0.f) : -INFINITY;
+    }
+    __syncwarp();
+  }
+  return a;
+}
+
+template <int kCols>
+__device__ __forceinline__ void finish_out(Product const& p, Ahead const& ahead, float (&acc)[kCols], int row0, int col0, float* patch)
+{
+  PairEpilogue const& e = p.e;
+  float const fa = ahead.fa, fb = ahead.fb, alpha = e.alpha;
   update_rows(e.out, e.ldc, p.M, p.N, e.beta != 0.f, acc, row0, col0, patch, [&](float old, float v) { return v * fa * fb * alpha + old; });
 }
 
-// predictions = product + bias in place, -inf beyond the last column.  The columns' biases go through the warp's patch: loaded side by side, read by all lanes.
+// predictions = product + bias in place, -inf beyond the last column
 template <int kCols>
-__device__ __forceinline__ void predictions(Product const& p, float (&acc)[kCols], int col0, float* patch)
+__device__ __forceinline__ void predictions(Ahead const& a, float (&acc)[kCols], float* patch)
 {
-  PairEpilogue const& e = p.e;
-  float const fa = pow2(-exp_of(e.ea)), fb = pow2(-exp_of(e.eb));
-#pragma unroll
-  for (int i = 0; i < kCols; i += 32) {
-    int const c = col0 + i + (int)(threadIdx.x & 31);
-    patch[i + (threadIdx.x & 31)] = c < p.N ? (e.bias ? __ldg(e.bias + c) : 0.f) : -INFINITY;
-  }
-  __syncwarp();
 #pragma unroll
   for (int i = 0; i < kCols; i += 4) {
     float4 const b = *(float4 const*)(patch + i);
-    acc[i] = fmaf(acc[i] * fa, fb, b.x); acc[i + 1] = fmaf(acc[i + 1] * fa, fb, b.y);
-    acc[i + 2] = fmaf(acc[i + 2] * fa, fb, b.z); acc[i + 3] = fmaf(acc[i + 3] * fa, fb, b.w);
+    acc[i] = fmaf(acc[i] * a.fa, a.fb, b.x); acc[i + 1] = fmaf(acc[i + 1] * a.fa, a.fb, b.y);
+    acc[i + 2] = fmaf(acc[i + 2] * a.fa, a.fb, b.z); acc[i + 3] = fmaf(acc[i + 3] * a.fa, a.fb, b.w);
   }
   __syncwarp();
 }
 
 template <int kCols>
-__device__ __forceinline__ void finish_seen(Product const& p, float (&acc)[kCols], int row, int col0, float* patch)
+__device__ __forceinline__ void finish_seen(Product const& p, Ahead const& ahead, float (&acc)[kCols], int row, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  predictions(p, acc, col0, patch);
+  predictions(ahead, acc, patch);
   bool const in = row < p.M;
   float top = -INFINITY;
 #pragma unroll
@@ -282,7 +303,7 @@ __device__ __forceinline__ void finish_seen(Product const& p, float (&acc)[kCols
 #pragma unroll
   for (int i = 0; i < kCols; ++i) sum += __expf(acc[i] - base);
   if (in) e.parts[(long long)(col0 / kCols) * p.M + row] = make_float2(top, sum);
-  int const at = in ? min(max((int)__ldg(e.labels + row) - 1, 0), e.classes - 1) - e.firstClass - col0 : -1;
+  int const at = in ? min(max((int)ahead.label - 1, 0), e.classes - 1) - e.firstClass - col0 : -1;
   bool const here = at >= 0 && at < kCols && col0 + at < p.N;
   if (__any_sync(0xffffffffu, here)) {
     float z = 0.f;
@@ -309,12 +330,11 @@ __device__ __forceinline__ float lane_sums(float (&v)[32])
 }
 
 template <int kCols>
-__device__ __forceinline__ void finish_grad(Product const& p, float (&acc)[kCols], int row0, int row, int col0, float* patch)
+__device__ __forceinline__ void finish_grad(Product const& p, Ahead const& ahead, float (&acc)[kCols], int row0, int row, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  predictions(p, acc, col0, patch);
-  bool const in = row < p.M;
-  float const l = in ? __ldg(e.labels + row) : 0.f, lse = in ? __ldg(e.lse + row) : 0.f;
+  predictions(ahead, acc, patch);
+  float const l = ahead.label, lse = ahead.lse;               // (rows behind the last: label 0)
   bool const real = l > 0.f && l <= (float)e.classes;
   if (l > (float)e.classes && e.status) atomicExch(e.status, kStatusBadLabel);
   int const at = min(max((int)l - 1, 0), e.classes - 1) - e.firstClass - col0;
@@ -335,20 +355,17 @@ __device__ __forceinline__ void finish_grad(Product const& p, float (&acc)[kCols
       if (row0 < p.M && c < p.N) e.db[(long long)(row0 / 32) * e.to.ld + c] = s;
     }
   }
-  float const f = pow2(e.toExp);
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) acc[i] *= f;
 #pragma unroll
   for (int i = 0; i < kCols; i += 64)
-    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, min(32, p.M - row0), &acc[i], patch);
+    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, min(32, p.M - row0), &acc[i], pow2(e.toExp), patch);
 }
 
 template <int kCols>
-__device__ __forceinline__ void finish_poly(Product const& p, float (&acc)[kCols], int row0, int col0, float* patch)
+__device__ __forceinline__ void finish_poly(Product const& p, Ahead const& ahead, float (&acc)[kCols], int row0, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
   int const rows = min(32, p.M - row0);
-  float const f = e.alpha * pow2(-exp_of(e.ea)) * pow2(-exp_of(e.eb));
+  float const f = e.alpha * ahead.fa * ahead.fb;
 #pragma unroll
   for (int i = 0; i < kCols; ++i) acc[i] *= f;
   if (e.beta != 0.f) {
@@ -379,12 +396,9 @@ __device__ __forceinline__ void finish_poly(Product const& p, float (&acc)[kCols
     update_rows(e.out, e.ldc, p.M, p.N, true, acc, row0, col0, patch, [&](float old, float v) { return old - e.rate * v; });
     return;
   }
-  float const ft = pow2(e.toExp);
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) acc[i] *= ft;
 #pragma unroll
   for (int i = 0; i < kCols; i += 64)
-    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, rows, &acc[i], patch);
+    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, rows, &acc[i], pow2(e.toExp), patch);
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -434,6 +448,8 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
     for (int w = first; w < batch.work; w += stride) {
       Item const t = item_of(batch, w);
       Product const& p = batch.p[t.prod];
+      int const row0 = t.tm * kTileRows + (int)rank * 128 + quarter * 32, col0 = t.tn * kTileCols + half * kCols;
+      Ahead const ahead = fetch_ahead<kKind, kCols>(p, row0 + lane, col0, patch);
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
@@ -483,11 +499,10 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         }
         if (threadIdx.x == 0) batch.tickets[slot] = 0;
       }
-      int const row0 = t.tm * kTileRows + (int)rank * 128 + quarter * 32, col0 = t.tn * kTileCols + half * kCols;
-      if (kKind == kPairOut)  finish_out(p, acc, row0, col0, patch);
-      if (kKind == kPairSeen) finish_seen(p, acc, row0 + lane, col0, patch);
-      if (kKind == kPairGrad) finish_grad(p, acc, row0, row0 + lane, col0, patch);
-      if (kKind == kPairPoly) finish_poly(p, acc, row0, col0, patch);
+      if (kKind == kPairOut)  finish_out(p, ahead, acc, row0, col0, patch);
+      if (kKind == kPairSeen) finish_seen(p, ahead, acc, row0 + lane, col0, patch);
+      if (kKind == kPairGrad) finish_grad(p, ahead, acc, row0, row0 + lane, col0, patch);
+      if (kKind == kPairPoly) finish_poly(p, ahead, acc, row0, col0, patch);
     }
     if (dead && lane == 0) atomicCAS(batch.status, 0, 42);
   } else {
