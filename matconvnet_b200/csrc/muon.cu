@@ -1,8 +1,10 @@
 // The Muon solver (include/vlb.h has the formulas).
+#include "muon_small.cuh"
 #include "pairs.cuh"
 #include "products.cuh"
 #include <math.h>
 #include <algorithm>
+#include <vector>
 
 namespace {
 
@@ -163,7 +165,7 @@ step_many_kernel(const __grid_constant__ Jobs jobs, double epsilon)
   for (size_t i = (size_t)block * kThreads + threadIdx.x; i < j.n; i += (size_t)j.blocks * kThreads) j.w[i] -= j.rate * (j.u[i] * f);
 }
 
-// The largest magnitude of t + b t' + c t'' over [0, s]: of a*t + b*t^3 + c*t^5 or of b*t + c*t^2, with 2% for what lies between the samples.
+// The largest magnitude of a polynomial over [0, s], with 2% for what lies between the samples.
 template <class F>
 double most(F f, double s)
 {
@@ -179,23 +181,41 @@ int exp_below_half(double m)
   return m < 1e-25 ? 97 : 14 - (int)ceil(log2(m));
 }
 
+// The exponents of the halves through the steps: every element of a matrix is at most its largest singular value, which the polynomials bound.
+struct Exponents {
+  std::vector<int> x, gram, poly;
+  explicit Exponents(vlb_muon_opts const& o)
+  {
+    double s = 1;
+    x.push_back(exp_below_half(s));
+    for (int k = 0; k < o.steps; ++k) {
+      double const s2 = s * s;
+      gram.push_back(exp_below_half(s2));
+      poly.push_back(exp_below_half(most([&](double t) { return t * (o.b + t * o.c); }, s2)));
+      s = most([&](double t) { return t * (o.a + t * t * (o.b + t * t * o.c)); }, s);
+      x.push_back(exp_below_half(s));
+    }
+  }
+};
+
 int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* o)
 {
+  // all small: all steps in one launch.  (Beside larger ones they cost next to nothing in the launches that those need.)
+  bool small = true;
+  for (int i = 0; i < count; ++i) small = small && vlb::small_fits(u[i].rows, u[i].cols, o->steps);
   Jobs jobs = {};
-  vlb::PairProduct step[3 * kMost] = {};
-  vlb::PairProduct *const gram = step, *const poly = step + count, *const next = step + 2 * count;
   vlb::Pair x[2][kMost], a[kMost], q[kMost];
   size_t bytes = 0;
-  char* at = nullptr;
+  char *at = nullptr, *split = nullptr;
   auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
-  char* split = nullptr;
   for (int pass = 0; pass < 2; ++pass) {
     bytes = 0;
-    split = take(vlb::kPairSplitBytes);
+    split = take(small ? vlb::small_scratch(count) : vlb::kPairSplitBytes);
     for (int i = 0; i < count; ++i) {
       int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
       jobs.j[i].u = (float*)take(sizeof(float) * (size_t)rows * cols);
       jobs.j[i].parts = (double*)take(sizeof(double) * kMaxParts);
+      if (small) continue;
       x[0][i] = vlb::pair_at(take(vlb::pair_bytes(rows, cols)), rows, cols);
       x[1][i] = vlb::pair_at(take(vlb::pair_bytes(rows, cols)), rows, cols);
       a[i] = vlb::pair_at(take(vlb::pair_bytes(m, m)), m, m);
@@ -215,7 +235,6 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
     j.block0 = blocks;
     j.blocks = j.partCount = (int)vlb::grid_for((j.n + 3) / 4, kThreads, kMaxParts);
     blocks += j.blocks;
-    j.x = x[0][i];
   }
   vlb::launch(ctx->stream, momentum_many_kernel, (unsigned)blocks, kThreads, 0, jobs, (float)gradMult, (float)o->momentum, o->nesterov);
   VLB_LAUNCHED(ctx, 1);
@@ -224,11 +243,20 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
     VLB_LAUNCHED(ctx, 1);
     return VLB_Success;
   }
-  double s = 1;                                        // no singular value is larger
-  int ex = exp_below_half(s);
+  Exponents const e(*o);
+  if (small) {
+    vlb::SmallMatrix m[kMost];
+    vlb::SmallSteps steps = {};
+    steps.count = o->steps; steps.epsilon = o->epsilon;
+    steps.a = (float)o->a; steps.b = (float)o->b; steps.c = (float)o->c;
+    std::copy(e.x.begin(), e.x.end(), steps.x); std::copy(e.gram.begin(), e.gram.end(), steps.gram); std::copy(e.poly.begin(), e.poly.end(), steps.poly);
+    for (int i = 0; i < count; ++i) m[i] = {u[i].W, jobs.j[i].u, jobs.j[i].parts, jobs.j[i].partCount, u[i].rows, u[i].cols, jobs.j[i].rate};
+    return vlb::small_matrices(ctx, m, count, steps, split);
+  }
   blocks = 0;
   for (int i = 0; i < count; ++i) {
     Job& j = jobs.j[i];
+    j.x = x[0][i];
     int const groups = (int)(j.x.ld / 16);
     j.rowsPer = std::max(1, 512 / groups);
     j.perRow = vlb::FastDiv(groups);
@@ -236,18 +264,17 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
     j.blocks = vlb::ceil_div(j.x.rows, j.rowsPer);
     blocks += j.blocks;
   }
-  vlb::launch(ctx->stream, make_x_kernel, (unsigned)blocks, kThreads, 0, jobs, o->epsilon, ex);
+  vlb::launch(ctx->stream, make_x_kernel, (unsigned)blocks, kThreads, 0, jobs, o->epsilon, e.x[0]);
   VLB_LAUNCHED(ctx, 1);
+  vlb::PairProduct step[3 * kMost];
+  vlb::PairProduct *const gram = step, *const poly = step + count, *const next = step + 2 * count;
   for (int k = 0; k < o->steps; ++k) {
-    // every element of a matrix is at most its largest singular value, which the polynomials bound
-    double const s2 = s * s;
-    s = most([&](double t) { return t * (o->a + t * t * (o->b + t * t * o->c)); }, s);
-    int const ea = exp_below_half(s2), eq = exp_below_half(most([&](double t) { return t * (o->b + t * o->c); }, s2)), en = exp_below_half(s);
+    int const ex = e.x[k], ea = e.gram[k], eq = e.poly[k];
     for (int i = 0; i < count; ++i) {
       int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
       bool const tall = rows > cols;
       vlb::Pair const& xi = x[k & 1][i];
-      vlb::PairProduct &g = gram[i], &p = poly[i], &n = next[i];
+      vlb::PairProduct &g = gram[i] = {}, &p = poly[i] = {}, &n = next[i] = {};
       g.a = g.b = {xi, tall, false};
       g.M = g.N = m; g.K = std::max(rows, cols);
       g.symmetric = true;
@@ -261,13 +288,12 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
       n.M = rows; n.N = cols; n.K = m;
       n.e.ea.value = tall ? ex : eq; n.e.eb.value = tall ? eq : ex;
       n.e.alpha = 1.f; n.e.beta = (float)o->a; n.e.add = xi; n.e.addExp = ex;
-      if (k + 1 < o->steps) { n.e.to = x[(k + 1) & 1][i]; n.e.toExp = en; }
+      if (k + 1 < o->steps) { n.e.to = x[(k + 1) & 1][i]; n.e.toExp = e.x[k + 1]; }
       else                  { n.e.out = u[i].W; n.e.ldc = cols; n.e.rate = jobs.j[i].rate; }
     }
     int const tile = vlb::pair_tile(ctx, step, 3 * count);          // (one for all: what one product leaves of a symmetric matrix the next one reads)
     for (int set = 0; set < 3; ++set)
       if (int const rc = vlb::products_of_pairs(ctx, vlb::kPairPoly, step + set * count, count, split, tile)) return rc;
-    ex = en;
   }
   return VLB_Success;
 }
