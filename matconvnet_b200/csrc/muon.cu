@@ -210,7 +210,7 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
   auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
   for (int pass = 0; pass < 2; ++pass) {
     bytes = 0;
-    split = take(small ? vlb::small_scratch(count) : vlb::kPairSplitBytes);
+    split = take(small ? 0 : vlb::kPairSplitBytes);
     for (int i = 0; i < count; ++i) {
       int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
       jobs.j[i].u = (float*)take(sizeof(float) * (size_t)rows * cols);
@@ -251,7 +251,7 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
     steps.a = (float)o->a; steps.b = (float)o->b; steps.c = (float)o->c;
     std::copy(e.x.begin(), e.x.end(), steps.x); std::copy(e.gram.begin(), e.gram.end(), steps.gram); std::copy(e.poly.begin(), e.poly.end(), steps.poly);
     for (int i = 0; i < count; ++i) m[i] = {u[i].W, jobs.j[i].u, jobs.j[i].parts, jobs.j[i].partCount, u[i].rows, u[i].cols, jobs.j[i].rate};
-    return vlb::small_matrices(ctx, m, count, steps, split);
+    return vlb::small_matrices(ctx, m, count, steps);
   }
   blocks = 0;
   for (int i = 0; i < count; ++i) {

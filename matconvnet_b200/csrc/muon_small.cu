@@ -4,12 +4,13 @@
 //
 // X, the matrix or its transpose, has m <= 128 rows; CTA r of the cluster has up to 256 of its columns, as pairs of halves (pairs.cuh) in the layout that the tensor
 // core reads both along the rows (A = X X': the columns are the reduction) and along the columns (Q X: the rows are).  A step:
-//   A = X X'        every CTA for its columns, in chains of 64; the CTAs' sums are added through scratch memory, each CTA adding a share of the rows for all
+//   A = X X'        every CTA for its columns, in chains of 64; each CTA then adds up a share of the elements over the cluster's shared memories and leaves the
+//                   totals in the same places of all of them
 //   Q = b A + c A A every CTA for itself
 //   X = a X + Q X   every CTA its columns, in place
 // The arithmetic is that of pairs.cu: three products of halves each, chains of 64 products, sums in single precision.
-// Warps 0-7 move data between registers and tensor memory, shared memory and scratch: warp w has TMEM lanes (rows) 32 (w % 4) ... and half w / 4 of the columns;
-// one thread of warp 8 issues the MMAs.
+// Warps 0-15 move data between registers, tensor memory and shared memory: warp w has TMEM lanes (rows) 32 (w % 4) ... and quarter w / 4 of the columns; one thread
+// of warp 16 issues the MMAs.
 #include "muon_small.cuh"
 #include "pairs.cuh"
 #include "tc_common.cuh"
@@ -19,13 +20,12 @@ namespace {
 using vlb::SmallMatrix; using vlb::SmallSteps; using vlb::pow2;
 using vlb::kSmallMost; using vlb::kSmallSide; using vlb::kSmallLong;
 
-constexpr int kMovers = 256, kThreads = 288;
+constexpr int kMovers = 512, kThreads = 544;
 constexpr int kPart = 128 * 128, kBlock = 2 * kPart;          // bytes of 128 rows x 64 halves, and of hi and lo of them
 constexpr int kMostBlocks = 4;                                // 64-column blocks of X in a CTA
 constexpr size_t kSmem = (size_t)(kMostBlocks + 2) * kBlock + 1024;
-constexpr int kGramFloats = 128 * 128;
 
-struct Matrices { SmallMatrix m[kSmallMost]; SmallSteps steps; float* scratch; int* status; int cluster; };
+struct Matrices { SmallMatrix m[kSmallMost]; SmallSteps steps; int* status; int cluster; };
 
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
@@ -58,6 +58,18 @@ __device__ __forceinline__ void all_threads() { asm volatile("bar.sync 1, %0;" :
 __device__ __forceinline__ void movers() { asm volatile("bar.sync 2, %0;" ::"n"(kMovers) : "memory"); }
 __device__ __forceinline__ void cluster_sync()
 { asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// the same shared-memory place in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank)
+{ uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank)); return r; }
+__device__ __forceinline__ float4 load_cluster(uint32_t addr)
+{
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, float4 v)
+{ asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory"); }
 
 // Eight neighbouring halves of a row of a block: place c of row r lies at c ^ (r % 8), the 128-byte swizzle.
 __device__ __forceinline__ uint4& place(char* block, int row, int c) { return *(uint4*)(block + row * 128 + ((c ^ (row & 7)) << 4)); }
@@ -98,7 +110,7 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
   char* const gramAt = base + kMostBlocks * kBlock;           // A, then Q: two blocks
   int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = all.cluster, rank = (int)blockIdx.x % G, which = (int)blockIdx.x / G;
   if (threadIdx.x == 0) { mbar_init(smem_u32(&through), 1); asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
-  if (warp == 8) tmem_alloc(smem_u32(&tmemAt), 512);
+  if (warp == 16) tmem_alloc(smem_u32(&tmemAt), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -113,7 +125,7 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
   int const rowBlocks = m > 64 ? 2 : 1;
   uint32_t phase = 0;
   bool dead = false;
-  if (warp == 8) {
+  if (warp == 16) {
     uint32_t const xAt = smem_u32(base), gAt = smem_u32(gramAt);
     uint64_t const rowStep = 32 >> 4, colStep = 2048 >> 4;
     uint32_t const square = (1u << 4) | (128u >> 3 << 17) | (128u >> 4 << 24), next = (1u << 4) | (1u << 16) | ((uint32_t)(per >> 3) << 17) | (128u >> 4 << 24);
@@ -128,7 +140,7 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
         umma_commit(smem_u32(&through));
       }
       __syncwarp();
-      cluster_sync();                                         // the CTAs' sums are in scratch
+      cluster_sync();                                         // the CTAs' sums are there
       cluster_sync();                                         // their totals are
       all_threads();                                          // A is there
       tc_fence_after();
@@ -153,7 +165,8 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
       __syncwarp();
     }
   } else {
-    int const quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    int const quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
+    bool const rowsIn = quarter * 32 < m, in = rowsIn && part * 32 < m;            // whether the warp has rows of X, and elements of A
     uint32_t const lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     // the factor that normalises
     double sum = 0;
@@ -166,6 +179,7 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
     float const norm = (float)(1. / (sqrt(sum) + st.epsilon));
     // X: a thread takes eight neighbouring columns of a row; neighbouring threads what is neighbouring in memory
     float const f0 = pow2(st.x[0]);
+#pragma unroll 4
     for (int t = threadIdx.x; t < 128 * per / 8; t += kMovers) {
       int const r = tall ? t % 128 : t / (per / 8), c = tall ? t / 128 : t % (per / 8);
       float v[8];
@@ -184,120 +198,129 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
       tc_fence_after();
     };
     auto handed = [&] { fence_async_smem(); tc_fence_before(); all_threads(); };
-    float* const sumsAt = all.scratch + (size_t)which * (G + 1) * kGramFloats;                 // of each CTA, then the totals
+    float4* const gramSums = (float4*)gramAt;                 // [column / 4][row]: side by side for a warp
+    uint32_t const gramAddr = smem_u32(gramAt);
     for (int k = 0; k < st.count; ++k) {
+      float const unX = pow2(-st.x[k]), toA = pow2(st.gram[k]), unA = pow2(-st.gram[k]), toQ = pow2(st.poly[k]), unQ = pow2(-st.poly[k]), toX = pow2(st.x[k + 1]);
       handed();
       done();
-      // A: 64 columns of a row, the columns of half `half`
-      float g[64];
+      // A: 32 columns of a row
+      float g[32];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) g[i] = 0.f;
-      for (int b = 0; b < blocks; ++b) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r[16];
-          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 64 * half + 16 * q), r);
+      for (int i = 0; i < 32; ++i) g[i] = 0.f;
+      if (in)
+        for (int b = 0; b < blocks; ++b) {
+          uint32_t r[32];
+          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part), r);
+          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part + 16), r + 16);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) g[16 * q + i] += __uint_as_float(r[i]);
+          for (int i = 0; i < 32; ++i) g[i] += __uint_as_float(r[i]);
+        }
+      if (G > 1 && in) {
+        // (nothing reads Q any more)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gramSums[(8 * part + i) * 128 + row] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
+      }
+      __syncwarp();
+      cluster_sync();
+      if (G > 1) {
+        // a place is read and written by one thread of the cluster alone
+        int const rows = (m + 31) / 32 * 32, places = (m + 3) / 4 * rows, share = (places + G - 1) / G, end = min((rank + 1) * share, places);
+        for (int i = rank * share + (int)threadIdx.x; i < end; i += kMovers) {
+          uint32_t const at = gramAddr + 16u * (uint32_t)(i / rows * 128 + i % rows);
+          float4 v[8], t = make_float4(0, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) if (c < G) v[c] = load_cluster(in_cta(at, c));
+#pragma unroll
+          for (int c = 0; c < 8; ++c) if (c < G) { t.x += v[c].x; t.y += v[c].y; t.z += v[c].z; t.w += v[c].w; }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) if (c < G) store_cluster(in_cta(at, c), t);
         }
       }
-      if (G > 1) {
-        // [column / 4][row]: side by side for a warp
-        float4* const own = (float4*)(sumsAt + (size_t)rank * kGramFloats) + (16 * half) * 128 + row;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) __stcg(own + i * 128, make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]));
-        __threadfence();
-      }
+      __syncwarp();
       cluster_sync();
-      float4* const totals = (float4*)(sumsAt + (size_t)G * kGramFloats);
       if (G > 1) {
-        int const share = kGramFloats / 4 / G;
-        for (int i = rank * share + (int)threadIdx.x; i < (rank + 1) * share; i += kMovers) {
-          float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-          for (int c = 0; c < G; ++c) {
-            float4 const v = __ldcg((float4 const*)(sumsAt + (size_t)c * kGramFloats) + i);
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        if (in) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float4 const v = 8 * part + i < (m + 3) / 4 ? gramSums[(8 * part + i) * 128 + row] : make_float4(0, 0, 0, 0);
+            g[4 * i] = v.x; g[4 * i + 1] = v.y; g[4 * i + 2] = v.z; g[4 * i + 3] = v.w;
           }
-          __stcg(totals + i, s);
         }
-        __threadfence();
+        movers();                                             // before A takes the places of the totals
       }
-      cluster_sync();
-      if (G > 1) {
-        float4 const* const from = totals + (16 * half) * 128 + row;
+      char* const gramBlock = gramAt + part / 2 * kBlock;
+      int const gramPlace = part % 2 * 4;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float4 const v = __ldcg(from + i * 128);
-          g[4 * i] = v.x; g[4 * i + 1] = v.y; g[4 * i + 2] = v.z; g[4 * i + 3] = v.w;
-        }
-      }
-      float const unX = pow2(-st.x[k]), toA = pow2(st.gram[k]), unA = pow2(-st.gram[k]), toQ = pow2(st.poly[k]), unQ = pow2(-st.poly[k]), toX = pow2(st.x[k + 1]);
+      for (int i = 0; i < 32; ++i) g[i] = g[i] * unX * unX;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) g[i] = g[i] * unX * unX;
-      char* const gramBlock = gramAt + half * kBlock;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
+      for (int c = 0; c < 4; ++c) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toA;
-        put8(gramBlock, row, c, v);
+        put8(gramBlock, row, gramPlace + c, v);               // (zeros behind the last row and column)
       }
       handed();
       done();
       // Q = b A + c A A
-      float const fa = st.c * unA * unA;
+      if (in) {
+        float const fa = st.c * unA * unA;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) g[i] *= st.b;
-      for (int b = 0; b < rowBlocks; ++b) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r[16];
-          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 64 * half + 16 * q), r);
+        for (int i = 0; i < 32; ++i) g[i] *= st.b;
+        for (int b = 0; b < rowBlocks; ++b) {
+          uint32_t r[32];
+          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part), r);
+          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part + 16), r + 16);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) g[16 * q + i] = fmaf(fa, __uint_as_float(r[i]), g[16 * q + i]);
+          for (int i = 0; i < 32; ++i) g[i] = fmaf(fa, __uint_as_float(r[i]), g[i]);
         }
-      }
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float v[8];
+        for (int c = 0; c < 4; ++c) {
+          float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toQ;
-        put8(gramBlock, row, c, v);
+          for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toQ;
+          put8(gramBlock, row, gramPlace + c, v);
+        }
       }
       handed();
       done();
-      // X = a X + Q X, the warp's half of the columns, eight at a time
+      // X = a X + Q X, the warp's quarter of the columns, sixteen at a time
       bool const last = k + 1 == st.count;
-      for (int c8 = half * (per / 16); c8 < (half + 1) * (per / 16); ++c8) {
-        uint32_t r[2][8];
-        tmem_ld8_issue(lanes + (uint32_t)(8 * c8), r[0]);
-        if (rowBlocks > 1) tmem_ld8_issue(lanes + (uint32_t)(256 + 8 * c8), r[1]);
-        float v[8];
-        char* const block = base + c8 / 8 * kBlock;
-        get8(block, row, c8 % 8, v);
-        tmem_ld_wait();
+      if (rowsIn)
+        for (int c16 = part * (per / 64); c16 < (part + 1) * (per / 64); ++c16) {
+          uint32_t r[2][16];
+          tmem_ld16_issue(lanes + (uint32_t)(16 * c16), r[0]);
+          if (rowBlocks > 1) tmem_ld16_issue(lanes + (uint32_t)(256 + 16 * c16), r[1]);
+          char* const block = base + c16 / 4 * kBlock;
+          float v[2][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float const q = __uint_as_float(r[0][i]) + (rowBlocks > 1 ? __uint_as_float(r[1][i]) : 0.f);
-          v[i] = st.a * (v[i] * unX) + q * unQ * unX;
-        }
-        if (!last) {
+          for (int q = 0; q < 2; ++q) get8(block, row, c16 % 4 * 2 + q, v[q]);
+          tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= toX;
-          put8(block, row, c8 % 8, v);
-        } else if (row < m) {
+          for (int q = 0; q < 2; ++q) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            int const j = c8 * 8 + i;
-            if (j >= mine) break;
-            float* const w = mat.w + (tall ? (size_t)(j0 + j) * mat.cols + row : (size_t)row * mat.cols + j0 + j);
-            *w -= mat.rate * v[i];
+            for (int i = 0; i < 8; ++i) {
+              float const t = __uint_as_float(r[0][8 * q + i]) + (rowBlocks > 1 ? __uint_as_float(r[1][8 * q + i]) : 0.f);
+              v[q][i] = st.a * (v[q][i] * unX) + t * unQ * unX;
+            }
+            if (!last) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[q][i] *= toX;
+              put8(block, row, c16 % 4 * 2 + q, v[q]);
+            } else {
+              int const j = 16 * c16 + 8 * q;
+              float* const w = mat.w + (tall ? (size_t)(j0 + j) * mat.cols + row : (size_t)row * mat.cols + j0 + j);
+              size_t const step = tall ? mat.cols : 1;
+              float old[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) old[i] = row < m && j + i < mine ? w[i * step] : 0.f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) if (row < m && j + i < mine) w[i * step] = old[i] - mat.rate * v[q][i];
+            }
           }
         }
-      }
     }
     if (dead && lane == 0) atomicCAS(all.status, 0, 44);
   }
@@ -305,7 +328,7 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
   __syncthreads();
   cluster_sync();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace
@@ -317,15 +340,12 @@ bool small_fits(int rows, int cols, int steps)
   return std::min(rows, cols) <= kSmallSide && std::max(rows, cols) <= kSmallLong && steps > 0 && steps <= kSmallSteps;
 }
 
-size_t small_scratch(int count) { return sizeof(float) * kGramFloats * 9 * (size_t)count; }
-
-int small_matrices(vlb_ctx* ctx, SmallMatrix const* m, int count, SmallSteps const& steps, void* scratch)
+int small_matrices(vlb_ctx* ctx, SmallMatrix const* m, int count, SmallSteps const& steps)
 {
   Matrices all;
   int longest = 0;
   for (int i = 0; i < count; ++i) { all.m[i] = m[i]; longest = std::max(longest, std::max(m[i].rows, m[i].cols)); }
   all.steps = steps;
-  all.scratch = (float*)scratch;
   all.status = ctx->deviceStatus;
   // as many CTAs to a matrix as its longer side has 128 columns for, at most eight (with 256 each 64 x 576 CLUSTERFIG)
   all.cluster = 1;

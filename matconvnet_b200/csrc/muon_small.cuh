@@ -20,8 +20,7 @@ struct SmallSteps {
 
 // Fits: at most kSmallSide rows or columns, at most kSmallLong of the other, at most kSmallSteps steps.
 bool small_fits(int rows, int cols, int steps);
-size_t small_scratch(int count);
 
-int small_matrices(vlb_ctx* ctx, SmallMatrix const* m, int count, SmallSteps const& steps, void* scratch);
+int small_matrices(vlb_ctx* ctx, SmallMatrix const* m, int count, SmallSteps const& steps);
 
 }  // namespace vlb
