@@ -9,8 +9,8 @@
 //   Q = b A + c A A every CTA for itself
 //   X = a X + Q X   every CTA its columns, in place
 // The arithmetic is that of pairs.cu: three products of halves each, chains of 64 products, sums in single precision.
-// Warps 0-15 move data between registers, tensor memory and shared memory: warp w has TMEM lanes (rows) 32 (w % 4) ... and quarter w / 4 of the columns; one thread
-// of warp 16 issues the MMAs.
+// Sixteen warps move data between registers, tensor memory and shared memory: warp w has TMEM lanes (rows) 32 (w % 4) ... and quarter w / 4 of the columns.  One of
+// their threads issues the MMAs: nothing else could be done meanwhile, and without a warp for it a thread has 128 registers.
 #include "muon_small.cuh"
 #include "pairs.cuh"
 #include "tc_common.cuh"
@@ -20,7 +20,7 @@ namespace {
 using vlb::SmallMatrix; using vlb::SmallSteps; using vlb::pow2;
 using vlb::kSmallMost; using vlb::kSmallSide; using vlb::kSmallLong;
 
-constexpr int kMovers = 512, kThreads = 544;
+constexpr int kThreads = 512;
 constexpr int kPart = 128 * 128, kBlock = 2 * kPart;          // bytes of 128 rows x 64 halves, and of hi and lo of them
 constexpr int kMostBlocks = 4;                                // 64-column blocks of X in a CTA
 constexpr size_t kSmem = (size_t)(kMostBlocks + 2) * kBlock + 1024;
@@ -54,8 +54,6 @@ __device__ __forceinline__ void chain(uint32_t d, uint64_t aH, uint64_t aL, uint
   }
 }
 
-__device__ __forceinline__ void all_threads() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-__device__ __forceinline__ void movers() { asm volatile("bar.sync 2, %0;" ::"n"(kMovers) : "memory"); }
 __device__ __forceinline__ void cluster_sync()
 { asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
@@ -105,12 +103,12 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
   extern __shared__ char raw[];
   __shared__ __align__(8) uint64_t through;
   __shared__ uint32_t tmemAt;
-  __shared__ double sums[kMovers / 32];
+  __shared__ double sums[kThreads / 32];
   char* const base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   char* const gramAt = base + kMostBlocks * kBlock;           // A, then Q: two blocks
   int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = all.cluster, rank = (int)blockIdx.x % G, which = (int)blockIdx.x / G;
   if (threadIdx.x == 0) { mbar_init(smem_u32(&through), 1); asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
-  if (warp == 16) tmem_alloc(smem_u32(&tmemAt), 512);
+  if (warp == 0) tmem_alloc(smem_u32(&tmemAt), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -125,210 +123,194 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
   int const rowBlocks = m > 64 ? 2 : 1;
   uint32_t phase = 0;
   bool dead = false;
-  if (warp == 16) {
-    uint32_t const xAt = smem_u32(base), gAt = smem_u32(gramAt);
-    uint64_t const rowStep = 32 >> 4, colStep = 2048 >> 4;
-    uint32_t const square = (1u << 4) | (128u >> 3 << 17) | (128u >> 4 << 24), next = (1u << 4) | (1u << 16) | ((uint32_t)(per >> 3) << 17) | (128u >> 4 << 24);
-    for (int k = 0; k < st.count; ++k) {
-      all_threads();                                          // X is there
-      tc_fence_after();
-      if (lane == 0) {
-        for (int b = 0; b < blocks; ++b) {
-          uint64_t const h = make_desc(xAt + b * kBlock, 16, 1024), l = make_desc(xAt + b * kBlock + kPart, 16, 1024);
-          chain(tmem + 128 * b, h, l, rowStep, h, l, rowStep, square, three);
-        }
-        umma_commit(smem_u32(&through));
-      }
-      __syncwarp();
-      cluster_sync();                                         // the CTAs' sums are there
-      cluster_sync();                                         // their totals are
-      all_threads();                                          // A is there
-      tc_fence_after();
-      if (lane == 0) {
-        for (int b = 0; b < rowBlocks; ++b) {
-          uint64_t const h = make_desc(gAt + b * kBlock, 16, 1024), l = make_desc(gAt + b * kBlock + kPart, 16, 1024);
-          chain(tmem + 128 * b, h, l, rowStep, h, l, rowStep, square, three);
-        }
-        umma_commit(smem_u32(&through));
-      }
-      __syncwarp();
-      all_threads();                                          // Q is there
-      tc_fence_after();
-      if (lane == 0) {
-        for (int b = 0; b < rowBlocks; ++b) {                 // rows 64 b ... of X are the reduction
-          uint64_t const h = make_desc(gAt + b * kBlock, 16, 1024), l = make_desc(gAt + b * kBlock + kPart, 16, 1024);
-          uint64_t const xh = make_desc(xAt + b * 64 * 128, kBlock, 1024), xl = make_desc(xAt + kPart + b * 64 * 128, kBlock, 1024);
-          chain(tmem + 256 * b, h, l, rowStep, xh, xl, colStep, next, three);
-        }
-        umma_commit(smem_u32(&through));
-      }
-      __syncwarp();
-    }
-  } else {
-    int const quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
-    bool const rowsIn = quarter * 32 < m, in = rowsIn && part * 32 < m;            // whether the warp has rows of X, and elements of A
-    uint32_t const lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    // the factor that normalises
-    double sum = 0;
-    for (int i = threadIdx.x; i < mat.partCount; i += kMovers) sum += mat.parts[i];
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sums[warp] = sum;
-    movers();
-    sum = 0;
-    for (int i = 0; i < kMovers / 32; ++i) sum += sums[i];
-    float const norm = (float)(1. / (sqrt(sum) + st.epsilon));
-    // X: a thread takes eight neighbouring columns of a row; neighbouring threads what is neighbouring in memory
-    float const f0 = pow2(st.x[0]);
+  int const quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
+  bool const rowsIn = quarter * 32 < m, in = rowsIn && part * 32 < m;            // whether the warp has rows of X, and elements of A
+  uint32_t const lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+  // the factor that normalises
+  double sum = 0;
+  for (int i = threadIdx.x; i < mat.partCount; i += kThreads) sum += mat.parts[i];
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int i = 0; i < kThreads / 32; ++i) sum += sums[i];
+  float const norm = (float)(1. / (sqrt(sum) + st.epsilon));
+  // X: a thread takes eight neighbouring columns of a row; neighbouring threads what is neighbouring in memory
+  float const f0 = pow2(st.x[0]);
 #pragma unroll 4
-    for (int t = threadIdx.x; t < 128 * per / 8; t += kMovers) {
-      int const r = tall ? t % 128 : t / (per / 8), c = tall ? t / 128 : t % (per / 8);
+  for (int t = threadIdx.x; t < 128 * per / 8; t += kThreads) {
+    int const r = tall ? t % 128 : t / (per / 8), c = tall ? t / 128 : t % (per / 8);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      int const j = c * 8 + i;
+      bool const in = r < m && j < mine;
+      size_t const at = tall ? (size_t)(j0 + j) * mat.cols + r : (size_t)r * mat.cols + j0 + j;
+      v[i] = in ? __ldg(mat.u + at) * norm * f0 : 0.f;
+    }
+    put8(base + c / 8 * kBlock, r, c % 8, v);
+  }
+  uint32_t const xAt = smem_u32(base), gramAddr = smem_u32(gramAt);
+  uint64_t const rowStep = 32 >> 4, colStep = 2048 >> 4;
+  uint32_t const square = (1u << 4) | (128u >> 3 << 17) | (128u >> 4 << 24), next = (1u << 4) | (1u << 16) | ((uint32_t)(per >> 3) << 17) | (128u >> 4 << 24);
+  // What the threads wrote is handed to the tensor core, `issue` starts its work, and all wait for the end of it.
+  auto multiply = [&](auto issue) {
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      issue();
+      umma_commit(smem_u32(&through));
+    }
+    __syncwarp();
+    if (!dead && !mbar_wait(smem_u32(&through), phase)) dead = true;
+    phase ^= 1u;
+    __syncwarp();
+    tc_fence_after();
+  };
+  float4* const gramSums = (float4*)gramAt;                 // [column / 4][row]: side by side for a warp
+  for (int k = 0; k < st.count; ++k) {
+    float const unX = pow2(-st.x[k]), toA = pow2(st.gram[k]), unA = pow2(-st.gram[k]), toQ = pow2(st.poly[k]), unQ = pow2(-st.poly[k]), toX = pow2(st.x[k + 1]);
+    multiply([&] {
+      for (int b = 0; b < blocks; ++b) {
+        uint64_t const h = make_desc(xAt + b * kBlock, 16, 1024), l = make_desc(xAt + b * kBlock + kPart, 16, 1024);
+        chain(tmem + 128 * b, h, l, rowStep, h, l, rowStep, square, three);
+      }
+    });
+    // A: 32 columns of a row
+    float g[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) g[i] = 0.f;
+    if (in)
+      for (int b = 0; b < blocks; ++b) {
+        uint32_t r[32];
+        tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part), r);
+        tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part + 16), r + 16);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) g[i] += __uint_as_float(r[i]);
+      }
+    if (G > 1 && in) {
+      // (nothing reads Q any more)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gramSums[(8 * part + i) * 128 + row] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
+    }
+    __syncwarp();
+    cluster_sync();
+    if (G > 1) {
+      // a place is read and written by one thread of the cluster alone
+      int const rows = (m + 31) / 32 * 32, places = (m + 3) / 4 * rows, share = (places + G - 1) / G, end = min((rank + 1) * share, places);
+      for (int i = rank * share + (int)threadIdx.x; i < end; i += kThreads) {
+        uint32_t const at = gramAddr + 16u * (uint32_t)(i / rows * 128 + i % rows);
+        float4 v[8], t = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) if (c < G) v[c] = load_cluster(in_cta(at, c));
+#pragma unroll
+        for (int c = 0; c < 8; ++c) if (c < G) { t.x += v[c].x; t.y += v[c].y; t.z += v[c].z; t.w += v[c].w; }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) if (c < G) store_cluster(in_cta(at, c), t);
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (G > 1) {
+      if (in) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float4 const v = 8 * part + i < (m + 3) / 4 ? gramSums[(8 * part + i) * 128 + row] : make_float4(0, 0, 0, 0);
+          g[4 * i] = v.x; g[4 * i + 1] = v.y; g[4 * i + 2] = v.z; g[4 * i + 3] = v.w;
+        }
+      }
+      __syncthreads();                                             // before A takes the places of the totals
+    }
+    char* const gramBlock = gramAt + part / 2 * kBlock;
+    int const gramPlace = part % 2 * 4;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) g[i] = g[i] * unX * unX;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
       float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int const j = c * 8 + i;
-        bool const in = r < m && j < mine;
-        size_t const at = tall ? (size_t)(j0 + j) * mat.cols + r : (size_t)r * mat.cols + j0 + j;
-        v[i] = in ? __ldg(mat.u + at) * norm * f0 : 0.f;
-      }
-      put8(base + c / 8 * kBlock, r, c % 8, v);
+      for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toA;
+      put8(gramBlock, row, gramPlace + c, v);               // (zeros behind the last row and column)
     }
-    auto done = [&] {
-      if (!dead && !mbar_wait(smem_u32(&through), phase)) dead = true;
-      phase ^= 1u;
-      tc_fence_after();
-    };
-    auto handed = [&] { fence_async_smem(); tc_fence_before(); all_threads(); };
-    float4* const gramSums = (float4*)gramAt;                 // [column / 4][row]: side by side for a warp
-    uint32_t const gramAddr = smem_u32(gramAt);
-    for (int k = 0; k < st.count; ++k) {
-      float const unX = pow2(-st.x[k]), toA = pow2(st.gram[k]), unA = pow2(-st.gram[k]), toQ = pow2(st.poly[k]), unQ = pow2(-st.poly[k]), toX = pow2(st.x[k + 1]);
-      handed();
-      done();
-      // A: 32 columns of a row
-      float g[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) g[i] = 0.f;
-      if (in)
-        for (int b = 0; b < blocks; ++b) {
-          uint32_t r[32];
-          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part), r);
-          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part + 16), r + 16);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) g[i] += __uint_as_float(r[i]);
-        }
-      if (G > 1 && in) {
-        // (nothing reads Q any more)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) gramSums[(8 * part + i) * 128 + row] = make_float4(g[4 * i], g[4 * i + 1], g[4 * i + 2], g[4 * i + 3]);
+    multiply([&] {
+      for (int b = 0; b < rowBlocks; ++b) {
+        uint64_t const h = make_desc(gramAddr + b * kBlock, 16, 1024), l = make_desc(gramAddr + b * kBlock + kPart, 16, 1024);
+        chain(tmem + 128 * b, h, l, rowStep, h, l, rowStep, square, three);
       }
-      __syncwarp();
-      cluster_sync();
-      if (G > 1) {
-        // a place is read and written by one thread of the cluster alone
-        int const rows = (m + 31) / 32 * 32, places = (m + 3) / 4 * rows, share = (places + G - 1) / G, end = min((rank + 1) * share, places);
-        for (int i = rank * share + (int)threadIdx.x; i < end; i += kMovers) {
-          uint32_t const at = gramAddr + 16u * (uint32_t)(i / rows * 128 + i % rows);
-          float4 v[8], t = make_float4(0, 0, 0, 0);
+    });
+    // Q = b A + c A A
+    if (in) {
+      float const fa = st.c * unA * unA;
 #pragma unroll
-          for (int c = 0; c < 8; ++c) if (c < G) v[c] = load_cluster(in_cta(at, c));
+      for (int i = 0; i < 32; ++i) g[i] *= st.b;
+      for (int b = 0; b < rowBlocks; ++b) {
+        uint32_t r[32];
+        tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part), r);
+        tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part + 16), r + 16);
+        tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 8; ++c) if (c < G) { t.x += v[c].x; t.y += v[c].y; t.z += v[c].z; t.w += v[c].w; }
-#pragma unroll
-          for (int c = 0; c < 8; ++c) if (c < G) store_cluster(in_cta(at, c), t);
-        }
+        for (int i = 0; i < 32; ++i) g[i] = fmaf(fa, __uint_as_float(r[i]), g[i]);
       }
-      __syncwarp();
-      cluster_sync();
-      if (G > 1) {
-        if (in) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float4 const v = 8 * part + i < (m + 3) / 4 ? gramSums[(8 * part + i) * 128 + row] : make_float4(0, 0, 0, 0);
-            g[4 * i] = v.x; g[4 * i + 1] = v.y; g[4 * i + 2] = v.z; g[4 * i + 3] = v.w;
-          }
-        }
-        movers();                                             // before A takes the places of the totals
-      }
-      char* const gramBlock = gramAt + part / 2 * kBlock;
-      int const gramPlace = part % 2 * 4;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) g[i] = g[i] * unX * unX;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toA;
-        put8(gramBlock, row, gramPlace + c, v);               // (zeros behind the last row and column)
+        for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toQ;
+        put8(gramBlock, row, gramPlace + c, v);
       }
-      handed();
-      done();
-      // Q = b A + c A A
-      if (in) {
-        float const fa = st.c * unA * unA;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] *= st.b;
-        for (int b = 0; b < rowBlocks; ++b) {
-          uint32_t r[32];
-          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part), r);
-          tmem_ld16_issue(lanes + (uint32_t)(128 * b + 32 * part + 16), r + 16);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) g[i] = fmaf(fa, __uint_as_float(r[i]), g[i]);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = g[8 * c + i] * toQ;
-          put8(gramBlock, row, gramPlace + c, v);
-        }
+    }
+    multiply([&] {
+      for (int b = 0; b < rowBlocks; ++b) {                     // rows 64 b ... of X are the reduction
+        uint64_t const h = make_desc(gramAddr + b * kBlock, 16, 1024), l = make_desc(gramAddr + b * kBlock + kPart, 16, 1024);
+        uint64_t const xh = make_desc(xAt + b * 64 * 128, kBlock, 1024), xl = make_desc(xAt + kPart + b * 64 * 128, kBlock, 1024);
+        chain(tmem + 256 * b, h, l, rowStep, xh, xl, colStep, next, three);
       }
-      handed();
-      done();
-      // X = a X + Q X, the warp's quarter of the columns, sixteen at a time
-      bool const last = k + 1 == st.count;
-      if (rowsIn)
-        for (int c16 = part * (per / 64); c16 < (part + 1) * (per / 64); ++c16) {
-          uint32_t r[2][16];
-          tmem_ld16_issue(lanes + (uint32_t)(16 * c16), r[0]);
-          if (rowBlocks > 1) tmem_ld16_issue(lanes + (uint32_t)(256 + 16 * c16), r[1]);
-          char* const block = base + c16 / 4 * kBlock;
-          float v[2][8];
+    });
+    // X = a X + Q X, the warp's quarter of the columns, sixteen at a time
+    bool const last = k + 1 == st.count;
+    if (rowsIn)
+      for (int c16 = part * (per / 64); c16 < (part + 1) * (per / 64); ++c16) {
+        uint32_t r[2][16];
+        tmem_ld16_issue(lanes + (uint32_t)(16 * c16), r[0]);
+        if (rowBlocks > 1) tmem_ld16_issue(lanes + (uint32_t)(256 + 16 * c16), r[1]);
+        char* const block = base + c16 / 4 * kBlock;
+        float v[2][8];
 #pragma unroll
-          for (int q = 0; q < 2; ++q) get8(block, row, c16 % 4 * 2 + q, v[q]);
-          tmem_ld_wait();
+        for (int q = 0; q < 2; ++q) get8(block, row, c16 % 4 * 2 + q, v[q]);
+        tmem_ld_wait();
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < 2; ++q) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float const t = __uint_as_float(r[0][8 * q + i]) + (rowBlocks > 1 ? __uint_as_float(r[1][8 * q + i]) : 0.f);
-              v[q][i] = st.a * (v[q][i] * unX) + t * unQ * unX;
-            }
-            if (!last) {
+          for (int i = 0; i < 8; ++i) {
+            float const t = __uint_as_float(r[0][8 * q + i]) + (rowBlocks > 1 ? __uint_as_float(r[1][8 * q + i]) : 0.f);
+            v[q][i] = st.a * (v[q][i] * unX) + t * unQ * unX;
+          }
+          if (!last) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[q][i] *= toX;
-              put8(block, row, c16 % 4 * 2 + q, v[q]);
-            } else {
-              int const j = 16 * c16 + 8 * q;
-              float* const w = mat.w + (tall ? (size_t)(j0 + j) * mat.cols + row : (size_t)row * mat.cols + j0 + j);
-              size_t const step = tall ? mat.cols : 1;
-              float old[8];
+            for (int i = 0; i < 8; ++i) v[q][i] *= toX;
+            put8(block, row, c16 % 4 * 2 + q, v[q]);
+          } else {
+            int const j = 16 * c16 + 8 * q;
+            float* const w = mat.w + (tall ? (size_t)(j0 + j) * mat.cols + row : (size_t)row * mat.cols + j0 + j);
+            size_t const step = tall ? mat.cols : 1;
+            float old[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) old[i] = row < m && j + i < mine ? w[i * step] : 0.f;
+            for (int i = 0; i < 8; ++i) old[i] = row < m && j + i < mine ? w[i * step] : 0.f;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) if (row < m && j + i < mine) w[i * step] = old[i] - mat.rate * v[q][i];
-            }
+            for (int i = 0; i < 8; ++i) if (row < m && j + i < mine) w[i * step] = old[i] - mat.rate * v[q][i];
           }
         }
-    }
-    if (dead && lane == 0) atomicCAS(all.status, 0, 44);
+      }
   }
+  if (dead && lane == 0) atomicCAS(all.status, 0, 44);
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
-  if (warp == 16) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace
