@@ -10,7 +10,7 @@
 // A tile is 256 x 256 on a pair of CTAs (cta_group::2: each loads 128 rows of A and 128 of B and holds 128 rows of the accumulator) or 128 x 128 on one.
 // Roles of a CTA's warps: 0-7 drain (warp w: TMEM lanes 32 (w % 4), half w / 4 of the columns), 8 loads A, 10 loads B, 9 issues the MMAs (of the pair's first
 // CTA), 11 completes the warpgroup that gives registers to the drain warps (setmaxnreg moves them by whole warpgroups; a pair's drain threads hold 128 sums each).
-// Persistent: CTAs walk the work (product, tile, range of the reduction) with a stride; pipeline indices run through, so a tile's epilogue overlaps the next
+// Persistent: CTAs walk the work (product, tile, range of the reduction) in a fixed order (item_at); pipeline indices run through, so a tile's epilogue overlaps the next
 // tile's first chains.  A reduction that is cut leaves its partial sums in scratch; the drain warps that take a tile's last ticket add them up in the order of
 // the ranges, so results do not depend on timing.
 #include "pairs.cuh"
@@ -44,11 +44,29 @@ template <int kMax> struct Batch {
   CUtensorMap map[4 * kMax];                            // of each product A along its rows, along its columns, B likewise; those that are used
   Product p[kMax];
   int count, work, three;
+  int lead, behind, even;                               // item_at
   int early;                                            // few CTAs: the next launch may take the other SMs right away
   float* split;
   int* tickets;
   int* status;
 };
+
+// The t-th item of place c of C, or -1: first the longest ones, the first product's `lead` items, with a stride; then the others, of which the `behind` places
+// that had one more of the long ones take `even` less than they otherwise would.  Derivatives of 2047 images, 50001 classes (32 tiles of 782 k-blocks beside 784 of
+// 32): 1277 us with a stride throughout, 927 so.
+template <int kMax>
+__device__ __forceinline__ int item_at(Batch<kMax> const& b, int c, int C, int t)
+{
+  int const first = c < b.lead ? (b.lead - c + C - 1) / C : 0;
+  if (t < first) return c + t * C;
+  t -= first;
+  int w = b.lead + t * C + c;
+  if (t >= b.even) {
+    if (c < b.behind) return -1;
+    w = b.lead + b.even * C + (t - b.even) * (C - b.behind) + c - b.behind;
+  }
+  return w < b.work ? w : -1;
+}
 
 struct Item { int prod, tile, tm, tn, split, kb0, kb1; };
 
@@ -414,7 +432,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
   uint32_t const base = (smem_u32(raw) + 1023u) & ~1023u;
   int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t const rank = kCtas == 2 ? rank_in_cluster() : 0u;
-  int const first = (int)blockIdx.x / kCtas, stride = (int)gridDim.x / kCtas;
+  int const place = (int)blockIdx.x / kCtas, places = (int)gridDim.x / kCtas;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(&full[i]), 2);
@@ -430,8 +448,8 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
   tc_fence_after();
   uint32_t const tmem = tmemAt;
   if (batch.early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 8 * 32 && first < batch.work) {       // the maps of the first item, on their way before there is anything to load
-    CUtensorMap const* const map = batch.map + 4 * item_of(batch, first).prod;
+  if (threadIdx.x == 8 * 32 && place < batch.work) {       // the maps of the first item, on their way before there is anything to load
+    CUtensorMap const* const map = batch.map + 4 * item_of(batch, place).prod;
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"(map + i) : "memory");
   }
@@ -445,7 +463,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
     float* const patch = (float*)(raw + (base - smem_u32(raw)) + kStages * kStageBytes) + warp * kPatch;
     uint32_t const lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kCols);
     int j = 0;
-    for (int w = first; w < batch.work; w += stride) {
+    for (int i = 0, w; (w = item_at(batch, place, places, i)) >= 0; ++i) {
       Item const t = item_of(batch, w);
       Product const& p = batch.p[t.prod];
       int const row0 = t.tm * kTileRows + (int)rank * 128 + quarter * 32, col0 = t.tn * kTileCols + half * kCols;
@@ -512,7 +530,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         bool const isA = warp == 8;
         int it = 0;
         uint32_t const bytes = (batch.three ? 2u : 1u) * kHalfTile;
-        for (int w = first; w < batch.work && !dead; w += stride) {
+        for (int i = 0, w; !dead && (w = item_at(batch, place, places, i)) >= 0; ++i) {
           Item const t = item_of(batch, w);
           Product const& p = batch.p[t.prod];
           int const tile = isA ? t.tm : t.tn, byCols = isA ? p.byColsA : p.byColsB, lower = isA ? p.lowerA : p.lowerB, r0 = tile * kTileRows + (int)rank * 128;
@@ -548,14 +566,15 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
                  (j < kAcc || mbar_wait(smem_u32(&empty[j % kAcc]), (uint32_t)(j / kAcc - 1) & 1u));
         };
         int j = 0;
-        if (first < batch.work) dead = !ready(0);
-        for (int w = first; w < batch.work && !dead; w += stride) {
+        if (place < batch.work) dead = !ready(0);
+        for (int i = 0, w = item_at(batch, place, places, 0), after; !dead && w >= 0; ++i, w = after) {
+          after = item_at(batch, place, places, i + 1);
           Item const t = item_of(batch, w);
           Product const& p = batch.p[t.prod];
           for (int kb = t.kb0; kb < t.kb1 && !dead; ++kb, ++j) {
             int const s = j % kStages, acc = j % kAcc;
             // the next k-block is waited for when the tensor core still has the end of this one to work on: 250 cycles per k-block
-            bool const more = kb + 1 < t.kb1 || w + stride < batch.work;
+            bool const more = kb + 1 < t.kb1 || after >= 0;
             tc_fence_after();
             uint32_t const st = base + (uint32_t)s * kStageBytes, d = tmem + (uint32_t)(acc * kTileCols);
             bool const ca = along_cols(p.byColsA, p.lowerA, t.tm, kTileRows, kb), cb = along_cols(p.byColsB, p.lowerB, t.tn, kTileCols, kb);
@@ -744,39 +763,70 @@ int splits_of(int kBlocks, long long tiles, int clusters, int ctas)
 }
 
 template <int kKind, int kMax, int kCtas>
-int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
+int run(vlb_ctx* ctx, PairProduct const* given, int count, void* split)
 {
   constexpr int kTile = 128 * kCtas;
+  TileCost const& cost = kCost[kCtas - 1];
   Batch<kMax> b;
   b.three = ctx->precision != VLB_PRECISION_TF32;
   int const clusters = ctx->smCount / kCtas;
   long long tiles = 0;
-  for (int i = 0; i < count; ++i) tiles += tiles_of(p[i], kTile);
+  double total = 0;
+  int order[vlb::kMaxPairProducts], splits[vlb::kMaxPairProducts], blocks[vlb::kMaxPairProducts];
+  for (int i = 0; i < count; ++i) {
+    order[i] = i;
+    blocks[i] = vlb::ceil_div(given[i].K, kDepth);
+    tiles += tiles_of(given[i], kTile);
+    total += tiles_of(given[i], kTile) * (blocks[i] * cost.block + cost.ends);
+  }
+  double const share = total / clusters;                // what a place has to do
+  for (int i = 0; i < count; ++i) {
+    splits[i] = splits_of(blocks[i], tiles, clusters, kCtas);
+    // a tile that would take more than half of it is cut too, beside others
+    if (splits[i] == 1 && count > 1 && blocks[i] >= 64) splits[i] = std::max(1, std::min(16, (int)ceil(2 * blocks[i] * cost.block / share)));
+  }
+  std::stable_sort(order, order + count, [&](int x, int y) { return vlb::ceil_div(blocks[x], splits[x]) > vlb::ceil_div(blocks[y], splits[y]); });
   size_t const partBytes = sizeof(float) * 128 * kTile;
   int slot = 0;
   long long part = 0, work = 0;
+  double rest = 0;                                      // time of all but the first product's items
   for (int i = 0; i < count; ++i) {
-    PairProduct const& q = p[i];
+    PairProduct const& q = given[order[i]];
     Product& d = b.p[i];
-    d.M = q.M; d.N = q.N; d.kBlocks = vlb::ceil_div(q.K, kDepth);
+    d.M = q.M; d.N = q.N; d.kBlocks = blocks[order[i]];
     d.tilesM = vlb::ceil_div(q.M, kTile); d.tilesN = vlb::ceil_div(q.N, kTile);
-    int const t = tiles_of(q, kTile);
-    d.splits = 1;
-    int const t2 = splits_of(d.kBlocks, tiles, clusters, kCtas);
-    if (t2 > 1 && (slot + t) * kCtas < 4095 && (size_t)((part + (long long)t * t2) * kCtas) * partBytes <= vlb::kPairSplitBytes) d.splits = t2;
+    int const t = tiles_of(q, kTile), s = splits[order[i]];
+    bool const fits = (slot + t) * kCtas < 4095 && (size_t)((part + (long long)t * s) * kCtas) * partBytes <= vlb::kPairSplitBytes;
+    d.splits = fits ? s : 1;
     d.slot0 = slot; d.part0 = part;
     if (d.splits > 1) { slot += t; part += (long long)t * d.splits; }
     work += (long long)t * d.splits;
+    if (work > INT32_MAX / 4) return vlb::set_error(ctx, VLB_IllegalArgument, "the matrices are too large");
     d.work = (int)work;
+    if (i) rest += (double)t * d.splits * (vlb::ceil_div(d.kBlocks, d.splits) * cost.block + cost.ends);
     d.byColsA = q.a.byCols; d.byColsB = q.b.byCols; d.lowerA = q.a.lower; d.lowerB = q.b.lower; d.symmetric = q.symmetric;
     d.same = q.symmetric && q.a.m.hi == q.b.m.hi && q.a.byCols == q.b.byCols && q.a.lower == q.b.lower;
     d.e = q.e;
     if (!encode_side(&b.map[4 * i], q.a, b.three) || !encode_side(&b.map[4 * i + 2], q.b, b.three))
       return vlb::set_error(ctx, VLB_Cuda, "a tensor map could not be made");
   }
-  if (work > INT32_MAX) return vlb::set_error(ctx, VLB_IllegalArgument, "the matrices are too large");
+  int const places = (int)std::min<long long>(clusters, work);
+  b.lead = count > 1 ? b.p[0].work : (int)work;
+  b.behind = b.lead % places;
+  b.even = (int)work;
+  if (count > 1 && work > b.lead && b.behind) {
+    double const one = vlb::ceil_div(b.p[0].kBlocks, b.p[0].splits) * cost.block + cost.ends, each = rest / (double)(work - b.lead);
+    long long const others = work - b.lead;
+    int const near = (int)std::max(0., ((b.lead * one + rest) / places - (b.lead / places + 1) * one) / each);
+    double least = 1e30;
+    for (int e : {near, near + 1, vlb::ceil_div(others, places)}) {
+      double const behind = (b.lead / places + 1) * one + std::min<long long>(e, vlb::ceil_div(others, places)) * each;
+      double const ahead = (b.lead / places) * one + (e + vlb::ceil_div(std::max(0ll, others - (long long)e * places), places - b.behind)) * each;
+      if (std::max(behind, ahead) < least) { least = std::max(behind, ahead); b.even = e; }
+    }
+  }
   b.count = count; b.work = (int)work;
-  // The next launch's blocks are set up on the free SMs while this one runs, and wait there for its end (pdl_wait): Muon on one 3x3x64x64 bank EARLYFIG.
+  // The next launch's blocks are set up on the free SMs while this one runs, and wait there for its end (pdl_wait): EARLYFIG.
   b.early = std::min<long long>(clusters, work) * kCtas * 2 <= ctx->smCount;
   b.split = (float*)split;
   b.tickets = ctx->deviceStatus + 64;
@@ -797,7 +847,7 @@ int run(vlb_ctx* ctx, PairProduct const* p, int count, void* split)
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = kCtas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(std::min<long long>(clusters, work) * kCtas)); cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3((unsigned)(places * kCtas)); cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem; cfg.stream = ctx->stream; cfg.attrs = attr; cfg.numAttrs = 2;
   cudaLaunchKernelEx(&cfg, kernel, b);
   VLB_LAUNCHED(ctx, 1);
