@@ -356,26 +356,29 @@ __device__ __forceinline__ void finish_grad(Product const& p, Ahead const& ahead
   bool const real = l > 0.f && l <= (float)e.classes;
   if (l > (float)e.classes && e.status) atomicExch(e.status, kStatusBadLabel);
   int const at = min(max((int)l - 1, 0), e.classes - 1) - e.firstClass - col0;
+  // 64 columns at a time, so that the stores of one group are on their way while the next is computed
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) acc[i] = real ? __expf(acc[i] - lse) : 0.f;
-  if (__any_sync(0xffffffffu, real && at >= 0 && at < kCols)) {
+  for (int c0 = 0; c0 < kCols; c0 += 64) {
+    float v[64];
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) acc[i] -= real && i == at ? 1.f : 0.f;
-  }
-  if (e.db) {
+    for (int i = 0; i < 64; ++i) v[i] = real ? __expf(acc[c0 + i] - lse) : 0.f;
+    if (__any_sync(0xffffffffu, real && at >= c0 && at < c0 + 64)) {
 #pragma unroll
-    for (int g = 0; g < kCols / 32; ++g) {
-      float v[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = acc[g * 32 + i];
-      float const s = lane_sums(v);
-      int const c = col0 + g * 32 + (threadIdx.x & 31);
-      if (row0 < p.M && c < p.N) e.db[(long long)(row0 / 32) * e.to.ld + c] = s;
+      for (int i = 0; i < 64; ++i) v[i] -= real && c0 + i == at ? 1.f : 0.f;
     }
-  }
+    if (e.db) {
 #pragma unroll
-  for (int i = 0; i < kCols; i += 64)
-    if (col0 + i < e.to.ld) store_pair64(e.to, row0, col0 + i, min(32, p.M - row0), &acc[i], pow2(e.toExp), patch);
+      for (int g = 0; g < 2; ++g) {
+        float t[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) t[i] = v[g * 32 + i];
+        float const s = lane_sums(t);
+        int const c = col0 + c0 + g * 32 + (threadIdx.x & 31);
+        if (row0 < p.M && c < p.N) e.db[(long long)(row0 / 32) * e.to.ld + c] = s;
+      }
+    }
+    if (col0 + c0 < e.to.ld) store_pair64(e.to, row0, col0 + c0, min(32, p.M - row0), v, pow2(e.toExp), patch);
+  }
 }
 
 template <int kCols>
