@@ -57,5 +57,7 @@ int fc_dgrad_half(vlb_ctx* ctx, ConvGeom const& g, float* dX, float const* F, fl
 int fc_wgrad_half(vlb_ctx* ctx, ConvGeom const& g, float* dF, float const* X, float const* dY);
 cudaError_t half_set_wait_limit(long long cycles, cudaStream_t stream);
 cudaError_t pairs_set_wait_limit(long long cycles, cudaStream_t stream);
+cudaError_t small_set_wait_limit(long long cycles, cudaStream_t stream);
+cudaError_t lnorm_set_wait_limit(long long cycles, cudaStream_t stream);
 
 }  // namespace vlb

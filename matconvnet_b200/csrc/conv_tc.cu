@@ -2345,6 +2345,8 @@ extern "C" int vlb_ctx_set_wait_limit(vlb_ctx* ctx, long long cycles)
   cudaError_t e = cudaMemcpyToSymbolAsync(gWaitCycles, &v, sizeof(v), 0, cudaMemcpyHostToDevice, ctx->stream);
   if (e == cudaSuccess) e = vlb::half_set_wait_limit(cycles, ctx->stream);
   if (e == cudaSuccess) e = vlb::pairs_set_wait_limit(cycles, ctx->stream);
+  if (e == cudaSuccess) e = vlb::small_set_wait_limit(cycles, ctx->stream);
+  if (e == cudaSuccess) e = vlb::lnorm_set_wait_limit(cycles, ctx->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
   if (e != cudaSuccess) { cudaGetLastError(); return vlb::set_error(ctx, VLB_Cuda, cudaGetErrorString(e)); }
   return VLB_Success;

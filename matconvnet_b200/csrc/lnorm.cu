@@ -11,7 +11,8 @@
 
 namespace {
 
-constexpr int kMaxParts = 148 * 4;      // blocks of a backward pass, at most
+// Blocks of a backward pass, at most: four per SM, and parts of 64 MB.
+int most_parts(vlb_ctx* ctx, int C) { return (int)std::max<long long>(1, std::min<long long>(4 * ctx->smCount, (64ll << 20) / (8ll * C))); }
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -615,6 +616,16 @@ bool with_row(int C, F f)
 
 }  // namespace
 
+namespace vlb {
+
+cudaError_t lnorm_set_wait_limit(long long cycles, cudaStream_t stream)
+{
+  long long const v = cycles == 0 ? kWaitCycles : cycles;
+  return cudaMemcpyToSymbolAsync(gWaitCycles, &v, sizeof(v), 0, cudaMemcpyHostToDevice, stream);
+}
+
+}  // namespace vlb
+
 extern "C" {
 
 int vlb_lnorm_forward(vlb_ctx* ctx, float* Y, float const* X, float const* g, float const* b, int H, int W, int C, int N, double eps)
@@ -665,10 +676,10 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
   VLB_REQUIRE(ctx, X && g && dY, "lnorm_backward: null tensor");
   VLB_REQUIRE(ctx, eps >= 0, "lnorm_backward: epsilon is negative");
   if (!dX && !dG && !dB) return VLB_Success;
-  int const P = H * W, positions = P * N;
+  int const P = H * W, positions = P * N, most = most_parts(ctx, C);
   float* parts = nullptr;
   if (dG || dB) {
-    parts = (float*)vlb::workspace(ctx, sizeof(float) * 2 * (size_t)C * kMaxParts);
+    parts = (float*)vlb::workspace(ctx, sizeof(float) * 2 * (size_t)C * most);
     if (!parts) return vlb::pass_error(ctx, ctx->lastError, "vlb_lnorm_backward");
   }
   int blocks = 0;
@@ -679,7 +690,7 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
       constexpr int kThreads = decltype(threads)::value, kVec = decltype(count)::value, kRows = block_of(kThreads) / kThreads;
       // as many blocks as fit the device at once: half of its threads, with sixteen values each of three tensors in registers; groups of rows of 16 KB
       int const perSm = std::max(1, std::min(4, 512 / block_of(kThreads))), per = kThreads == 32 ? std::max(1, std::min(4096 / (C * kRows), N / (kRows * ctx->smCount * perSm))) : 1;
-      blocks = std::min(vlb::ceil_div(N, kRows * per), std::min(kMaxParts, ctx->smCount * perSm));
+      blocks = std::min(vlb::ceil_div(N, kRows * per), std::min(most, ctx->smCount * perSm));
       auto const kernel = vec ? rows_bwd_kernel<kThreads, kVec, true> : rows_bwd_kernel<kThreads, kVec, false>;
       size_t const smem = vec ? sizeof(float) * kStages * 2 * per * kRows * C : 0;
       static bool ready[64];                               // (of this kernel and device)
@@ -692,14 +703,14 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
     });
     if (failed != cudaSuccess) return vlb::set_error(ctx, VLB_Cuda, cudaGetErrorString(failed));
     if (!blocks) {
-      blocks = std::min(N, ctx->smCount * 2);
+      blocks = std::min(N, std::min(most, ctx->smCount * 2));
       vlb::launch(ctx->stream, rows_bwd_long_kernel, (unsigned)blocks, 1024, 0, dX, parts, X, g, dY, N, C, (float)eps);
     }
   }
   if (!blocks) {
     int const tiles = vlb::ceil_div(positions, 32);
     auto run = [&](auto kernel, int warps) {
-      blocks = std::min(tiles, std::min(kMaxParts, ctx->smCount * std::max(1, std::min(4, 32 / warps))));
+      blocks = std::min(tiles, std::min(most, ctx->smCount * std::max(1, std::min(4, 32 / warps))));
       vlb::launch(ctx->stream, kernel, (unsigned)blocks, warps * 32, 0, dX, parts, X, g, dY, (long long)positions, tiles, P, C, (float)eps);
     };
     bool const four = wide(P, {dX, X, dY});

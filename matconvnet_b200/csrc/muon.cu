@@ -10,53 +10,14 @@ namespace {
 
 constexpr int kThreads = 256, kMaxParts = 592;
 
-// Momentum; u = what is to be orthogonalised; a part of the sum of its squares per block, in double precision.
-__global__ void __launch_bounds__(kThreads)
-momentum_kernel(float* __restrict__ u, float* __restrict__ s1, float const* __restrict__ w, float const* __restrict__ g, size_t n, float gradMult,
-                float decay, float momentum, int nesterov, double* __restrict__ parts)
-{
-  vlb::pdl_wait();
-  double sum = 0;
-  for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kThreads) {
-    float const d = gradMult * g[i] + decay * w[i], m = momentum * s1[i] + d, v = nesterov ? d + momentum * m : m;
-    s1[i] = m;
-    u[i] = v;
-    sum += (double)v * v;
-  }
-  __shared__ double all[kThreads / 32];
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kThreads / 32; ++i) sum += all[i];
-    parts[blockIdx.x] = sum;
-  }
-}
-
-__global__ void normalise_kernel(float* __restrict__ u, size_t n, double const* __restrict__ parts, int count, double epsilon)
-{
-  vlb::pdl_wait();
-  double sum = 0;
-  for (int i = 0; i < count; ++i) sum += parts[i];
-  float const f = (float)(1. / (sqrt(sum) + epsilon));
-  for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kThreads) u[i] *= f;
-}
-
-__global__ void step_kernel(float* __restrict__ w, float const* __restrict__ x, size_t n, float rate)
-{
-  vlb::pdl_wait();
-  for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kThreads) w[i] -= rate * x[i];
-}
-
-// ------------------------------------------------------------------ on pairs of halves (pairs.cu)
-constexpr int kMost = vlb::kMaxPairProducts;
+constexpr int kMost = vlb::kMaxPairProducts;          // parameters in one pass
 
 // One parameter's share of a launch over several: blocks block0 ... block0 + blocks - 1.
 struct Job {
   float *w, *s1; float const* g; float* u;
   size_t n;
   float decay, rate;
-  double* parts;                     // sums of squares, one per block of momentum_many_kernel
+  double* parts;                     // sums of squares, one per block of momentum_kernel
   int partCount, block0, blocks, vec;
   vlb::Pair x;
   int rowsPer; vlb::FastDiv perRow;  // make_x_kernel: rows of a block, sixteen columns at a time
@@ -82,8 +43,9 @@ __device__ __forceinline__ double block_sum(double sum)
   return sum;
 }
 
+// Momentum; u = what is to be orthogonalised; a part of the sum of its squares per block, in double precision.
 __global__ void __launch_bounds__(kThreads)
-momentum_many_kernel(const __grid_constant__ Jobs jobs, float gradMult, float momentum, int nesterov)
+momentum_kernel(const __grid_constant__ Jobs jobs, float gradMult, float momentum, int nesterov)
 {
   vlb::pdl_wait();
   int block = blockIdx.x;
@@ -123,7 +85,7 @@ __device__ __forceinline__ float norm_factor(Job const& j, double epsilon)
   return (float)(1. / (sqrt(block_sum(sum)) + epsilon));
 }
 
-// u / (|u| + epsilon) as a pair scaled by 2^e.
+// u / (|u| + epsilon), as a pair scaled by 2^e
 __global__ void __launch_bounds__(kThreads)
 make_x_kernel(const __grid_constant__ Jobs jobs, double epsilon, int e)
 {
@@ -154,9 +116,28 @@ make_x_kernel(const __grid_constant__ Jobs jobs, double epsilon, int e)
   }
 }
 
+// u / (|u| + epsilon) in place
+__global__ void __launch_bounds__(kThreads)
+normalise_kernel(const __grid_constant__ Jobs jobs, double epsilon)
+{
+  vlb::pdl_wait();
+  int block = blockIdx.x;
+  Job const& j = job_of(jobs, block);
+  float const f = norm_factor(j, epsilon);
+  for (size_t i = (size_t)block * kThreads + threadIdx.x; i < j.n; i += (size_t)j.blocks * kThreads) j.u[i] *= f;
+}
+
+// w -= rate * x
+__global__ void __launch_bounds__(kThreads)
+subtract_kernel(float* __restrict__ w, float const* __restrict__ x, size_t n, float rate)
+{
+  vlb::pdl_wait();
+  for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kThreads) w[i] -= rate * x[i];
+}
+
 // Without a Newton-Schulz step.
 __global__ void __launch_bounds__(kThreads)
-step_many_kernel(const __grid_constant__ Jobs jobs, double epsilon)
+step_kernel(const __grid_constant__ Jobs jobs, double epsilon)
 {
   vlb::pdl_wait();
   int block = blockIdx.x;
@@ -198,6 +179,25 @@ struct Exponents {
   }
 };
 
+// What momentum_kernel and those that share its blocks need; u and parts are set.  Returns the number of blocks.
+int set_up(Jobs& jobs, int count, vlb_muon_param const* u)
+{
+  jobs.count = count;
+  int blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    Job& j = jobs.j[i];
+    j.w = u[i].W; j.s1 = u[i].S1; j.g = u[i].G;
+    j.n = (size_t)u[i].rows * u[i].cols;
+    j.decay = (float)u[i].decay;
+    j.rate = (float)(u[i].lr * sqrt(std::max(1., (double)u[i].rows / u[i].cols)));
+    j.vec = j.n % 4 == 0 && (((uintptr_t)j.w | (uintptr_t)j.s1 | (uintptr_t)j.g) & 15) == 0;
+    j.block0 = blocks;
+    j.blocks = j.partCount = (int)vlb::grid_for((j.n + 3) / 4, kThreads, kMaxParts);
+    blocks += j.blocks;
+  }
+  return blocks;
+}
+
 int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* o)
 {
   // all small: all steps in one launch.  (Beside larger ones they cost next to nothing in the launches that those need.)
@@ -223,23 +223,11 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
     }
     if (pass == 0 && !(at = (char*)vlb::workspace(ctx, bytes))) return ctx->lastError;
   }
-  jobs.count = count;
-  int blocks = 0;
-  for (int i = 0; i < count; ++i) {
-    Job& j = jobs.j[i];
-    j.w = u[i].W; j.s1 = u[i].S1; j.g = u[i].G;
-    j.n = (size_t)u[i].rows * u[i].cols;
-    j.decay = (float)u[i].decay;
-    j.rate = (float)(u[i].lr * sqrt(std::max(1., (double)u[i].rows / u[i].cols)));
-    j.vec = j.n % 4 == 0 && (((uintptr_t)j.w | (uintptr_t)j.s1 | (uintptr_t)j.g) & 15) == 0;
-    j.block0 = blocks;
-    j.blocks = j.partCount = (int)vlb::grid_for((j.n + 3) / 4, kThreads, kMaxParts);
-    blocks += j.blocks;
-  }
-  vlb::launch(ctx->stream, momentum_many_kernel, (unsigned)blocks, kThreads, 0, jobs, (float)gradMult, (float)o->momentum, o->nesterov);
+  int blocks = set_up(jobs, count, u);
+  vlb::launch(ctx->stream, momentum_kernel, (unsigned)blocks, kThreads, 0, jobs, (float)gradMult, (float)o->momentum, o->nesterov);
   VLB_LAUNCHED(ctx, 1);
   if (o->steps == 0) {
-    vlb::launch(ctx->stream, step_many_kernel, (unsigned)blocks, kThreads, 0, jobs, o->epsilon);
+    vlb::launch(ctx->stream, step_kernel, (unsigned)blocks, kThreads, 0, jobs, o->epsilon);
     VLB_LAUNCHED(ctx, 1);
     return VLB_Success;
   }
@@ -298,6 +286,32 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
   return VLB_Success;
 }
 
+// VLB_PRECISION_FP32: products on CUDA cores, one parameter after the other.
+int update_exact(vlb_ctx* ctx, vlb_muon_param const& u, double gradMult, vlb_muon_opts const* o)
+{
+  int const rows = u.rows, cols = u.cols, m = std::min(rows, cols);
+  size_t const n = (size_t)rows * cols;
+  Jobs jobs = {};
+  jobs.j[0].parts = (double*)vlb::workspace(ctx, sizeof(double) * kMaxParts + sizeof(float) * (2 * n + 2 * (size_t)m * m));
+  if (!jobs.j[0].parts) return ctx->lastError;
+  float *x = jobs.j[0].u = (float*)(jobs.j[0].parts + kMaxParts), *next = x + n, *const a = next + n, *const q = a + (size_t)m * m;
+  unsigned const blocks = (unsigned)set_up(jobs, 1, &u);
+  vlb::launch(ctx->stream, momentum_kernel, blocks, kThreads, 0, jobs, (float)gradMult, (float)o->momentum, o->nesterov);
+  vlb::launch(ctx->stream, normalise_kernel, blocks, kThreads, 0, jobs, o->epsilon);
+  for (int k = 0; k < o->steps; ++k) {
+    vlb::Strided const byRow = {x, cols, 1}, byCol = {x, 1, cols};
+    if (rows <= cols) vlb::products_exact(ctx, a, m, m, m, cols, byRow, byRow, 1.f, 0.f, nullptr, nullptr);
+    else              vlb::products_exact(ctx, a, m, m, m, rows, byCol, byCol, 1.f, 0.f, nullptr, nullptr);
+    vlb::products_exact(ctx, q, m, m, m, m, {a, m, 1}, {a, m, 1}, (float)o->c, (float)o->b, a, nullptr);
+    if (rows <= cols) vlb::products_exact(ctx, next, cols, rows, cols, rows, {q, m, 1}, byCol, 1.f, (float)o->a, x, nullptr);
+    else              vlb::products_exact(ctx, next, cols, rows, cols, cols, byRow, {q, m, 1}, 1.f, (float)o->a, x, nullptr);
+    std::swap(x, next);
+  }
+  vlb::launch(ctx->stream, subtract_kernel, blocks, kThreads, 0, u.W, x, n, jobs.j[0].rate);
+  VLB_LAUNCHED(ctx, 3);
+  return VLB_Success;
+}
+
 bool overlap(void const* p, size_t n, void const* q, size_t m) { return (char const*)p < (char const*)q + m && (char const*)q < (char const*)p + n; }
 
 // Whether what one of them writes is anything of the other's.
@@ -319,46 +333,19 @@ int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, doubl
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, count >= 0 && (u || count == 0) && o, "muon_update_many: null argument");
   VLB_REQUIRE(ctx, o->steps >= 0 && o->epsilon >= 0, "muon_update_many: steps and epsilon must not be negative");
-  size_t most = 0;
   for (int i = 0; i < count; ++i) {
     VLB_REQUIRE(ctx, u[i].rows > 0 && u[i].cols > 0, "muon_update_many: bad shape");
     VLB_REQUIRE(ctx, u[i].W && u[i].S1 && u[i].G, "muon_update_many: null tensor");
-    size_t const m = std::min(u[i].rows, u[i].cols);
-    most = std::max(most, 2 * (size_t)u[i].rows * u[i].cols + 2 * m * m);
   }
-  if (count == 0) return VLB_Success;
-  if (ctx->precision != VLB_PRECISION_FP32) {
-    for (int first = 0, end; first < count; first = end) {
-      for (end = first + 1; end < count && end - first < kMost; ++end) {
-        bool apart = true;
-        for (int i = first; apart && i < end; ++i) apart = !overlap(u[i], u[end]);
-        if (!apart) break;
-      }
-      if (int const rc = update_on_pairs(ctx, end - first, u + first, gradMult, o)) return vlb::pass_error(ctx, rc, "vlb_muon_update_many");
+  bool const exact = ctx->precision == VLB_PRECISION_FP32;
+  for (int first = 0, end; first < count; first = end) {
+    for (end = first + 1; end < count && end - first < (exact ? 1 : kMost); ++end) {
+      bool apart = true;
+      for (int i = first; apart && i < end; ++i) apart = !overlap(u[i], u[end]);
+      if (!apart) break;
     }
-    return vlb::check_launch(ctx, "vlb_muon_update_many");
-  }
-  double* const parts = (double*)vlb::workspace(ctx, sizeof(double) * kMaxParts + sizeof(float) * most);
-  if (!parts) return vlb::pass_error(ctx, ctx->lastError, "vlb_muon_update_many");
-  for (int i = 0; i < count; ++i) {
-    int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
-    size_t const n = (size_t)rows * cols;
-    float *x = (float*)(parts + kMaxParts), *next = x + n, *const a = next + n, *const q = a + (size_t)m * m;
-    unsigned const grid = vlb::grid_for(n, kThreads, kMaxParts);
-    vlb::launch(ctx->stream, momentum_kernel, grid, kThreads, 0, x, u[i].S1, u[i].W, u[i].G, n, (float)gradMult, (float)u[i].decay,
-                (float)o->momentum, o->nesterov, parts);
-    vlb::launch(ctx->stream, normalise_kernel, grid, kThreads, 0, x, n, parts, (int)grid, o->epsilon);
-    for (int k = 0; k < o->steps; ++k) {
-      vlb::Strided const byRow = {x, cols, 1}, byCol = {x, 1, cols};
-      if (rows <= cols) vlb::products_exact(ctx, a, m, m, m, cols, byRow, byRow, 1.f, 0.f, nullptr, nullptr);
-      else              vlb::products_exact(ctx, a, m, m, m, rows, byCol, byCol, 1.f, 0.f, nullptr, nullptr);
-      vlb::products_exact(ctx, q, m, m, m, m, {a, m, 1}, {a, m, 1}, (float)o->c, (float)o->b, a, nullptr);
-      if (rows <= cols) vlb::products_exact(ctx, next, cols, rows, cols, rows, {q, m, 1}, byCol, 1.f, (float)o->a, x, nullptr);
-      else              vlb::products_exact(ctx, next, cols, rows, cols, cols, byRow, {q, m, 1}, 1.f, (float)o->a, x, nullptr);
-      std::swap(x, next);
-    }
-    vlb::launch(ctx->stream, step_kernel, grid, kThreads, 0, u[i].W, x, n, (float)(u[i].lr * sqrt(std::max(1., (double)rows / cols))));
-    VLB_LAUNCHED(ctx, 3);
+    int const rc = exact ? update_exact(ctx, u[first], gradMult, o) : update_on_pairs(ctx, end - first, u + first, gradMult, o);
+    if (rc) return vlb::pass_error(ctx, rc, "vlb_muon_update_many");
   }
   return vlb::check_launch(ctx, "vlb_muon_update_many");
 }

@@ -25,7 +25,7 @@ constexpr int kPart = 128 * 128, kBlock = 2 * kPart;          // bytes of 128 ro
 constexpr int kMostBlocks = 4;                                // 64-column blocks of X in a CTA
 constexpr size_t kSmem = (size_t)(kMostBlocks + 2) * kBlock + 1024;
 
-struct Matrices { SmallMatrix m[kSmallMost]; SmallSteps steps; int* status; int cluster; };
+struct Matrices { SmallMatrix m[kSmallMost]; SmallSteps steps; int* status; int cluster, idle; };      // idle: test switch, no wait is answered
 
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
 {
@@ -160,8 +160,8 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
     __syncthreads();
     if (threadIdx.x == 0) {
       tc_fence_after();
-      issue();
-      umma_commit(smem_u32(&through));
+      if (!all.idle) issue();
+      if (!all.idle) umma_commit(smem_u32(&through));
     }
     __syncwarp();
     if (!dead && !mbar_wait(smem_u32(&through), phase)) dead = true;
@@ -329,7 +329,8 @@ int small_matrices(vlb_ctx* ctx, SmallMatrix const* m, int count, SmallSteps con
   for (int i = 0; i < count; ++i) { all.m[i] = m[i]; longest = std::max(longest, std::max(m[i].rows, m[i].cols)); }
   all.steps = steps;
   all.status = ctx->deviceStatus;
-  // as many CTAs to a matrix as its longer side has 128 columns for, at most eight (with 256 each 64 x 576 CLUSTERFIG)
+  all.idle = ctx->testSwitch & 1;
+  // as many CTAs to a matrix as its longer side has 128 columns for, at most eight (64 x 576: 58 us; with 256 each 70)
   all.cluster = 1;
   while (all.cluster < 8 && all.cluster * 128 < longest) all.cluster *= 2;
   static bool ready[64];
@@ -349,6 +350,12 @@ int small_matrices(vlb_ctx* ctx, SmallMatrix const* m, int count, SmallSteps con
   cudaLaunchKernelEx(&cfg, small_kernel, all, ctx->precision != VLB_PRECISION_TF32);
   VLB_LAUNCHED(ctx, 1);
   return check_launch(ctx, "small_matrices");
+}
+
+cudaError_t small_set_wait_limit(long long cycles, cudaStream_t stream)
+{
+  long long const v = cycles == 0 ? kWaitCycles : cycles;
+  return cudaMemcpyToSymbolAsync(gWaitCycles, &v, sizeof(v), 0, cudaMemcpyHostToDevice, stream);
 }
 
 }  // namespace vlb

@@ -45,7 +45,7 @@ template <int kMax> struct Batch {
   Product p[kMax];
   int count, work, three;
   int lead, behind, even;                               // item_at
-  int early;                                            // few CTAs: the next launch may take the other SMs right away
+  int idle;                                             // test switch: nothing is loaded, so that every wait runs out
   float* split;
   int* tickets;
   int* status;
@@ -450,7 +450,6 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
   if (kCtas == 2) cluster_sync();
   tc_fence_after();
   uint32_t const tmem = tmemAt;
-  if (batch.early) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 8 * 32 && place < batch.work) {       // the maps of the first item, on their way before there is anything to load
     CUtensorMap const* const map = batch.map + 4 * item_of(batch, place).prod;
 #pragma unroll
@@ -533,7 +532,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         bool const isA = warp == 8;
         int it = 0;
         uint32_t const bytes = (batch.three ? 2u : 1u) * kHalfTile;
-        for (int i = 0, w; !dead && (w = item_at(batch, place, places, i)) >= 0; ++i) {
+        for (int i = 0, w; !dead && !batch.idle && (w = item_at(batch, place, places, i)) >= 0; ++i) {
           Item const t = item_of(batch, w);
           Product const& p = batch.p[t.prod];
           int const tile = isA ? t.tm : t.tn, byCols = isA ? p.byColsA : p.byColsB, lower = isA ? p.lowerA : p.lowerB, r0 = tile * kTileRows + (int)rank * 128;
@@ -772,6 +771,7 @@ int run(vlb_ctx* ctx, PairProduct const* given, int count, void* split)
   TileCost const& cost = kCost[kCtas - 1];
   Batch<kMax> b;
   b.three = ctx->precision != VLB_PRECISION_TF32;
+  b.idle = ctx->testSwitch & 1;
   int const clusters = ctx->smCount / kCtas;
   long long tiles = 0;
   double total = 0;
@@ -829,8 +829,6 @@ int run(vlb_ctx* ctx, PairProduct const* given, int count, void* split)
     }
   }
   b.count = count; b.work = (int)work;
-  // The next launch's blocks are set up on the free SMs while this one runs, and wait there for its end (pdl_wait): EARLYFIG.
-  b.early = std::min<long long>(clusters, work) * kCtas * 2 <= ctx->smCount;
   b.split = (float*)split;
   b.tickets = ctx->deviceStatus + 64;
   b.status = ctx->deviceStatus;

@@ -242,6 +242,112 @@ def test_the_same_every_time_in_a_graph_and_on_another_stream(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,d,k", [(40, 512, 20003), (700, 64, 9000)])
+def test_in_pieces_of_classes(gpu, n, d, k):
+    """Bit 5 of the test switches refuses scratch that a call can do without: the smallest pieces."""
+    from matconvnet_b200 import capi
+    nn, mat, _ = gpu
+    ctx = capi.Context()
+    ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 32))
+    x, f, b, c = _inputs(n, (1, 1, d), k, 12)
+    c[3] = k
+    before = ctx.launches
+    _check(nn, mat, x, f, b, c, (1, 1, d), ctx=ctx)
+    pieces = ctx.launches - before
+    ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 0))
+    before = ctx.launches
+    _check(nn, mat, x, f, b, c, (1, 1, d), ctx=ctx)
+    assert pieces > ctx.launches - before
+
+
+@pytest.mark.gpu
+def test_more_images_than_go_through_at_once(gpu):
+    nn, mat, _ = gpu
+    _check(nn, mat, *_inputs(16384 + 77, (1, 1, 40), 90, 13), (1, 1, 40))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,k", [(2100, 130, 2300), (513, 1030, 900), (1, 50000, 20), (17, 30000, 40)])
+def test_larger_tiles_and_long_rows(gpu, n, d, k):
+    nn, mat, _ = gpu
+    _check(nn, mat, *_inputs(n, (1, 1, d), k, 14), (1, 1, d))
+
+
+@pytest.mark.gpu
+def test_an_image_or_class_is_as_exact_beside_far_larger_ones(gpu):
+    """Values keep their digits down to 2^-28 of the largest of the tensor: images and classes 2^14 smaller than others, each against itself."""
+    nn, mat, _ = gpu
+    n, d, k = 200, 136, 300
+    x, f, b, c = _inputs(n, (1, 1, d), k, 15)
+    c[c == 0] = 1
+    small = np.arange(n) % 2 == 0
+    x[small] *= np.float32(2.0 ** -14)
+    xd, fd, bd, cd = _up(mat, x, f, b, c, (1, 1, d))
+    _, lse, dx, df, _ = _oracle(x, f, b, c)
+    gl, gs = nn.vl_nnfcsoftmaxloss(xd, fd, bd, cd)
+    assert np.abs(gs.cpu().numpy() - lse).max() <= TOL_LSE * 10
+    gx, gf, _ = nn.vl_nnfcsoftmaxloss(xd, fd, bd, cd, 1.0, lse=gs)
+    got = _down(gx)
+    for i in range(n):
+        assert _rel(got[i], dx[i]) <= TOL
+    # half of the classes with filters 2^14 smaller: their derivatives are sums over the same images
+    x, f, b, c = _inputs(n, (1, 1, d), k, 16)
+    f[::2] *= np.float32(2.0 ** -14)
+    xd, fd, bd, cd = _up(mat, x, f, b, c, (1, 1, d))
+    _, lse, dx, df, db = _oracle(x, f, b, c)
+    gx, gf, gb = nn.vl_nnfcsoftmaxloss(xd, fd, bd, cd, 1.0)
+    got = _down(gf)
+    for i in range(k):
+        assert _rel(got[i], df[i]) <= TOL
+    assert _rel(_down(gx), dx) <= TOL and _rel(gb.cpu().numpy(), db) <= TOL
+
+
+@pytest.mark.gpu
+def test_two_contexts_on_two_streams_at_once(gpu):
+    import torch
+    from matconvnet_b200 import capi
+    nn, mat, _ = gpu
+    work = []
+    for i, (n, d, k) in enumerate([(300, 200, 3000), (4, 512, 2000), (900, 72, 700)]):
+        data = _up(mat, *_inputs(n, (1, 1, d), k, 20 + i), (1, 1, d))
+        ctx = capi.Context()
+        want = nn.vl_nnfcsoftmaxloss(*data, ctx=ctx) + nn.vl_nnfcsoftmaxloss(*data, 1.0, ctx=ctx)
+        work.append((data, ctx, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for data, ctx, _, stream in work:
+            with torch.cuda.stream(stream):
+                got.append(nn.vl_nnfcsoftmaxloss(*data, ctx=ctx) + nn.vl_nnfcsoftmaxloss(*data, 1.0, ctx=ctx))
+        torch.cuda.synchronize()
+        for g, (_, ctx, want, _) in zip(got, work):
+            assert all((p == q).all() for p, q in zip(g, want)) and ctx.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out(gpu):
+    """Nothing is loaded, so no wait is ever answered: the kernels give up, say so and leave everything as the next call needs it."""
+    from matconvnet_b200 import capi
+    nn, mat, _ = gpu
+    for n, d, k in ((64, 2048, 200), (2100, 130, 2300)):
+        ctx = capi.Context()
+        data = _up(mat, *_inputs(n, (1, 1, d), k, 17), (1, 1, d))
+        call = lambda: nn.vl_nnfcsoftmaxloss(*data, ctx=ctx) + nn.vl_nnfcsoftmaxloss(*data, 1.0, ctx=ctx)       # noqa: E731
+        want = call()
+        assert ctx.device_status() == 0
+        try:
+            ctx.check(ctx.lib.vlb_ctx_set_wait_limit(ctx.handle, 200000))
+            ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 1))
+            call()
+            with pytest.raises(capi.VlbError, match="TIMEOUT|Timeout|timeout"):
+                ctx.device_status()
+        finally:
+            ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 0))
+            ctx.check(ctx.lib.vlb_ctx_set_wait_limit(ctx.handle, 0))
+        assert all((p == q).all() for p, q in zip(call(), want)) and ctx.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_strides_and_alignment(gpu):
     import torch
     nn, mat, _ = gpu

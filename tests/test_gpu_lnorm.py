@@ -16,8 +16,8 @@ from conftest import rel_l2
 TOL_L2, TOL_MAX = 2e-6, 1.2e-5
 
 SHAPES = [(1, 1, 1, 1), (1, 1, 1, 7), (1, 1, 5, 1), (1, 1, 64, 33), (1, 1, 1024, 1), (1, 1, 1000, 257), (1, 1, 1023, 64), (1, 1, 4096, 70),
-          (1, 1, 4099, 5), (1, 1, 8192, 19), (1, 1, 12289, 6), (1, 1, 70001, 3),
-          (2, 1, 3, 4), (7, 5, 33, 3), (28, 28, 96, 2), (35, 47, 90, 2), (3, 3, 1031, 5), (1, 9, 512, 40), (64, 64, 17, 1), (5, 1, 6001, 2)]
+          (1, 1, 4099, 5), (1, 1, 8192, 19), (1, 1, 12289, 6), (1, 1, 70001, 3), (1, 1, 260, 5000), (1, 1, 64, 40000), (1, 1, 63, 3000),
+          (2, 1, 3, 4), (7, 5, 33, 3), (28, 28, 96, 2), (35, 47, 90, 2), (3, 3, 1031, 5), (1, 9, 512, 40), (64, 64, 17, 1), (5, 1, 6001, 2), (2, 2, 200, 700), (4, 1, 300, 9), (2, 6, 700, 3), (3, 1, 250, 2)]
 
 
 def _inputs(shape, seed=0, offset=0.5):
