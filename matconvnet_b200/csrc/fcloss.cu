@@ -382,21 +382,22 @@ few_predict_kernel(FewArgs a)
 #pragma unroll
     for (int r = 0; r < kRows; ++r) f[r] = a.f + (size_t)min(k + r, k1 - 1) * a.D;
 #pragma unroll 4
-    for (int d = 4 * lane; d < ld; d += 128) {
+    for (int d = kWide ? 4 * lane : lane; d < ld; d += 128) {      // four neighbouring columns, or four 32 apart
       float4 w[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         if (kWide) {
           w[r] = d < a.D ? __ldg((float4 const*)(f[r] + d)) : make_float4(0, 0, 0, 0);
         } else {
-          w[r].x = d < a.D ? __ldg(f[r] + d) : 0.f; w[r].y = d + 1 < a.D ? __ldg(f[r] + d + 1) : 0.f;
-          w[r].z = d + 2 < a.D ? __ldg(f[r] + d + 2) : 0.f; w[r].w = d + 3 < a.D ? __ldg(f[r] + d + 3) : 0.f;
+          w[r].x = d < a.D ? __ldg(f[r] + d) : 0.f; w[r].y = d + 32 < a.D ? __ldg(f[r] + d + 32) : 0.f;
+          w[r].z = d + 64 < a.D ? __ldg(f[r] + d + 64) : 0.f; w[r].w = d + 96 < a.D ? __ldg(f[r] + d + 96) : 0.f;
         }
       }
 #pragma unroll
       for (int i = 0; i < kImages; ++i) {
         if (kImages > 1 && i >= a.N) break;
-        float4 const q = *(float4 const*)(xs + i * ld + d);
+        float const* const xi = xs + i * ld + d;
+        float4 const q = kWide ? *(float4 const*)xi : make_float4(xi[0], xi[32], xi[64], xi[96]);
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
           acc[r * kImages + i] = fmaf(w[r].x, q.x, fmaf(w[r].y, q.y, fmaf(w[r].z, q.z, fmaf(w[r].w, q.w, acc[r * kImages + i]))));

@@ -643,6 +643,29 @@ struct SplitJob {
 };
 struct SplitJobs { SplitJob j[2]; int count; };
 
+// Sixteen neighbouring floats from p on, by 16-byte loads whatever the alignment of p; those in front of `begin` and from `end` on are not touched.
+__device__ __forceinline__ void load16(float (&v)[16], float const* p, float const* begin, float const* end)
+{
+  int const s = (int)((uintptr_t)p >> 2) & 3;
+  float const* const q = p - s;
+  float t[20];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) {
+    float const* const a = q + 4 * i;
+    if (a >= begin && a + 4 <= end) {
+      float4 const f = __ldg((float4 const*)a);
+      t[4 * i] = f.x; t[4 * i + 1] = f.y; t[4 * i + 2] = f.z; t[4 * i + 3] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[4 * i + k] = a + k >= begin && a + k < end ? __ldg(a + k) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 19; ++i) t[i] = s & 1 ? t[i + 1] : t[i];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = s & 2 ? t[i + 2] : t[i];
+}
+
 __global__ void __launch_bounds__(kSplitThreads)
 largest_kernel(const __grid_constant__ SplitJobs jobs)
 {
@@ -651,21 +674,38 @@ largest_kernel(const __grid_constant__ SplitJobs jobs)
   int const lane = threadIdx.x & 31, block = (int)blockIdx.x - j.block0, cols = j.s.to.cols;
   long long const units = (long long)j.s.to.rows * j.segments;
   unsigned m = 0;
-  for (long long u = (long long)block * (kSplitThreads / 32) + (threadIdx.x >> 5); u < units; u += (long long)j.blocks * (kSplitThreads / 32)) {
-    long long const row = u / j.segments;
-    int const c0 = (int)(u - row * j.segments) * kSegment, c1 = min(c0 + kSegment, cols);
-    if (!is_real(j.s.labels, row, j.s.classes)) continue;
-    float const* const x = j.s.x + row * cols;
-    if (j.vec) {
+  if (!j.s.labels) {                                      // one run of floats: a head up to a 16-byte boundary, fours, a tail
+    long long const n = (long long)j.s.to.rows * cols, head = min(n, (long long)((4 - ((uintptr_t)j.s.x >> 2)) & 3)), fours = (n - head) / 4;
+    float4 const* const x4 = (float4 const*)(j.s.x + head);
+    long long const step = (long long)j.blocks * kSplitThreads;
+    for (long long i = (long long)block * kSplitThreads + threadIdx.x; i < fours; i += 8 * step) {
+      float4 q[8];
 #pragma unroll
-      for (int i = 0; i < kSegment / 128; ++i) {
-        int const c = c0 + 4 * (lane + 32 * i);
-        float4 const q = c < c1 ? __ldg((float4 const*)(x + c)) : make_float4(0, 0, 0, 0);
-        m = max(max(m, max(finite_bits(q.x), finite_bits(q.y))), max(finite_bits(q.z), finite_bits(q.w)));
-      }
-    } else {
+      for (int k = 0; k < 8; ++k) q[k] = __ldg(x4 + min(i + k * step, fours - 1));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = max(max(m, max(finite_bits(q[k].x), finite_bits(q[k].y))), max(finite_bits(q[k].z), finite_bits(q[k].w)));
+    }
+    if (block == 0) {
+      if (threadIdx.x < head) m = max(m, finite_bits(__ldg(j.s.x + threadIdx.x)));
+      if (threadIdx.x < n - head - 4 * fours) m = max(m, finite_bits(__ldg(j.s.x + head + 4 * fours + threadIdx.x)));
+    }
+  } else {
+    for (long long u = (long long)block * (kSplitThreads / 32) + (threadIdx.x >> 5); u < units; u += (long long)j.blocks * (kSplitThreads / 32)) {
+      long long const row = u / j.segments;
+      int const c0 = (int)(u - row * j.segments) * kSegment, c1 = min(c0 + kSegment, cols);
+      if (!is_real(j.s.labels, row, j.s.classes)) continue;
+      float const* const x = j.s.x + row * cols;
+      if (j.vec) {
+#pragma unroll
+        for (int i = 0; i < kSegment / 128; ++i) {
+          int const c = c0 + 4 * (lane + 32 * i);
+          float4 const q = c < c1 ? __ldg((float4 const*)(x + c)) : make_float4(0, 0, 0, 0);
+          m = max(max(m, max(finite_bits(q.x), finite_bits(q.y))), max(finite_bits(q.z), finite_bits(q.w)));
+        }
+      } else {
 #pragma unroll 8
-      for (int c = c0 + lane; c < c1; c += 32) m = max(m, finite_bits(__ldg(x + c)));
+        for (int c = c0 + lane; c < c1; c += 32) m = max(m, finite_bits(__ldg(x + c)));
+      }
     }
   }
   m = __reduce_max_sync(0xffffffffu, m);
@@ -713,11 +753,10 @@ make_pair_kernel(const __grid_constant__ SplitJobs jobs)
           v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
         }
       } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = c + i < to.cols ? __ldg(p + i) : 0.f;
+        load16(v, p, j.s.x, j.s.x + (long long)to.rows * to.cols);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = real ? v[i] * f : 0.f;
+      for (int i = 0; i < 16; ++i) v[i] = real && c + i < to.cols ? v[i] * f : 0.f;
       store_pair16(to, row, c, v);
     }
 }
