@@ -186,7 +186,8 @@ constexpr size_t kMostScratch = 1u << 30;   // what the pieces of classes may ta
 struct Plan {
   int images, piece;                        // images at a time, classes at a time
   size_t bytes;
-  unsigned *largest, *partial;              // of X, of the piece of F
+  int *expX, *expF;                         // exponents of X and of the piece of F
+  unsigned* partial;
   char *x, *f, *dz, *split;
   float2* parts; float *label, *lse, *db;
   double* sums;
@@ -200,8 +201,9 @@ struct Plan {
     piece = (int)std::min<long long>(K, vlb::ceil_div(vlb::ceil_div(K, pieces), 256) * 256ll);
     bytes = 0;
     auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
-    largest = (unsigned*)take(256);
-    partial = (unsigned*)take(2 * sizeof(unsigned) * vlb::kPairPartials);
+    expX = (int*)take(sizeof(int) * (size_t)vlb::ceil_div(images, 64));
+    expF = (int*)take(sizeof(int) * (size_t)vlb::ceil_div(piece, 64));
+    partial = (unsigned*)take(sizeof(unsigned) * (vlb::pair_partials(images) + vlb::pair_partials(piece)));
     x = take(vlb::pair_bytes(images, D));
     f = take(vlb::pair_bytes(piece, D));
     split = take(vlb::kPairSplitBytes);
@@ -238,7 +240,7 @@ Sides sides(Problem const& q, Plan const& plan, int n0, int k0, bool withImages)
 {
   int const rows = std::min(plan.images, q.N - n0), cols = std::min(plan.piece, q.K - k0);
   Sides const s = {vlb::pair_at(plan.x, rows, q.D), vlb::pair_at(plan.f, cols, q.D)};
-  vlb::PairSource const from[2] = {{s.f, q.F + (size_t)k0 * q.D, plan.largest + 1, nullptr, 0}, {s.x, q.X + (size_t)n0 * q.D, plan.largest, q.labels + n0, q.K}};
+  vlb::PairSource const from[2] = {{s.f, q.F + (size_t)k0 * q.D, plan.expF, nullptr, 0}, {s.x, q.X + (size_t)n0 * q.D, plan.expX, q.labels + n0, q.K}};
   vlb::make_pairs(q.ctx, from, withImages ? 2 : 1, plan.partial);
   return s;
 }
@@ -248,7 +250,7 @@ vlb::PairProduct predictions(Problem const& q, Plan const& plan, vlb::Pair x, vl
   vlb::PairProduct p = {};
   p.a = {x, false, false}; p.b = {f, false, false};
   p.M = x.rows; p.N = f.rows; p.K = q.D;
-  p.e.ea.largest = plan.largest; p.e.eb.largest = plan.largest + 1;
+  p.e.ea.blocks = plan.expX; p.e.eb.blocks = plan.expF;
   p.e.bias = q.b ? q.b + k0 : nullptr;
   p.e.labels = q.labels + n0;
   p.e.firstClass = k0; p.e.classes = q.K;
@@ -315,14 +317,14 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
         vlb::PairProduct& d = two[count++];
         d.a = {dz, false, false}; d.b = {f, true, false};
         d.M = x.rows; d.N = q.D; d.K = cols;
-        d.e.eb.largest = plan.largest + 1;
+        d.e.eb.blocks = plan.expF;
         d.e.out = dX + (size_t)n0 * q.D; d.e.beta = k0 ? 1.f : 0.f;
       }
       if (dF) {
         vlb::PairProduct& d = two[count++];
         d.a = {dz, true, false}; d.b = {x, true, false};
         d.M = cols; d.N = q.D; d.K = x.rows;
-        d.e.eb.largest = plan.largest;
+        d.e.eb.blocks = plan.expX;
         d.e.out = dF + (size_t)k0 * q.D; d.e.beta = n0 ? 1.f : 0.f;
       }
       for (int i = 0; i < count; ++i) { two[i].e.ea.value = kDzExp; two[i].e.alpha = scale; two[i].e.ldc = q.D; }

@@ -21,7 +21,7 @@ namespace {
 
 using vlb::PairEpilogue; using vlb::PairKind; using vlb::PairProduct; using vlb::Pair;
 using vlb::kPairOut; using vlb::kPairSeen; using vlb::kPairGrad; using vlb::kPairPoly;
-using vlb::pow2; using vlb::exp_of; using vlb::store_pair16;
+using vlb::pow2; using vlb::store_pair16;
 
 constexpr int kThreads = 384, kDrainWarps = 8;
 constexpr int kLaunchRegs = 168, kDrainRegs = 224, kOtherRegs = 56;     // registers per thread: 8 * 224 + 4 * 56 = 12 * 168
@@ -263,13 +263,19 @@ __device__ __forceinline__ void update_rows(float* out, long long ldc, int M, in
 
 // What the epilogue of a tile takes from global memory, fetched before its products: the sides' scales, and for predictions the row's label and lse and, in the
 // warp's patch, the columns' biases (-inf beyond the last column).  Fetched when they are needed they cost 2 us per tile.
-struct Ahead { float fa, fb, label, lse; };
+struct Ahead { float fa, fb[2], label, lse; };             // fb: of the thread's first and second 64 columns
+
+// The factor that takes the exponent of row `row` of a side back; a side whose rows are the reduction has its factors in the chains.
+__device__ __forceinline__ float unscale(vlb::PairExp const& e, int byCols, int row)
+{ return e.blocks ? (byCols ? 1.f : pow2(-__ldg(e.blocks + row / 64))) : pow2(-e.value); }
 
 template <int kKind, int kCols>
 __device__ __forceinline__ Ahead fetch_ahead(Product const& p, int row, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  Ahead a = {pow2(-exp_of(e.ea)), pow2(-exp_of(e.eb)), 0.f, 0.f};
+  Ahead a = {unscale(e.ea, p.byColsA, min(row, p.M - 1)), {}, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kCols / 64; ++i) a.fb[i] = unscale(e.eb, p.byColsB, min(col0 + 64 * i, p.N - 1));
   if (kKind == kPairSeen || kKind == kPairGrad) {
     if (row < p.M) {
       a.label = __ldg(e.labels + row);
@@ -289,8 +295,10 @@ template <int kCols>
 __device__ __forceinline__ void finish_out(Product const& p, Ahead const& ahead, float (&acc)[kCols], int row0, int col0, float* patch)
 {
   PairEpilogue const& e = p.e;
-  float const fa = ahead.fa, fb = ahead.fb, alpha = e.alpha;
-  update_rows(e.out, e.ldc, p.M, p.N, e.beta != 0.f, acc, row0, col0, patch, [&](float old, float v) { return v * fa * fb * alpha + old; });
+  float const fa = ahead.fa, alpha = e.alpha;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) acc[i] *= ahead.fb[i / 64];
+  update_rows(e.out, e.ldc, p.M, p.N, e.beta != 0.f, acc, row0, col0, patch, [&](float old, float v) { return v * fa * alpha + old; });
 }
 
 // predictions = product + bias in place, -inf beyond the last column
@@ -300,8 +308,9 @@ __device__ __forceinline__ void predictions(Ahead const& a, float (&acc)[kCols],
 #pragma unroll
   for (int i = 0; i < kCols; i += 4) {
     float4 const b = *(float4 const*)(patch + i);
-    acc[i] = fmaf(acc[i] * a.fa, a.fb, b.x); acc[i + 1] = fmaf(acc[i + 1] * a.fa, a.fb, b.y);
-    acc[i + 2] = fmaf(acc[i + 2] * a.fa, a.fb, b.z); acc[i + 3] = fmaf(acc[i + 3] * a.fa, a.fb, b.w);
+    float const f = a.fb[i / 64];
+    acc[i] = fmaf(acc[i] * a.fa, f, b.x); acc[i + 1] = fmaf(acc[i + 1] * a.fa, f, b.y);
+    acc[i + 2] = fmaf(acc[i + 2] * a.fa, f, b.z); acc[i + 3] = fmaf(acc[i + 3] * a.fa, f, b.w);
   }
   __syncwarp();
 }
@@ -386,7 +395,7 @@ __device__ __forceinline__ void finish_poly(Product const& p, Ahead const& ahead
 {
   PairEpilogue const& e = p.e;
   int const rows = min(32, p.M - row0);
-  float const f = e.alpha * ahead.fa * ahead.fb;
+  float const f = e.alpha * ahead.fa * ahead.fb[0];            // (one number on either side)
 #pragma unroll
   for (int i = 0; i < kCols; ++i) acc[i] *= f;
   if (e.beta != 0.f) {
@@ -473,7 +482,12 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
       float acc[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+      // exponents that change with the k-block: of a side whose rows are the reduction
+      int const* const chainExp = kKind != kPairOut ? nullptr : p.byColsA && p.e.ea.blocks ? p.e.ea.blocks : p.byColsB ? p.e.eb.blocks : nullptr;
+      int nextExp = kKind == kPairOut && chainExp ? __ldg(chainExp + t.kb0) : 0;
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++j) {
+        float const f = pow2(-nextExp);
+        if (kKind == kPairOut && chainExp && kb + 1 < t.kb1) nextExp = __ldg(chainExp + kb + 1);
         if (!dead && !mbar_wait(smem_u32(&done[j % kRing]), (uint32_t)(j / kRing) & 1u)) dead = true;
         if (dead) continue;
         tc_fence_after();
@@ -486,7 +500,10 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
           tmem_ld_wait();
           if (g + 1 < kCols / 16) tmem_ld16_issue(at + 16u * (g + 1), r[(g + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[g * 16 + i] += __uint_as_float(r[g & 1][i]);
+          for (int i = 0; i < 16; ++i) {
+            float const v = __uint_as_float(r[g & 1][i]);
+            acc[g * 16 + i] = kKind == kPairOut ? fmaf(v, f, acc[g * 16 + i]) : acc[g * 16 + i] + v;
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -631,15 +648,16 @@ __device__ __forceinline__ unsigned finite_bits(float v)
   return b < 0x7f800000u ? b : 0u;
 }
 
-constexpr int kSplitThreads = 256;
-constexpr int kSegment = 1024;                // floats of a row that a warp takes at a time
+// 64 rows, which share an exponent, are cut into segments of columns where there are few of them: a block takes one.  First the blocks' largest magnitudes, in a launch
+// of their own, then the pairs.  (Both in one launch by blocks that have all of their 64 rows, the second reading from L2: 124 us instead of 44 + 65 for 50001 x 1000,
+// 472 instead of 130 + 268 for 100000 x 2048: what L2 holds of them is too few blocks to keep the memory busy.)
+constexpr int kSplitThreads = 512;
 
 struct SplitJob {
   vlb::PairSource s;
-  unsigned* partial;                          // largest magnitude seen by each block of largest_kernel
-  int block0, blocks, segments;               // blocks of largest_kernel; segments of a row
-  int pair0, pairs, rowsPer, vec;             // blocks of make_pair_kernel, their rows at a time
-  vlb::FastDiv perRow;
+  unsigned* partial;                          // largest magnitude of each block
+  int block0, segments, groups, vec;          // first block; segments of 64 rows; columns / 16 of a segment
+  vlb::FastDiv31 perRow;                      // by groups
 };
 struct SplitJobs { SplitJob j[2]; int count; };
 
@@ -666,99 +684,81 @@ __device__ __forceinline__ void load16(float (&v)[16], float const* p, float con
   for (int i = 0; i < 16; ++i) v[i] = s & 2 ? t[i + 2] : t[i];
 }
 
-__global__ void __launch_bounds__(kSplitThreads)
-largest_kernel(const __grid_constant__ SplitJobs jobs)
+// f(row, column, sixteen values) for the columns of a block; rows that count as zeros give zeros.
+template <class F>
+__device__ __forceinline__ void each16(SplitJob const& j, int rb, int seg, F f)
 {
-  vlb::pdl_wait();
-  SplitJob const& j = jobs.j[jobs.count > 1 && (int)blockIdx.x >= jobs.j[1].block0];
-  int const lane = threadIdx.x & 31, block = (int)blockIdx.x - j.block0, cols = j.s.to.cols;
-  long long const units = (long long)j.s.to.rows * j.segments;
-  unsigned m = 0;
-  if (!j.s.labels) {                                      // one run of floats: a head up to a 16-byte boundary, fours, a tail
-    long long const n = (long long)j.s.to.rows * cols, head = min(n, (long long)((4 - ((uintptr_t)j.s.x >> 2)) & 3)), fours = (n - head) / 4;
-    float4 const* const x4 = (float4 const*)(j.s.x + head);
-    long long const step = (long long)j.blocks * kSplitThreads;
-    for (long long i = (long long)block * kSplitThreads + threadIdx.x; i < fours; i += 8 * step) {
-      float4 q[8];
+  vlb::Pair const& to = j.s.to;
+  int const first = seg * j.groups, most = min(j.groups, (int)(to.ld / 16) - first);
+  float const* const end = j.s.x + (long long)to.rows * to.cols;
+#pragma unroll 2
+  for (int t = threadIdx.x; t < 64 * j.groups; t += kSplitThreads) {
+    int const r = j.perRow(t), g = t - r * j.groups, c = (first + g) * 16;
+    long long const row = rb * 64ll + r;
+    if (row >= to.rows || g >= most) continue;
+    float v[16];
+    float const* const p = j.s.x + row * to.cols + c;
+    if (j.vec && c + 16 <= to.cols) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = __ldg(x4 + min(i + k * step, fours - 1));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(max(m, max(finite_bits(q[k].x), finite_bits(q[k].y))), max(finite_bits(q[k].z), finite_bits(q[k].w)));
-    }
-    if (block == 0) {
-      if (threadIdx.x < head) m = max(m, finite_bits(__ldg(j.s.x + threadIdx.x)));
-      if (threadIdx.x < n - head - 4 * fours) m = max(m, finite_bits(__ldg(j.s.x + head + 4 * fours + threadIdx.x)));
-    }
-  } else {
-    for (long long u = (long long)block * (kSplitThreads / 32) + (threadIdx.x >> 5); u < units; u += (long long)j.blocks * (kSplitThreads / 32)) {
-      long long const row = u / j.segments;
-      int const c0 = (int)(u - row * j.segments) * kSegment, c1 = min(c0 + kSegment, cols);
-      if (!is_real(j.s.labels, row, j.s.classes)) continue;
-      float const* const x = j.s.x + row * cols;
-      if (j.vec) {
-#pragma unroll
-        for (int i = 0; i < kSegment / 128; ++i) {
-          int const c = c0 + 4 * (lane + 32 * i);
-          float4 const q = c < c1 ? __ldg((float4 const*)(x + c)) : make_float4(0, 0, 0, 0);
-          m = max(max(m, max(finite_bits(q.x), finite_bits(q.y))), max(finite_bits(q.z), finite_bits(q.w)));
-        }
-      } else {
-#pragma unroll 8
-        for (int c = c0 + lane; c < c1; c += 32) m = max(m, finite_bits(__ldg(x + c)));
+      for (int i = 0; i < 4; ++i) {
+        float4 const q = __ldg((float4 const*)p + i);
+        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
       }
+    } else {
+      load16(v, p, j.s.x, end);
     }
-  }
-  m = __reduce_max_sync(0xffffffffu, m);
-  __shared__ unsigned all[kSplitThreads / 32];
-  if (lane == 0) all[threadIdx.x >> 5] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kSplitThreads / 32; ++i) m = max(m, all[i]);
-    j.partial[block] = m;
+    bool const real = is_real(j.s.labels, row, j.s.classes);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = real && c + i < to.cols ? v[i] : 0.f;
+    f(row, c, v);
   }
 }
 
-// A block takes rowsPer rows at a time, a thread sixteen neighbouring columns.
-__global__ void __launch_bounds__(kSplitThreads)
-make_pair_kernel(const __grid_constant__ SplitJobs jobs)
+__device__ __forceinline__ unsigned block_max(unsigned m)
 {
-  vlb::pdl_wait();
-  SplitJob const& j = jobs.j[jobs.count > 1 && (int)blockIdx.x >= jobs.j[1].pair0];
-  int const block = (int)blockIdx.x - j.pair0;
-  unsigned m = 0;
-  for (int i = threadIdx.x; i < j.blocks; i += kSplitThreads) m = max(m, __ldg(j.partial + i));
-  m = __reduce_max_sync(0xffffffffu, m);
   __shared__ unsigned all[kSplitThreads / 32];
+  m = __reduce_max_sync(0xffffffffu, m);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = m;
   __syncthreads();
   m = all[0];
 #pragma unroll
   for (int i = 1; i < kSplitThreads / 32; ++i) m = max(m, all[i]);
-  if (block == 0 && threadIdx.x == 0) *j.s.largest = m;
-  vlb::Pair const& to = j.s.to;
-  float const f = pow2(vlb::pair_exp(__uint_as_float(m)));
-  int const groups = (int)(to.ld / 16);
-  for (long long row0 = (long long)block * j.rowsPer; row0 < to.rows; row0 += (long long)j.pairs * j.rowsPer)
-    for (int t = threadIdx.x; t < j.rowsPer * groups; t += kSplitThreads) {
-      int const r = j.perRow(t), c = (t - r * groups) * 16;
-      long long const row = row0 + r;
-      if (row >= to.rows) break;
-      float v[16];
-      bool const real = is_real(j.s.labels, row, j.s.classes);
-      float const* const p = j.s.x + row * to.cols + c;
-      if (j.vec && c + 16 <= to.cols) {
+  return m;
+}
+
+__global__ void __launch_bounds__(kSplitThreads)
+largest_kernel(const __grid_constant__ SplitJobs jobs)
+{
+  vlb::pdl_wait();
+  SplitJob const& j = jobs.j[jobs.count > 1 && (int)blockIdx.x >= jobs.j[1].block0];
+  int const block = (int)blockIdx.x - j.block0, rb = block / j.segments;
+  unsigned m = 0;
+  each16(j, rb, block - rb * j.segments, [&](long long, int, float const (&v)[16]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float4 const q = __ldg((float4 const*)p + i);
-          v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-        }
-      } else {
-        load16(v, p, j.s.x, j.s.x + (long long)to.rows * to.cols);
-      }
+    for (int i = 0; i < 16; ++i) m = max(m, finite_bits(v[i]));
+  });
+  m = block_max(m);
+  if (threadIdx.x == 0) j.partial[block] = m;
+}
+
+__global__ void __launch_bounds__(kSplitThreads)
+make_pair_kernel(const __grid_constant__ SplitJobs jobs)
+{
+  vlb::pdl_wait();
+  SplitJob const& j = jobs.j[jobs.count > 1 && (int)blockIdx.x >= jobs.j[1].block0];
+  int const block = (int)blockIdx.x - j.block0, rb = block / j.segments, seg = block - rb * j.segments;
+  unsigned m = 0;
+  for (int i = threadIdx.x; i < j.segments; i += kSplitThreads) m = max(m, __ldg(j.partial + rb * j.segments + i));
+  m = block_max(m);
+  int const e = vlb::pair_exp(__uint_as_float(m));
+  if (seg == 0 && threadIdx.x == 0) j.s.exps[rb] = e;
+  float const f = pow2(e);
+  each16(j, rb, seg, [&](long long row, int c, float (&v)[16]) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = real && c + i < to.cols ? v[i] * f : 0.f;
-      store_pair16(to, row, c, v);
-    }
+    for (int i = 0; i < 16; ++i) v[i] *= f;
+    store_pair16(j.s.to, row, c, v);
+  });
 }
 
 // ------------------------------------------------------------------ host
@@ -908,24 +908,24 @@ void make_pairs(vlb_ctx* ctx, PairSource const* s, int count, unsigned* partial)
 {
   SplitJobs jobs;
   jobs.count = count;
-  int blocks = 0, pairs = 0;
+  int blocks = 0;
   for (int i = 0; i < count; ++i) {
     SplitJob& j = jobs.j[i];
     j.s = s[i];
-    j.partial = partial + i * kPairPartials;
-    j.segments = ceil_div(s[i].to.cols, kSegment);
+    j.partial = partial;
+    partial += pair_partials(s[i].to.rows);
     j.vec = ((uintptr_t)s[i].x & 15) == 0 && s[i].to.cols % 4 == 0;
+    int const rowBlocks = ceil_div(s[i].to.rows, 64), all = (int)(s[i].to.ld / 16);
+    // two blocks per SM where 64 rows at a time do not give as many; sixteen columns of all 64 rows, two per thread, at least
+    int const want = std::min(ceil_div(all, 16), std::max(1, 2 * ctx->smCount / rowBlocks));
+    j.groups = ceil_div(all, want);
+    j.segments = ceil_div(all, j.groups);
+    j.perRow = FastDiv31(j.groups);
     j.block0 = blocks;
-    j.blocks = (int)std::min<long long>(((long long)s[i].to.rows * j.segments + kSplitThreads / 32 - 1) / (kSplitThreads / 32), std::min(ctx->smCount * 6, kPairPartials));
-    int const groups = (int)(s[i].to.ld / 16);
-    j.rowsPer = std::max(1, 512 / groups);
-    j.perRow = FastDiv(groups);
-    j.pair0 = pairs;
-    j.pairs = std::min(ceil_div(s[i].to.rows, j.rowsPer), ctx->smCount * 8);
-    blocks += j.blocks; pairs += j.pairs;
+    blocks += rowBlocks * j.segments;
   }
   launch(ctx->stream, largest_kernel, (unsigned)blocks, kSplitThreads, 0, jobs);
-  launch(ctx->stream, make_pair_kernel, (unsigned)pairs, kSplitThreads, 0, jobs);
+  launch(ctx->stream, make_pair_kernel, (unsigned)blocks, kSplitThreads, 0, jobs);
   VLB_LAUNCHED(ctx, 2);
 }
 

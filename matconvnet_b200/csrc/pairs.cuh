@@ -6,8 +6,8 @@
 namespace vlb {
 
 // A matrix of single-precision values x as  x * 2^e = hi + lo * 2^-11  with hi = half(x * 2^e), lo = half((x * 2^e - hi) * 2^11): 22 significant bits where the
-// largest magnitude lies in [2^14, 2^15) for everything down to 2^-28 of it, an error of 2^-50 of it below that.  Rows of ld halves, ld a multiple of 64; what
-// lies between cols and ld is not read.
+// largest magnitude lies in [2^14, 2^15) for everything down to 2^-28 of it, an error of 2^-50 of it below that.  e belongs to 64 rows -- the rows of a k-block where
+// they are the reduction -- or is one number.  Rows of ld halves, ld a multiple of 64; what lies between cols and ld is not read.
 struct Pair {
   __half *hi, *lo;
   int rows, cols;
@@ -26,8 +26,8 @@ inline Pair pair_at(void* p, int rows, int cols)
 // matrix only the tiles on and under the diagonal are there, as a symmetric product with the same tiles left them.
 struct PairSide { Pair m; bool byCols, lower; };
 
-// The exponent e of a pair: that of the largest magnitude, whose bits are in a word on the device, or a number.
-struct PairExp { unsigned const* largest; int value; };
+// The exponents of a pair: one per 64 rows, on the device, or a number.
+struct PairExp { int const* blocks; int value; };
 
 enum PairKind {
   kPairOut = 0,      // out = [out +] alpha * product
@@ -64,12 +64,12 @@ constexpr size_t kPairSplitBytes = 64u << 20;
 // Parts per row that kPairSeen writes of N columns.
 inline int pair_parts(int N, int tile) { return 2 * ceil_div(N, tile); }
 
-// A matrix of floats, rows one after the other, to be made a pair: with the exponent of its largest finite magnitude, whose bits are left in *largest.
+// A matrix of floats, rows one after the other, to be made a pair, with the exponent of the largest finite magnitude of each 64 rows, left in exps.
 // labels (or NULL): rows whose label is not in 1 ... classes count as zeros, whatever they hold.
-struct PairSource { Pair to; float const* x; unsigned* largest; float const* labels; int classes; };
+struct PairSource { Pair to; float const* x; int* exps; float const* labels; int classes; };
 
-// One or two of them, in two launches.  partial: kPairPartials words of scratch for each.
-constexpr int kPairPartials = 1024;
+// One or two of them.  partial: pair_partials(rows) words of scratch for each, one after the other.
+inline size_t pair_partials(int rows) { return (size_t)ceil_div(rows, 64) + 1024; }
 void make_pairs(vlb_ctx* ctx, PairSource const* s, int count, unsigned* partial);
 
 // The tiles, 256 x 256 or 128 x 128, that take less time for these products, all of them together.
@@ -87,8 +87,6 @@ __device__ __forceinline__ void store32(void* p, uint32_t const (&v)[8])
 // The exponent that brings the magnitude m into [2^14, 2^15); at most 116, so that 2^e and its inverse are normal numbers.
 __device__ __forceinline__ int pair_exp(float m) { return m > 0.f ? min(141 - (int)(__float_as_uint(m) >> 23), 116) : 0; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }        // -126 <= e <= 127
-
-__device__ __forceinline__ int exp_of(PairExp const& e) { return e.largest ? pair_exp(__uint_as_float(__ldg(e.largest))) : e.value; }
 
 // hi and lo of a value that has been multiplied by 2^e.  An infinity or a not-a-number is all hi.
 __device__ __forceinline__ void pair_of(float v, __half& hi, __half& lo)

@@ -275,7 +275,8 @@ def test_larger_tiles_and_long_rows(gpu, n, d, k):
 
 @pytest.mark.gpu
 def test_an_image_or_class_is_as_exact_beside_far_larger_ones(gpu):
-    """Values keep their digits down to 2^-28 of the largest of the tensor: images and classes 2^14 smaller than others, each against itself."""
+    """Values keep their digits down to 2^-28 of the largest of 64 neighbouring images (classes), whatever the others are: images and classes 2^14
+    smaller than every other one, each against itself, and one image in each of some blocks of 64 whose values make all others vanish beside it."""
     nn, mat, _ = gpu
     n, d, k = 200, 136, 300
     x, f, b, c = _inputs(n, (1, 1, d), k, 15)
@@ -300,6 +301,18 @@ def test_an_image_or_class_is_as_exact_beside_far_larger_ones(gpu):
     for i in range(k):
         assert _rel(got[i], df[i]) <= TOL
     assert _rel(_down(gx), dx) <= TOL and _rel(gb.cpu().numpy(), db) <= TOL
+    # images 0 and 130 are 2^60 times as large: what the blocks of 64 without them hold keeps its digits
+    x, f, b, c = _inputs(n, (1, 1, d), k, 18)
+    c[c == 0] = 1
+    huge = [0, 130]
+    x[huge] *= np.float32(2.0 ** 60)
+    xd, fd, bd, cd = _up(mat, x, f, b, c, (1, 1, d))
+    _, lse, dx, _, _ = _oracle(x, f, b, c)
+    gl, gs = nn.vl_nnfcsoftmaxloss(xd, fd, bd, cd)
+    gx, _, _ = nn.vl_nnfcsoftmaxloss(xd, fd, bd, cd, 1.0, lse=gs)
+    got, sums = _down(gx), gs.cpu().numpy()
+    for i in list(range(64, 128)) + list(range(192, n)):
+        assert abs(sums[i] - lse[i]) <= TOL_LSE * 10 and _rel(got[i], dx[i]) <= TOL
 
 
 @pytest.mark.gpu
