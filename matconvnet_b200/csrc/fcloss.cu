@@ -491,7 +491,7 @@ few_predict_kernel(FewArgs a)
 constexpr int kFewThreads = 128;
 
 template <int kImages, bool kWide>
-__global__ void __launch_bounds__(kFewThreads)
+__global__ void __launch_bounds__(kFewThreads, kImages <= 4 ? 8 : 2)
 few_derivatives_kernel(float* __restrict__ dF, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ f, float const* __restrict__ dz,
                        float const* __restrict__ labels, int N, int D, int K, int perBlock)
 {
@@ -504,30 +504,50 @@ few_derivatives_kernel(float* __restrict__ dF, float* __restrict__ parts, float 
     if (n < N && label_of(labels, n, K, nullptr).real)
 #pragma unroll
       for (int i = 0; i < 4; ++i) if (col(i) < D) xv[n][i] = __ldg(x + (size_t)n * D + col(i));
-#pragma unroll 4
-  for (int k = k0; k < k1; ++k) {
-    float w[4] = {}, o[4] = {}, g[kImages];
-    if (parts) {
-      if (kWide) {
-        float4 const q = col(0) < D ? __ldg((float4 const*)(f + (size_t)k * D + col(0))) : make_float4(0, 0, 0, 0);
-        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
-      } else {
+  // rows of F are asked for kAhead classes before they are used
+  constexpr int kAhead = 4;
+  float w[kAhead][4] = {};
+  auto fetch = [&](float (&v)[4], int k) {
+    if (!parts || k >= k1) return;
+    float const* const p = f + (size_t)k * D;
+    if (kWide) {
+      float4 const q = col(0) < D ? __ldg((float4 const*)(p + col(0))) : make_float4(0, 0, 0, 0);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = col(i) < D ? __ldg(f + (size_t)k * D + col(i)) : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) v[i] = col(i) < D ? __ldg(p + col(i)) : 0.f;
     }
+  };
 #pragma unroll
-    for (int n = 0; n < kImages; ++n) g[n] = __ldg(dz + (size_t)k * kImages + n);
+  for (int u = 0; u < kAhead; ++u) fetch(w[u], k0 + u);
+  for (int kb = k0; kb < k1; kb += kAhead) {
 #pragma unroll
-    for (int n = 0; n < kImages; ++n)
+    for (int u = 0; u < kAhead; ++u) {
+      int const k = kb + u;
+      if (k >= k1) break;
+      float o[4] = {}, g[kImages];
+      if (kImages >= 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { acc[n][i] = fmaf(g[n], w[i], acc[n][i]); o[i] = fmaf(g[n], xv[n][i], o[i]); }
-    if (dF) {
-      if (kWide) {
-        if (col(0) < D) *(float4*)(dF + (size_t)k * D + col(0)) = make_float4(o[0], o[1], o[2], o[3]);
+        for (int n = 0; n < kImages / 4; ++n) {
+          float4 const q = __ldg((float4 const*)(dz + (size_t)k * kImages) + n);
+          g[4 * n % kImages] = q.x; g[(4 * n + 1) % kImages] = q.y; g[(4 * n + 2) % kImages] = q.z; g[(4 * n + 3) % kImages] = q.w;
+        }
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) if (col(i) < D) dF[(size_t)k * D + col(i)] = o[i];
+        for (int n = 0; n < kImages; ++n) g[n] = __ldg(dz + (size_t)k * kImages + n);
+      }
+#pragma unroll
+      for (int n = 0; n < kImages; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { acc[n][i] = fmaf(g[n], w[u][i], acc[n][i]); o[i] = fmaf(g[n], xv[n][i], o[i]); }
+      fetch(w[u], k + kAhead);
+      if (dF) {
+        if (kWide) {
+          if (col(0) < D) *(float4*)(dF + (size_t)k * D + col(0)) = make_float4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) if (col(i) < D) dF[(size_t)k * D + col(i)] = o[i];
+        }
       }
     }
   }
@@ -540,21 +560,21 @@ few_derivatives_kernel(float* __restrict__ dF, float* __restrict__ parts, float 
 }
 
 // dX = the sum of the blocks' parts, in order: 32 elements to a block.
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(1024)
 few_sum_kernel(float* __restrict__ dX, float const* __restrict__ parts, int count, int n)
 {
   vlb::pdl_wait();
-  __shared__ float all[16][33];
+  __shared__ float all[32][33];
   int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, at = (int)blockIdx.x * 32 + tx;
   float s = 0.f;
   if (at < n) {
 #pragma unroll 4
-    for (int i = ty; i < count; i += 16) s += __ldg(parts + (size_t)i * n + at);
+    for (int i = ty; i < count; i += 32) s += __ldg(parts + (size_t)i * n + at);
   }
   all[ty][tx] = s;
   __syncthreads();
   if (ty) return;
-  for (int i = 1; i < 16; ++i) s += all[i][tx];
+  for (int i = 1; i < 32; ++i) s += all[i][tx];
   if (at < n) dX[at] = s;
 }
 
@@ -625,7 +645,10 @@ int forward_few(Problem const& q, float* loss, float* lse)
 
 int backward_few(Problem const& q, float* dX, float* dF, float* db, float const* lse, float scale)
 {
-  int const columns = vlb::ceil_div(q.D, 4 * kFewThreads), chunks = std::min(q.K, std::max(1, 4 * q.ctx->smCount / columns)), per = vlb::ceil_div(q.K, chunks);
+  // eight blocks per SM, as far as the parts of dX stay within 16 MB (81631 x 242, three images: 116 us with four per SM, 81 with eight and rows asked for ahead)
+  int const columns = vlb::ceil_div(q.D, 4 * kFewThreads);
+  int const most = dX ? (int)std::max<long long>(q.ctx->smCount, (4 << 20) / ((long long)q.N * q.D)) : INT32_MAX;
+  int const chunks = std::min(std::min(q.K, most), std::max(1, 8 * q.ctx->smCount / columns)), per = vlb::ceil_div(q.K, chunks);
   int const count = vlb::ceil_div(q.K, per);
   size_t const seen = (few_scratch(q) + 255) / 256 * 256, dzBytes = (sizeof(float) * (size_t)q.K * kFew + 255) / 256 * 256;
   char* const scratch = (char*)vlb::workspace(q.ctx, seen + 256 + dzBytes + (dX ? sizeof(float) * (size_t)count * q.N * q.D : 0));
@@ -646,7 +669,7 @@ int backward_few(Problem const& q, float* dX, float* dF, float* db, float const*
       VLB_LAUNCHED(q.ctx, 1);
     });
   if (dX) {
-    vlb::launch(q.ctx->stream, few_sum_kernel, (unsigned)vlb::ceil_div((long long)q.N * q.D, 32), 512, 0, dX, parts, count, q.N * q.D);
+    vlb::launch(q.ctx->stream, few_sum_kernel, (unsigned)vlb::ceil_div((long long)q.N * q.D, 32), 1024, 0, dX, parts, count, q.N * q.D);
     VLB_LAUNCHED(q.ctx, 1);
   }
   return vlb::check_launch(q.ctx, "vlb_fc_softmaxloss_backward");
