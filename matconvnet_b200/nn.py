@@ -246,7 +246,13 @@ def _muon_update_many(updates, grad_mult, opts, ctx):
             raise ValueError("parameter and gradient must have the same shape.")
     if int(o["steps"]) < 0 or not o["epsilon"] >= 0:
         raise ValueError("steps and epsilon must not be negative.")
-    items = [(w, state["s1"] if "s1" in state else torch.zeros_like(w), g, decay, lr) for w, state, g, decay, lr in updates]
+    fresh = {}                                # a state that is new and named twice is one momentum tensor
+    items = []
+    for w, state, g, decay, lr in updates:
+        s1 = state["s1"] if "s1" in state else fresh.setdefault(id(state), torch.zeros_like(w))
+        if s1.shape != w.shape:
+            raise ValueError("parameter and momentum must be column-major tensors of one shape.")
+        items.append((w, s1, g, decay, lr))
     _hostpath.muon(ctx or default_context(), items, grad_mult,
                    (o["momentum"], o["epsilon"], o["a"], o["b"], o["c"], bool(o["nesterov"]), int(o["steps"])))
     for (_, state, _, _, _), item in zip(updates, items):

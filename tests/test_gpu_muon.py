@@ -205,6 +205,22 @@ def test_weights_that_two_items_share_take_both_steps(gpu):
 
 
 @pytest.mark.gpu
+def test_a_new_state_that_two_items_share_takes_both_steps(gpu):
+    nn = gpu[0]
+    shape = (1, 1, 40, 30)
+    w0, _, g = _inputs(shape, 4)
+    g2 = _inputs(shape, 5)[2]
+    w, state, v, one = _up(w0, shape), {}, _up(w0, shape), {}
+    nn.solver_update_many_("muon", [(w, state, _up(g, shape), 0.1, 0.1), (w, state, _up(g2, shape), 0.1, 0.1)], 1.0, OPTS)
+    for d in (g, g2):
+        nn.solver_update_("muon", v, one, _up(d, shape), 1.0, 0.1, 0.1, OPTS)
+    assert state["t"] == 2 and (_down(w) == _down(v)).all() and (_down(state["s1"]) == _down(one["s1"])).all()
+    with pytest.raises(ValueError):
+        other = {}
+        nn.solver_update_many_("muon", [(w, other, _up(g, shape), 0.1, 0.1), (w.reshape(1, 1, 30, 40), other, _up(g, shape).reshape(1, 1, 30, 40), 0.1, 0.1)], 1.0, OPTS)
+
+
+@pytest.mark.gpu
 def test_in_a_graph_and_from_an_empty_state(gpu):
     import torch
     nn = gpu[0]
