@@ -40,8 +40,8 @@ enum {
                                cores rounded to TF32's 11 bits, about 5e-4 relative error -- strided, dilated and grouped layers
                                and all their gradients included.  Exact products as in the other modes: the direct kernels of a
                                network's image end (at most 64 inputs per output pixel forward, 27 for the filter gradient,
-                               4 input channels for the data gradient), fully connected forward passes of up to 8 images, and
-                               what FP32 below lists */
+                               4 input channels for the data gradient), fully connected forward passes of up to 8 images,
+                               vlb_fc_softmaxloss_* of up to 16 images, and what FP32 below lists */
   VLB_PRECISION_FP32 = 2    /* CUDA-core FMA implicit GEMM: exact fp32 products, slow; in every mode also the path for filter
                                groups of fewer than four channels, strided filters of more than 128 taps, more than 16
                                residue classes of a strided data gradient and reductions of more than 65535 x 32 */
@@ -54,6 +54,13 @@ enum {
  * Such errors show only where the largest values meet zeros or cancel.  Nothing is shared beyond the 64: a filter, channel, image or pixel that is small
  * beside others, by up to 2^100, is as exact as among its like.  Single values below about 2^-102 in magnitude lose digits as they near the subnormal
  * range.  An infinity or a not-a-number reaches the sums that it is part of and no others. */
+
+/* vlb_fc_softmaxloss_* of more than 16 images hold X, F and the derivative of the predictions as such halves.  64 images of X share a power of two, and 64
+ * classes of F: what is down to 2^-28 of the largest of them keeps 22 bits, smaller values are off by at most 2^-50 of it, and nothing is shared beyond
+ * them.  The derivative of the predictions before its factor dzdy / N, at most 1 in magnitude, keeps 22 bits down to 2^-28 and is off by at most 2^-50
+ * below.  An infinity or a not-a-number among the 64 reaches the sums that it is part of and no others.  vlb_muon_update_many does the same with the
+ * matrices of its steps, measured against the largest value that their elements can have.  VLB_PRECISION_TF32 keeps 11 bits; VLB_PRECISION_FP32 takes
+ * products on CUDA cores. */
 
 /* ---- context: replaces vl::Context (bits/data.hpp:150-179) and the stream part of
  *      vl::CudaHelper (bits/datacu.hpp:60-158; setStream bits/datacu.cu:70-93) ---- */
