@@ -517,8 +517,11 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         int const slot = (p.slot0 + t.tile) * kCtas + (int)rank;
         float4* const all = (float4*)batch.split + (p.part0 * kCtas + (long long)(t.tile * kCtas + (int)rank) * p.splits) * (kCols / 4) * 256 + threadIdx.x;
         float4* const mine = all + (long long)t.split * (kCols / 4) * 256;
+        bool const any = row0 < p.M && col0 < p.N;            // rows and columns behind the matrix need no sums
+        if (any) {
 #pragma unroll
-        for (int i = 0; i < kCols / 4; ++i) mine[i * 256] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+          for (int i = 0; i < kCols / 4; ++i) mine[i * 256] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+        }
         __threadfence();
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (threadIdx.x == 0) ticket = atomicAdd(batch.tickets + slot, 1);
@@ -527,7 +530,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         __threadfence();
 #pragma unroll
         for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-        for (int s = 0; s < p.splits; ++s) {
+        for (int s = 0; any && s < p.splits; ++s) {
 #pragma unroll
           for (int i = 0; i < kCols / 4; ++i) {
             float4 const v = __ldcg(all + (long long)(s * (kCols / 4) + i) * 256);
