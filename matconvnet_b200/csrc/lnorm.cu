@@ -2,7 +2,7 @@
 //
 // A position's values are read once and held in registers through all passes over them: the mean, then the sum of squared differences from it (backward
 // together with the two sums of the derivative), then the result.  One position per image (tokens; P = 1): a position is a run of C floats and belongs to a warp or
-// a block.  Maps (P > 1): values of a position lie P floats apart, so that 32 neighbouring positions belong to a block, one per lane, and its warps share the
+// a block.  Maps (P > 1): values of a position lie P floats apart, so that neighbouring positions belong to neighbouring lanes, and a block's warps share the
 // channels.  Both count positions through the batch.  What does not fit the registers is read again for each pass, from L2.
 //
 // The sums over positions (dG, dB) are kept per channel by the threads that see it; each block leaves its part, and a second kernel adds the parts in order.
@@ -11,8 +11,8 @@
 
 namespace {
 
-// Blocks of a backward pass, at most: four per SM, and parts of 64 MB.
-int most_parts(vlb_ctx* ctx, int C) { return (int)std::max<long long>(1, std::min<long long>(4 * ctx->smCount, (64ll << 20) / (8ll * C))); }
+// Blocks of a backward pass, at most: eight per SM, and parts of 64 MB.
+int most_parts(vlb_ctx* ctx, int C) { return (int)std::max<long long>(1, std::min<long long>(8 * ctx->smCount, (64ll << 20) / (8ll * C))); }
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -281,32 +281,49 @@ rows_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
 }
 
 // ------------------------------------------------------------------ positions of maps
-// A block of kWarps warps takes 32 positions, kPos neighbouring ones to a lane: 1, or 4 by 16-byte loads where planes and tensors allow it; a warp's lanes then have
-// kPos channels at a time.  28 x 28 x 512 x 64 forward with kPos 1 / 4: 52 / 49 us.  A lane has kValues of the channels in registers (0: read again for every pass).
+// A block takes tiles of kQ neighbouring positions: a thread has kPos neighbouring ones -- 4, by 16-byte accesses, where planes and tensors allow it, or 1 -- of
+// kValues channels in its registers, a warp's lanes kQ / kPos groups of positions of as many channels as fit.Small blocks, several to an SM, and many
+// values to a thread: what waits at one block's sums is covered by the loads of another's, and the sums over channels go over few warps.  28 x 28 x 512 x 64 forward:
+// 36 us, by one block of 16 warps and 32 positions 49; backward 67 and 176 (a block of 32 warps); 64 x 64 x 64 x 64 backward 40, by blocks of 8 warps with 4 channels to
+// a thread 169.  Tiles that come ahead through a ring in shared memory gained nothing over that: 36 / 38 us forward, 67 / 68 backward.
 struct Place { size_t at; bool in; };
 
 __device__ __forceinline__ Place place_of(long long q, long long positions, int P, int C)
 {
   bool const in = q < positions;
-  long long const t = in ? q : positions - 1, n = t / P;
-  return {(size_t)(n * P * C + (t - n * P)), in};
+  unsigned const t = (unsigned)(in ? q : positions - 1), n = t / (unsigned)P;
+  return {(size_t)n * P * C + (t - n * P), in};
 }
 
-template <int kWarps, int kPos>
-struct Maps {
-  static constexpr int kLanes = 32 / kPos;
-  static __device__ __forceinline__ int channel(int i) { return (int)(threadIdx.x >> 5) * kPos + (int)(threadIdx.x & 31) / kLanes + kWarps * kPos * i; }
-  // the first of the lane's positions; those behind the batch's last (all kPos of them) repeat earlier ones
+// A kernel for maps: warps, positions of a tile and of a thread, channels of a thread, blocks that an SM holds.
+template <int W, int Q, int P, int V, int B>
+struct Shape { static constexpr int kWarps = W, kQ = Q, kPos = P, kValues = V, kPerSm = B; };
+
+template <class T>
+struct Strip {
+  static constexpr int kWarps = T::kWarps, kQ = T::kQ, kPos = T::kPos, kValues = T::kValues;
+  static constexpr int kLanes = kQ / kPos, kChannels = 32 / kLanes, kPass = kWarps * kChannels;       // lanes of a channel; channels of a warp's row, of a row of all warps
+  static __device__ __forceinline__ int channel(int i) { return i * kPass + (int)(threadIdx.x >> 5) * kChannels + (int)(threadIdx.x & 31) / kLanes; }
+  // the thread's first position; those behind the batch's last (all kPos of them) repeat earlier ones
   static __device__ __forceinline__ Place place(int tile, long long positions, int P, int C)
   {
-    long long const q = tile * 32ll + (threadIdx.x & 31) % kLanes * kPos;
+    long long const q = (long long)tile * kQ + (threadIdx.x & 31) % kLanes * kPos;
     Place const p = place_of(min(q, positions - kPos), positions, P, C);
     return {p.at, q < positions};
   }
-  static __device__ __forceinline__ void load(float (&v)[kPos], float const* __restrict__ p)
+  static __device__ __forceinline__ void load(float (&v)[kValues][kPos], float const* __restrict__ from, int P, int C)
   {
-    if (kPos == 4) { float4 const q = __ldg((float4 const*)p); v[0] = q.x; v[1 % kPos] = q.y; v[2 % kPos] = q.z; v[3 % kPos] = q.w; }
-    else v[0] = __ldg(p);
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) {
+      bool const in = channel(i) < C;
+      float const* const p = from + (size_t)P * channel(i);
+      if (kPos == 4) {
+        float4 const q = in ? __ldg((float4 const*)p) : make_float4(0, 0, 0, 0);
+        v[i][0] = q.x; v[i][1 % kPos] = q.y; v[i][2 % kPos] = q.z; v[i][3 % kPos] = q.w;
+      } else {
+        v[i][0] = in ? __ldg(p) : 0.f;
+      }
+    }
   }
   static __device__ __forceinline__ void store(float* __restrict__ p, float const (&v)[kPos])
   {
@@ -315,7 +332,7 @@ struct Maps {
   }
   // sums over the block's channels, position by position
   template <int kCount>
-  static __device__ __forceinline__ void totals(float (&v)[kCount][kPos], float (*red)[kWarps][32])
+  static __device__ __forceinline__ void totals(float (&v)[kCount][kPos], float (*red)[kWarps][kQ])
   {
     int const lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane % kLanes * kPos;
 #pragma unroll
@@ -344,78 +361,72 @@ struct Maps {
   }
 };
 
-template <int kWarps, int kPos, int kValues>
-__global__ void __launch_bounds__(kWarps * 32, kWarps > 16 ? 1 : 32 / kWarps)
-maps_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, long long positions, int P, int C,
-                float eps)
+template <class T>
+__global__ void __launch_bounds__(T::kWarps * 32, T::kPerSm)
+maps_fwd_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, long long positions, int tiles,
+                int P, int C, float eps)
 {
-  using M = Maps<kWarps, kPos>;
+  using S = Strip<T>;
+  constexpr int kPos = S::kPos, kValues = S::kValues;
+  __shared__ __align__(16) float red[2][2][S::kWarps][S::kQ];
   vlb::pdl_wait();
-  __shared__ __align__(16) float red[2][1][kWarps][32];
-  Place const at = M::place(blockIdx.x, positions, P, C);
-  float const* const xp = x + at.at;
-  float* const yp = y + at.at;
-  float v[kValues > 0 ? kValues : 1][kPos], s[1][kPos] = {};
-  if (kValues) {
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) {
-#pragma unroll
-      for (int p = 0; p < kPos; ++p) v[i][p] = 0.f;
-      if (M::channel(i) < C) M::load(v[i], xp + (size_t)P * M::channel(i));
-    }
+  float const n = (float)C;
+  int even = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, even ^= 1) {
+    Place const at = S::place(tile, positions, P, C);
+    float v[kValues][kPos], s[1][kPos] = {}, mean[kPos], r[kPos];
+    S::load(v, x + at.at, P, C);
 #pragma unroll
     for (int i = 0; i < kValues; ++i)
 #pragma unroll
       for (int p = 0; p < kPos; ++p) s[0][p] += v[i][p];
-  } else {
-#pragma unroll 8
-    for (int c = M::channel(0); c < C; c += kWarps * kPos) {
-      M::load(v[0], xp + (size_t)P * c);
+    S::totals(s, red[even]);
 #pragma unroll
-      for (int p = 0; p < kPos; ++p) s[0][p] += v[0][p];
-    }
-  }
-  M::totals(s, red[0]);
-  float mean[kPos], r[kPos];
-#pragma unroll
-  for (int p = 0; p < kPos; ++p) { mean[p] = s[0][p] / (float)C; s[0][p] = 0.f; }
-  if (kValues) {
+    for (int p = 0; p < kPos; ++p) { mean[p] = s[0][p] / n; s[0][p] = 0.f; }
 #pragma unroll
     for (int i = 0; i < kValues; ++i)
 #pragma unroll
-      for (int p = 0; p < kPos; ++p) { v[i][p] -= mean[p]; s[0][p] += M::channel(i) < C ? v[i][p] * v[i][p] : 0.f; }
-  } else {
+      for (int p = 0; p < kPos; ++p) { v[i][p] -= mean[p]; s[0][p] += S::channel(i) < C ? v[i][p] * v[i][p] : 0.f; }
+    S::totals(s, red[even] + 1);
+#pragma unroll
+    for (int p = 0; p < kPos; ++p) r[p] = 1.f / sqrtf(s[0][p] / n + eps);
+    float* to = y + at.at + (size_t)P * S::channel(0);
+    if (at.in)
+#pragma unroll
+      for (int i = 0; i < kValues; ++i, to += (size_t)P * S::kPass)
+        if (S::channel(i) < C) {
+          float const gc = __ldg(g + S::channel(i)), bc = __ldg(b + S::channel(i));
+#pragma unroll
+          for (int p = 0; p < kPos; ++p) v[i][p] = fmaf(gc, v[i][p] * r[p], bc);
+          S::store(to, v[i]);
+        }
+  }
+}
+
+// More channels than that: the values are read again for each pass.
+template <int kWarps>
+__global__ void __launch_bounds__(kWarps * 32)
+maps_fwd_long_kernel(float* __restrict__ y, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ b, long long positions, int P, int C,
+                     float eps)
+{
+  using S = Strip<Shape<kWarps, 32, 1, 1, 1>>;
+  __shared__ float red[2][1][kWarps][32];
+  vlb::pdl_wait();
+  int const warp = threadIdx.x >> 5;
+  Place const at = S::place(blockIdx.x, positions, P, C);
+  float const* const xp = x + at.at;
+  float m[1][1] = {}, s[1][1] = {};
 #pragma unroll 8
-    for (int c = M::channel(0); c < C; c += kWarps * kPos) {
-      M::load(v[0], xp + (size_t)P * c);
-#pragma unroll
-      for (int p = 0; p < kPos; ++p) s[0][p] += (v[0][p] - mean[p]) * (v[0][p] - mean[p]);
-    }
-  }
-  M::totals(s, red[1]);
-#pragma unroll
-  for (int p = 0; p < kPos; ++p) r[p] = 1.f / sqrtf(s[0][p] / (float)C + eps);
+  for (int c = warp; c < C; c += kWarps) m[0][0] += __ldg(xp + (size_t)P * c);
+  S::totals(m, red[0]);
+  float const mean = m[0][0] / (float)C;
+#pragma unroll 8
+  for (int c = warp; c < C; c += kWarps) { float const v = __ldg(xp + (size_t)P * c) - mean; s[0][0] += v * v; }
+  S::totals(s, red[1]);
+  float const r = 1.f / sqrtf(s[0][0] / (float)C + eps);
   if (!at.in) return;
-  if (kValues) {
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) {
-      int const c = M::channel(i);
-      if (c >= C) break;
-      float const gc = __ldg(g + c), bc = __ldg(b + c);
-#pragma unroll
-      for (int p = 0; p < kPos; ++p) v[i][p] = fmaf(gc, v[i][p] * r[p], bc);
-      M::store(yp + (size_t)P * c, v[i]);
-    }
-  } else {
-#pragma unroll 4
-    for (int c = M::channel(0); c < C; c += kWarps * kPos) {
-      float const gc = __ldg(g + c), bc = __ldg(b + c);
-      M::load(v[0], xp + (size_t)P * c);
-#pragma unroll
-      for (int p = 0; p < kPos; ++p) v[0][p] = fmaf(gc, (v[0][p] - mean[p]) * r[p], bc);
-      M::store(yp + (size_t)P * c, v[0]);
-    }
-  }
+#pragma unroll 8
+  for (int c = warp; c < C; c += kWarps) y[at.at + (size_t)P * c] = fmaf(__ldg(g + c), (__ldg(xp + (size_t)P * c) - mean) * r, __ldg(b + c));
 }
 
 // Sums over groups of kLanes neighbouring lanes of kCount values, both powers of two: lane l ends with v[0 ...] the totals of the values
@@ -439,85 +450,76 @@ __device__ __forceinline__ void lane_sums(float (&v)[kCount])
   for (int s = kFew; s < kLanes; s <<= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], s);
 }
 
-// Tiles of 32 positions in turn to the blocks.  parts: [block][2][C].
-template <int kWarps, int kPos, int kValues>
-__global__ void __launch_bounds__(kWarps * 32, kWarps == 16 && kPos * kValues < 16 ? 2 : 1)
+// Tiles in turn to the blocks.  parts: [block][2][C].
+template <class T>
+__global__ void __launch_bounds__(T::kWarps * 32, T::kPerSm)
 maps_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
                 long long positions, int tiles, int P, int C, float eps)
 {
-  using M = Maps<kWarps, kPos>;
-  constexpr int kSums = 2 * kValues, kOwn = kSums > M::kLanes ? kSums / M::kLanes : 1;      // dG of the lane's channels, then dB; totals that a lane ends with
+  using S = Strip<T>;
+  constexpr int kPos = S::kPos, kValues = S::kValues, kLanes = S::kLanes;
+  constexpr int kOwn = kValues > kLanes ? kValues / kLanes : 1;              // channels whose sums over positions end with a lane
+  __shared__ __align__(16) float red[2][4][S::kWarps][S::kQ];
   vlb::pdl_wait();
-  __shared__ __align__(16) float red[2][4][kWarps][32];
-  int const lane = threadIdx.x & 31;
   float const n = (float)C;
-  float sum[kOwn] = {};
+  float sumG[kOwn] = {}, sumB[kOwn] = {};
   int even = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, even ^= 1) {
-    Place const at = M::place(tile, positions, P, C);
-    float const *const xp = x + at.at, *const dp = dy + at.at;
-    float v[kValues][kPos], d[kValues][kPos], m[1][kPos] = {};
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) {
-#pragma unroll
-      for (int p = 0; p < kPos; ++p) v[i][p] = 0.f;
-      if (M::channel(i) < C) M::load(v[i], xp + (size_t)P * M::channel(i));
-    }
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) {
-#pragma unroll
-      for (int p = 0; p < kPos; ++p) d[i][p] = 0.f;
-      if (M::channel(i) < C) M::load(d[i], dp + (size_t)P * M::channel(i));
-    }
+    Place const at = S::place(tile, positions, P, C);
+    float v[kValues][kPos], d[kValues][kPos], m[1][kPos] = {}, s[3][kPos] = {};
+    S::load(v, x + at.at, P, C);
+    S::load(d, dy + at.at, P, C);
 #pragma unroll
     for (int i = 0; i < kValues; ++i)
 #pragma unroll
       for (int p = 0; p < kPos; ++p) m[0][p] += v[i][p];
-    M::totals(m, red[even] + 3);
-    float s[3][kPos] = {}, mean[kPos];
+    S::totals(m, red[even] + 3);
 #pragma unroll
-    for (int p = 0; p < kPos; ++p) mean[p] = m[0][p] / n;
+    for (int p = 0; p < kPos; ++p) m[0][p] /= n;
 #pragma unroll
     for (int i = 0; i < kValues; ++i) {
-      float const gc = M::channel(i) < C ? __ldg(g + M::channel(i)) : 0.f;
+      bool const real = S::channel(i) < C;
+      float const gc = real ? __ldg(g + S::channel(i)) : 0.f;
 #pragma unroll
       for (int p = 0; p < kPos; ++p) {
-        v[i][p] = M::channel(i) < C ? v[i][p] - mean[p] : 0.f;
+        v[i][p] = real ? v[i][p] - m[0][p] : 0.f;
         float const gd = gc * d[i][p];
         s[0][p] += v[i][p] * v[i][p]; s[1][p] += gd; s[2][p] += gd * v[i][p];
       }
     }
-    M::totals(s, red[even]);
+    S::totals(s, red[even]);
     float r[kPos], m1[kPos], m2[kPos];
 #pragma unroll
     for (int p = 0; p < kPos; ++p) { r[p] = 1.f / sqrtf(s[0][p] / n + eps); m1[p] = s[1][p] / n; m2[p] = s[2][p] * r[p] / n; }
-    if (parts) {
-      float t[kSums] = {};
+    float* to = dx + at.at + (size_t)P * S::channel(0);
+    float tG[kValues], tB[kValues];
 #pragma unroll
-      for (int i = 0; i < kValues; ++i)
+    for (int i = 0; i < kValues; ++i, to += (size_t)P * S::kPass) {
+      tG[i] = tB[i] = 0.f;
 #pragma unroll
-        for (int p = 0; p < kPos; ++p) { t[i] += at.in ? d[i][p] * (v[i][p] * r[p]) : 0.f; t[kValues + i] += at.in ? d[i][p] : 0.f; }
-      lane_sums<M::kLanes>(t);
+      for (int p = 0; p < kPos; ++p) { v[i][p] *= r[p]; tG[i] += d[i][p] * v[i][p]; tB[i] += d[i][p]; }
+      if (S::channel(i) < C && dx && at.in) {
+        float const gc = __ldg(g + S::channel(i));
+        float o[kPos];
 #pragma unroll
-      for (int k = 0; k < kOwn; ++k) sum[k] += t[k];
-    }
-    if (dx && at.in) {
-#pragma unroll
-      for (int i = 0; i < kValues; ++i) {
-        int const c = M::channel(i);
-        if (c >= C) break;
-        float const gc = __ldg(g + c);
-#pragma unroll
-        for (int p = 0; p < kPos; ++p) v[i][p] = r[p] * (gc * d[i][p] - m1[p] - v[i][p] * r[p] * m2[p]);
-        M::store(dx + at.at + (size_t)P * c, v[i]);
+        for (int p = 0; p < kPos; ++p) o[p] = r[p] * (gc * d[i][p] - m1[p] - v[i][p] * m2[p]);
+        S::store(to, o);
       }
+      if (!at.in) tG[i] = tB[i] = 0.f;
+    }
+    if (parts) {
+      lane_sums<kLanes>(tG);
+      lane_sums<kLanes>(tB);
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) { sumG[k] += tG[k]; sumB[k] += tB[k]; }
     }
   }
-  if (!parts || lane % M::kLanes >= kSums) return;
+  int const lane = threadIdx.x & 31;
+  if (!parts || lane % kLanes >= kValues) return;
 #pragma unroll
   for (int k = 0; k < kOwn; ++k) {
-    int const which = lane % M::kLanes * kOwn + k, c = M::channel(which % kValues);
-    if (c < C) parts[(size_t)blockIdx.x * 2 * C + (which < kValues ? 0 : C) + c] = sum[k];
+    int const c = S::channel(lane % kLanes * kOwn + k);
+    if (c < C) { parts[(size_t)blockIdx.x * 2 * C + c] = sumG[k]; parts[((size_t)blockIdx.x * 2 + 1) * C + c] = sumB[k]; }
   }
 }
 
@@ -528,8 +530,8 @@ maps_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
                      long long positions, int tiles, int P, int C, float eps)
 {
   vlb::pdl_wait();
-  using M = Maps<kWarps, 1>;
-  __shared__ __align__(16) float red[2][4][kWarps][32];
+  using M = Strip<Shape<kWarps, 32, 1, 1, 1>>;
+  __shared__ float red[2][4][kWarps][32];
   int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float const n = (float)C;
   float* const own = parts ? parts + (size_t)blockIdx.x * 2 * C : nullptr;
@@ -571,21 +573,26 @@ maps_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
   }
 }
 
-// dG and dB from the parts of `count` blocks, 32 columns per block, in a fixed order.
+// dG and dB from the parts of `count` blocks, kCols columns per block, in a fixed order.
+template <int kCols>
 __global__ void __launch_bounds__(1024)
 sum_blocks_kernel(float* __restrict__ dg, float* __restrict__ db, float const* __restrict__ parts, int count, int C)
 {
   vlb::pdl_wait();
-  __shared__ float all[32][33];
-  int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + tx;
+  __shared__ float all[32][kCols];
+  int const tx = threadIdx.x % kCols, ty = threadIdx.x / kCols, c = (int)blockIdx.x * kCols + tx;
   float s = 0.f;
   if (c < 2 * C) {
 #pragma unroll 4
-    for (int i = ty; i < count; i += 32) s += __ldg(parts + (size_t)i * 2 * C + c);
+    for (int i = ty; i < count; i += 1024 / kCols) s += __ldg(parts + (size_t)i * 2 * C + c);
   }
-  all[ty][tx] = s;
+#pragma unroll
+  for (int o = kCols; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) < kCols) all[threadIdx.x >> 5][tx] = s;
   __syncthreads();
   if (ty) return;
+  s = all[0][tx];
+#pragma unroll
   for (int i = 1; i < 32; ++i) s += all[i][tx];
   if (c < C) { if (dg) dg[c] = s; }
   else if (c < 2 * C) { if (db) db[c - C] = s; }
@@ -647,22 +654,31 @@ int vlb_lnorm_forward(vlb_ctx* ctx, float* Y, float const* X, float const* g, fl
     done = true;
   }
   if (!done) {
-    unsigned const grid = (unsigned)vlb::ceil_div(positions, 32);
-    auto run = [&](auto kernel, int warps) { vlb::launch(ctx->stream, kernel, grid, warps * 32, 0, Y, X, g, b, (long long)positions, P, C, (float)eps); };
+    auto run = [&](auto shape) {
+      using T = decltype(shape);
+      int const tiles = vlb::ceil_div(positions, T::kQ);
+      vlb::launch(ctx->stream, maps_fwd_kernel<T>, (unsigned)std::min(tiles, ctx->smCount * T::kPerSm), T::kWarps * 32, 0, Y, X, g, b, (long long)positions, tiles, P, C, (float)eps);
+    };
     if (wide(P, {Y, X})) {
-      if (C <= 32)        run(maps_fwd_kernel<8, 4, 1>, 8);
-      else if (C <= 128)  run(maps_fwd_kernel<8, 4, 4>, 8);
-      else if (C <= 256)  run(maps_fwd_kernel<8, 4, 8>, 8);
-      else if (C <= 512)  run(maps_fwd_kernel<16, 4, 8>, 16);
-      else if (C <= 1024) run(maps_fwd_kernel<32, 4, 8>, 32);
-      else                run(maps_fwd_kernel<32, 4, 0>, 32);
+      if (C <= 32)        run(Shape<2, 32, 4, 4, 16>{});
+      else if (C <= 64)   run(Shape<2, 32, 4, 8, 12>{});
+      else if (C <= 128)  run(Shape<4, 32, 4, 8, 8>{});
+      else if (C <= 256)  run(Shape<8, 32, 4, 8, 4>{});
+      else if (C <= 512)  run(Shape<8, 16, 4, 8, 4>{});
+      else if (C <= 1024) run(Shape<8, 16, 4, 16, 2>{});
+      else if (C <= 2048) run(Shape<16, 8, 4, 8, 2>{});
+      else done = true;
     } else {
-      if (C <= 32)        run(maps_fwd_kernel<8, 1, 4>, 8);
-      else if (C <= 128)  run(maps_fwd_kernel<8, 1, 16>, 8);
-      else if (C <= 256)  run(maps_fwd_kernel<16, 1, 16>, 16);
-      else if (C <= 512)  run(maps_fwd_kernel<16, 1, 32>, 16);
-      else                run(maps_fwd_kernel<32, 1, 0>, 32);
+      if (C <= 32)        run(Shape<2, 32, 1, 16, 16>{});
+      else if (C <= 64)   run(Shape<4, 32, 1, 16, 8>{});
+      else if (C <= 128)  run(Shape<4, 32, 1, 32, 6>{});
+      else if (C <= 256)  run(Shape<8, 32, 1, 32, 4>{});
+      else if (C <= 512)  run(Shape<8, 16, 1, 32, 4>{});
+      else if (C <= 1024) run(Shape<16, 16, 1, 32, 2>{});
+      else if (C <= 2048) run(Shape<16, 8, 1, 32, 2>{});
+      else done = true;
     }
+    if (done) vlb::launch(ctx->stream, maps_fwd_long_kernel<32>, (unsigned)vlb::ceil_div(positions, 32), 1024, 0, Y, X, g, b, (long long)positions, P, C, (float)eps);
   }
   VLB_LAUNCHED(ctx, 1);
   return vlb::check_launch(ctx, "vlb_lnorm_forward");
@@ -708,21 +724,40 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
     }
   }
   if (!blocks) {
-    int const tiles = vlb::ceil_div(positions, 32);
-    auto run = [&](auto kernel, int warps) {
-      blocks = std::min(tiles, std::min(most, ctx->smCount * std::max(1, std::min(4, 32 / warps))));
-      vlb::launch(ctx->stream, kernel, (unsigned)blocks, warps * 32, 0, dX, parts, X, g, dY, (long long)positions, tiles, P, C, (float)eps);
+    auto run = [&](auto shape) {
+      using T = decltype(shape);
+      int const tiles = vlb::ceil_div(positions, T::kQ);
+      blocks = std::min(tiles, std::min(most, ctx->smCount * T::kPerSm));
+      vlb::launch(ctx->stream, maps_bwd_kernel<T>, (unsigned)blocks, T::kWarps * 32, 0, dX, parts, X, g, dY, (long long)positions, tiles, P, C, (float)eps);
     };
-    bool const four = wide(P, {dX, X, dY});
-    if (C <= 32)       four ? run(maps_bwd_kernel<8, 4, 1>, 8) : run(maps_bwd_kernel<8, 1, 4>, 8);
-    else if (C <= 128) four ? run(maps_bwd_kernel<8, 4, 4>, 8) : run(maps_bwd_kernel<16, 1, 8>, 16);
-    else if (C <= 256) four ? run(maps_bwd_kernel<16, 4, 4>, 16) : run(maps_bwd_kernel<16, 1, 16>, 16);
-    else if (C <= 512) four ? run(maps_bwd_kernel<32, 4, 4>, 32) : run(maps_bwd_kernel<32, 1, 16>, 32);
-    else               run(maps_bwd_long_kernel<16>, 16);
+    if (wide(P, {dX, X, dY})) {
+      if (C <= 32)        run(Shape<2, 32, 4, 4, 8>{});
+      else if (C <= 64)   run(Shape<2, 32, 4, 8, 8>{});
+      else if (C <= 128)  run(Shape<4, 32, 4, 8, 4>{});
+      else if (C <= 256)  run(Shape<4, 16, 4, 8, 4>{});
+      else if (C <= 512)  run(Shape<4, 8, 4, 8, 4>{});
+      else if (C <= 1024) run(Shape<4, 8, 4, 16, 2>{});
+      else if (C <= 2048) run(Shape<16, 8, 4, 8, 1>{});
+    } else {
+      if (C <= 32)        run(Shape<2, 32, 1, 16, 8>{});
+      else if (C <= 64)   run(Shape<4, 32, 1, 16, 6>{});
+      else if (C <= 128)  run(Shape<4, 32, 1, 32, 4>{});
+      else if (C <= 256)  run(Shape<8, 32, 1, 32, 2>{});
+      else if (C <= 512)  run(Shape<8, 16, 1, 32, 2>{});
+      else if (C <= 1024) run(Shape<8, 8, 1, 32, 2>{});
+      else if (C <= 2048) run(Shape<16, 8, 1, 32, 1>{});
+    }
+    if (C > 2048) {
+      int const tiles = vlb::ceil_div(positions, 32);
+      blocks = std::min(tiles, std::min(most, ctx->smCount * 2));
+      vlb::launch(ctx->stream, maps_bwd_long_kernel<16>, (unsigned)blocks, 512, 0, dX, parts, X, g, dY, (long long)positions, tiles, P, C, (float)eps);
+    }
   }
   VLB_LAUNCHED(ctx, 1);
   if (parts) {
-    vlb::launch(ctx->stream, sum_blocks_kernel, (unsigned)vlb::ceil_div(2ll * C, 32), 1024, 0, dG, dB, parts, blocks, C);
+    // columns of a block: few, where 32 would leave most of the device idle
+    if (2ll * C >= 32ll * ctx->smCount) vlb::launch(ctx->stream, sum_blocks_kernel<32>, (unsigned)vlb::ceil_div(2ll * C, 32), 1024, 0, dG, dB, parts, blocks, C);
+    else                                vlb::launch(ctx->stream, sum_blocks_kernel<8>, (unsigned)vlb::ceil_div(2ll * C, 8), 1024, 0, dG, dB, parts, blocks, C);
     VLB_LAUNCHED(ctx, 1);
   }
   return vlb::check_launch(ctx, "vlb_lnorm_backward");
