@@ -78,10 +78,14 @@ __device__ __forceinline__ Item item_of(Batch<kMax> const& b, int w)
   while (kMax > 1 && w >= b.p[t.prod].work) ++t.prod;
   Product const& p = b.p[t.prod];
   if (t.prod) w -= b.p[t.prod - 1].work;
-  t.tile = w / p.splits;
-  t.split = w - t.tile * p.splits;
-  t.kb0 = (int)((long long)p.kBlocks * t.split / p.splits);
-  t.kb1 = (int)((long long)p.kBlocks * (t.split + 1) / p.splits);
+  t.tile = w; t.split = 0;
+  t.kb0 = 0; t.kb1 = p.kBlocks;
+  if (p.splits > 1) {                                   // (at most 64, of at most 2^25 k-blocks)
+    t.tile = w / p.splits;
+    t.split = w - t.tile * p.splits;
+    t.kb0 = (int)((unsigned)p.kBlocks * (unsigned)t.split / (unsigned)p.splits);
+    t.kb1 = (int)((unsigned)p.kBlocks * (unsigned)(t.split + 1) / (unsigned)p.splits);
+  }
   if (p.symmetric) {
     int i = (int)((sqrtf(8.f * t.tile + 1.f) - 1.f) * 0.5f);
     while (i * (i + 1) / 2 > t.tile) --i;
