@@ -77,6 +77,35 @@ def test_forward_and_backward(gpu, shape):
     _close(mat.to_numpy(db), rb, scale=max(np.abs(rb).max(), np.sqrt(positions)))
 
 
+# a shape of every kernel for maps, with and without 16-byte accesses, and more tiles than blocks run at one time
+MAPS = [(2, 2, 24, 9), (3, 7, 30, 11), (4, 4, 60, 7), (3, 1, 64, 50), (8, 2, 128, 3), (4, 1, 256, 11), (6, 2, 512, 5), (8, 4, 1000, 30), (4, 2, 1500, 5), (3, 3, 2048, 6),
+        (4, 3, 2049, 3), (16, 16, 40, 700), (13, 11, 120, 220), (8, 8, 300, 200), (9, 7, 300, 200), (8, 8, 700, 80)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MAPS)
+def test_maps_of_every_kind(gpu, shape):
+    test_forward_and_backward(gpu, shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 4, 200, 9), (7, 3, 200, 9), (1, 1, 300, 40)])
+def test_the_derivative_of_the_data_or_of_the_parameters_alone(gpu, shape):
+    import ctypes
+    import torch
+    nn, mat, ctx = gpu
+    x, g, b, dy = _inputs(shape, 2)
+    xd, gd, bd, dyd = (mat.from_numpy(a) for a in (x, g, b, dy))
+    want = nn.vl_nnlayernorm(xd, gd, bd, dyd)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())                                        # noqa: E731
+    ctx.check(ctx.lib.vlb_ctx_set_stream(ctx.handle, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    for asked in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 0, 1)):
+        got = [mat.from_numpy(np.asfortranarray(np.full(tuple(t.shape), 7, np.float32))) for t in want]
+        ctx.check(ctx.lib.vlb_lnorm_backward(ctx.handle, *(ptr(t) if a else None for t, a in zip(got, asked)), ptr(xd), ptr(gd), ptr(dyd), *shape, 1e-5))
+        for t, full, a in zip(got, want, asked):
+            assert (t == full).all() if a else (t == 7).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(1, 1, 513, 9), (5, 3, 40, 4)])
 def test_values_far_from_zero_and_outputs_asked_for(gpu, shape):
