@@ -482,6 +482,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
       Item const t = item_of(batch, w);
       Product const& p = batch.p[t.prod];
       int const row0 = t.tm * kTileRows + (int)rank * 128 + quarter * 32, col0 = t.tn * kTileCols + half * kCols;
+      bool const any = row0 < p.M && col0 < p.N;            // rows and columns behind the matrix need no sums
       Ahead const ahead = fetch_ahead<kKind, kCols>(p, row0 + lane, col0, patch);
       float acc[kCols];
 #pragma unroll
@@ -497,16 +498,18 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         tc_fence_after();
         int const buf = j % kAcc;
         uint32_t const at = lanes + (uint32_t)(buf * kTileCols);
-        uint32_t r[2][16];
-        tmem_ld16_issue(at, r[0]);
+        if (any) {
+          uint32_t r[2][16];
+          tmem_ld16_issue(at, r[0]);
 #pragma unroll
-        for (int g = 0; g < kCols / 16; ++g) {
-          tmem_ld_wait();
-          if (g + 1 < kCols / 16) tmem_ld16_issue(at + 16u * (g + 1), r[(g + 1) & 1]);
+          for (int g = 0; g < kCols / 16; ++g) {
+            tmem_ld_wait();
+            if (g + 1 < kCols / 16) tmem_ld16_issue(at + 16u * (g + 1), r[(g + 1) & 1]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float const v = __uint_as_float(r[g & 1][i]);
-            acc[g * 16 + i] = kKind == kPairOut ? fmaf(v, f, acc[g * 16 + i]) : acc[g * 16 + i] + v;
+            for (int i = 0; i < 16; ++i) {
+              float const v = __uint_as_float(r[g & 1][i]);
+              acc[g * 16 + i] = kKind == kPairOut ? fmaf(v, f, acc[g * 16 + i]) : acc[g * 16 + i] + v;
+            }
           }
         }
         tc_fence_before();
@@ -521,7 +524,6 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         int const slot = (p.slot0 + t.tile) * kCtas + (int)rank;
         float4* const all = (float4*)batch.split + (p.part0 * kCtas + (long long)(t.tile * kCtas + (int)rank) * p.splits) * (kCols / 4) * 256 + threadIdx.x;
         float4* const mine = all + (long long)t.split * (kCols / 4) * 256;
-        bool const any = row0 < p.M && col0 < p.N;            // rows and columns behind the matrix need no sums
         if (any) {
 #pragma unroll
           for (int i = 0; i < kCols / 4; ++i) mine[i * 256] = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
@@ -543,6 +545,7 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
         }
         if (threadIdx.x == 0) batch.tickets[slot] = 0;
       }
+      if (row0 >= p.M || (!any && kKind != kPairSeen)) continue;       // (half a tile's columns have a part, if an empty one)
       if (kKind == kPairOut)  finish_out(p, ahead, acc, row0, col0, patch);
       if (kKind == kPairSeen) finish_seen(p, ahead, acc, row0 + lane, col0, patch);
       if (kKind == kPairGrad) finish_grad(p, ahead, acc, row0, row0 + lane, col0, patch);
