@@ -123,6 +123,21 @@ __device__ __forceinline__ Part together(Part a, Part b)
   return {top, a.sum * expf(a.top - base) + b.sum * expf(b.top - base)};
 }
 
+// kCount parts into one, so that their exponentials do not wait for one another; part(i) is the i-th.
+template <int kCount, class F>
+__device__ __forceinline__ Part joined(Part p, F part)
+{
+  Part q[kCount];
+  float top = p.top;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) { q[i] = part(i); top = fmaxf(top, q[i].top); }
+  float const base = isinf(top) ? 0.f : top;
+  float sum = p.sum * expf(p.top - base);
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) sum += q[i].sum * expf(q[i].top - base);
+  return {top, sum};
+}
+
 // lse of 32 images per block from the parts of their predictions, and the loss by the block that is through last, which adds the blocks' sums in their order.
 // lse and labels: of the images first ... first + rows - 1; sums: one per block of 32 images of all `blocks`.
 __global__ void __launch_bounds__(1024)
@@ -134,15 +149,16 @@ lse_kernel(float* __restrict__ loss, float* __restrict__ lse, float2 const* __re
   int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, row = (int)blockIdx.x * 32 + tx;
   Part p = {-INFINITY, 0.f};
   if (row < rows)
-#pragma unroll 4
-    for (int i = ty; i < count; i += 32) {
-      float2 const v = parts[(long long)i * rows + row];
-      p = together(p, {v.x, v.y});
-    }
+    for (int i0 = ty; i0 < count; i0 += 32 * 8)
+      p = joined<8>(p, [&](int k) {
+        int const i = i0 + 32 * k;
+        float2 const v = i < count ? __ldg(parts + (long long)i * rows + row) : make_float2(-INFINITY, 0.f);
+        return Part{v.x, v.y};
+      });
   all[ty][tx] = p;
   __syncthreads();
   if (ty) return;
-  for (int i = 1; i < 32; ++i) p = together(p, all[i][tx]);
+  p = joined<31>(p, [&](int i) { return all[i + 1][tx]; });
   double term = 0;
   if (row < rows) {
     Label const l = label_of(labels, row, K, status);
@@ -166,15 +182,23 @@ lse_kernel(float* __restrict__ loss, float* __restrict__ lse, float2 const* __re
   if (tx == 0) { *loss = (float)(sum / N); *ticket = 0; }
 }
 
-// db[c] (+)= scale * sum of the rows of parts.
-__global__ void db_parts_kernel(float* __restrict__ db, float const* __restrict__ parts, long long ld, int cols, int rows, float scale, bool add)
+// db[c] (+)= scale * sum of the rows of parts: 32 columns to a block, its warps the rows in turn.
+__global__ void __launch_bounds__(kThreads)
+db_parts_kernel(float* __restrict__ db, float const* __restrict__ parts, long long ld, int cols, int rows, float scale, bool add)
 {
   vlb::pdl_wait();
-  int const c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= cols) return;
+  __shared__ float all[kThreads / 32][33];
+  int const tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + tx;
   float s = 0.f;
+  if (c < cols) {
 #pragma unroll 8
-  for (int r = 0; r < rows; ++r) s += parts[r * ld + c];
+    for (int r = ty; r < rows; r += kThreads / 32) s += __ldg(parts + r * ld + c);
+  }
+  all[ty][tx] = s;
+  __syncthreads();
+  if (ty || c >= cols) return;
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) s += all[i][tx];
   db[c] = add ? db[c] + s * scale : s * scale;
 }
 
@@ -306,7 +330,7 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
       p.e.status = q.ctx->deviceStatus;
       if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairGrad, &p, 1, plan.split, vlb::pair_tile(q.ctx, &p, 1))) return rc;
       if (db) {
-        vlb::launch(q.ctx->stream, db_parts_kernel, (unsigned)vlb::ceil_div(cols, kThreads), kThreads, 0, db + k0, plan.db, dz.ld, cols,
+        vlb::launch(q.ctx->stream, db_parts_kernel, (unsigned)vlb::ceil_div(cols, 32), kThreads, 0, db + k0, plan.db, dz.ld, cols,
                     vlb::ceil_div(x.rows, 32), scale, n0 > 0);
         VLB_LAUNCHED(q.ctx, 1);
       }
