@@ -5,7 +5,6 @@
 
 namespace {
 
-
 constexpr int kThreads = 256;
 
 // What the pieces so far have shown of an image's predictions: the largest, the sum of exp(z - largest), the label's.
@@ -702,6 +701,13 @@ int backward_few(Problem const& q, float* dX, float* dF, float* db, float const*
 // Classes per piece: predictions of a piece up to 64 MB.
 int piece_of(int N, int K) { return (int)std::min<long long>(K, std::max<long long>(64, (16ll << 20) / N / 64 * 64)); }
 
+// Images, classes and features are walked through with 32-bit counters, in strides of up to kStride.
+bool good_shape(int H, int W, int C, int N, int K)
+{
+  constexpr int kStride = 1 << 20;
+  return H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W <= INT32_MAX && (long long)H * W * C <= INT32_MAX - kStride && N <= INT32_MAX - kStride && K <= INT32_MAX - kStride;
+}
+
 }  // namespace
 
 extern "C" {
@@ -710,7 +716,7 @@ int vlb_fc_softmaxloss_forward(vlb_ctx* ctx, float* loss, float* lse, float cons
                                int H, int W, int C, int N, int K)
 {
   if (!ctx) return VLB_IllegalArgument;
-  VLB_REQUIRE(ctx, H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W * C <= INT32_MAX, "fc_softmaxloss_forward: bad shape");
+  VLB_REQUIRE(ctx, good_shape(H, W, C, N, K), "fc_softmaxloss_forward: bad shape");
   VLB_REQUIRE(ctx, loss && X && F && labels, "fc_softmaxloss_forward: null tensor");
   int const D = H * W * C;
   if (few_images(N, D)) return vlb::pass_error(ctx, forward_few({ctx, X, F, b, labels, N, D, K}, loss, lse), "vlb_fc_softmaxloss_forward");
@@ -736,7 +742,7 @@ int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, f
                                 float const* labels, float const* lse, double dzdy, int H, int W, int C, int N, int K)
 {
   if (!ctx) return VLB_IllegalArgument;
-  VLB_REQUIRE(ctx, H > 0 && W > 0 && C > 0 && N > 0 && K > 0 && (long long)H * W * C <= INT32_MAX, "fc_softmaxloss_backward: bad shape");
+  VLB_REQUIRE(ctx, good_shape(H, W, C, N, K), "fc_softmaxloss_backward: bad shape");
   VLB_REQUIRE(ctx, X && F && labels, "fc_softmaxloss_backward: null tensor");
   int const D = H * W * C;
   if (few_images(N, D))

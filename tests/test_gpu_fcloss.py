@@ -397,3 +397,14 @@ def test_refusals(gpu):
         nn.vl_nnfcsoftmaxloss(x[:, :, :, :0], f, b, c[:0])
     with pytest.raises(RuntimeError, match="bad shape"):
         nn.vl_nnfcsoftmaxloss(x, f[:, :, :, :0], None, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hwc,n,k", [((1, 1, 1), 3, 2**31 - 1), ((1, 1, 1), 2**31 - 1, 3), ((1, 1, 2**31 - 1), 3, 3), ((2**16, 2**16, 2), 3, 3), ((2**16, 2**15, 2**16), 3, 3)])
+def test_sizes_that_counters_do_not_hold_are_refused(gpu, hwc, n, k):
+    ctx = gpu[2]
+    # refused before anything is looked at
+    some = 256
+    assert ctx.lib.vlb_fc_softmaxloss_forward(ctx.handle, some, None, some, some, None, some, *hwc, n, k) == 7
+    assert ctx.lib.vlb_fc_softmaxloss_backward(ctx.handle, None, None, None, some, some, None, some, None, 1.0, *hwc, n, k) == 7
+    ctx.lib.vlb_ctx_reset_error(ctx.handle)
