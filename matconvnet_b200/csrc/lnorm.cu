@@ -598,7 +598,9 @@ sum_blocks_kernel(float* __restrict__ dg, float* __restrict__ db, float const* _
   else if (c < 2 * C) { if (db) db[c - C] = s; }
 }
 
-bool bad_shape(int H, int W, int C, int N) { return H <= 0 || W <= 0 || C <= 0 || N <= 0 || (long long)H * W * N > INT32_MAX - 64; }
+// Positions, and channels twice over, are walked through with 32-bit counters.
+bool bad_shape(int H, int W, int C, int N)
+{ return H <= 0 || W <= 0 || C <= 0 || N <= 0 || (long long)H * W > INT32_MAX || (long long)H * W * N > INT32_MAX - (1 << 20) || C > (1 << 30) - (1 << 20); }
 
 bool wide(int C, std::initializer_list<void const*> ps)
 {

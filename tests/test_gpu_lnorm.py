@@ -219,3 +219,13 @@ def test_refusals(gpu):
         nn.vl_nnlayernorm(x, g, b, epsilon=float("nan"))
     with pytest.raises(RuntimeError, match="bad shape"):
         nn.vl_nnlayernorm(x[:, :, :, :0], g, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 1, 2**31 - 1, 1), (1, 1, 2**30, 1), (1, 1, 1, 2**31 - 1), (2**16, 2**15, 4, 1), (2**31 - 1, 2**31 - 1, 4, 4), (2**16, 2**16, 4, 2**31 - 1)])
+def test_sizes_that_counters_do_not_hold_are_refused(gpu, shape):
+    ctx = gpu[2]
+    some = 256                               # refused before anything is looked at
+    assert ctx.lib.vlb_lnorm_forward(ctx.handle, some, some, some, some, *shape, 1e-5) == 7
+    assert ctx.lib.vlb_lnorm_backward(ctx.handle, some, None, None, some, some, some, *shape, 1e-5) == 7
+    ctx.lib.vlb_ctx_reset_error(ctx.handle)
