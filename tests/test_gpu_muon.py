@@ -265,3 +265,15 @@ def test_refusals(gpu):
     assert (w == before).all() and state["t"] == 1
     nn.solver_update_many_("muon", [], 1.0)
     assert torch.cuda.is_available()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(2**31 - 1, 1), (1, 2**31 - 1)])
+def test_sizes_that_counters_do_not_hold_are_refused(gpu, rows, cols):
+    import ctypes
+    from matconvnet_b200 import capi
+    ctx = gpu[2]
+    u = capi.MuonParam(256, 256, 256, rows, cols, 0.0, 0.1)              # refused before anything is looked at
+    o = capi.MuonOpts(0.95, 1e-7, 3.4445, -4.7750, 2.0315, 1, 5)
+    assert ctx.lib.vlb_muon_update_many(ctx.handle, 1, ctypes.byref(u), 1.0, ctypes.byref(o)) == 7
+    ctx.lib.vlb_ctx_reset_error(ctx.handle)
