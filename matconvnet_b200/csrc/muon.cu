@@ -20,7 +20,7 @@ struct Job {
   double* parts;                     // sums of squares, one per block of momentum_kernel
   int partCount, block0, blocks, vec;
   vlb::Pair x;
-  int rowsPer; vlb::FastDiv perRow;  // make_x_kernel: rows of a block, sixteen columns at a time
+  int rowsPer; vlb::FastDiv31 perRow;  // make_x_kernel: rows of a block, sixteen columns at a time (by groups of columns, of which there are up to 2^27)
 };
 struct Jobs { Job j[kMost]; int count; };
 
@@ -247,7 +247,7 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
     j.x = x[0][i];
     int const groups = (int)(j.x.ld / 16);
     j.rowsPer = std::max(1, 512 / groups);
-    j.perRow = vlb::FastDiv(groups);
+    j.perRow = vlb::FastDiv31(groups);
     j.block0 = blocks;
     j.blocks = vlb::ceil_div(j.x.rows, j.rowsPer);
     blocks += j.blocks;
