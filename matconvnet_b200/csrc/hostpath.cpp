@@ -632,6 +632,15 @@ void on_device_of(at::Tensor const& x, std::initializer_list<at::Tensor const*> 
   if (x.device().index() != c10::cuda::current_device()) fail(PyExc_ValueError, "X must be on the current CUDA device.");
 }
 
+// The dimensions as the C ABI takes them: 32-bit numbers.
+Shape int_shape4(at::Tensor const& t, char const* name)
+{
+  Shape const s = shape4(t);
+  for (int64_t d : s.d)
+    if (d > INT32_MAX) fail(PyExc_ValueError, "%s is too large: its dimensions must be 32-bit numbers.", name);
+  return s;
+}
+
 // ---------------------------------------------------------------- vl_nnlayernorm: ctx, x, g, b, dzdy, epsilon, der_out
 PyObject* lnorm(PyObject*, Args a, Py_ssize_t n)
 {
@@ -639,7 +648,7 @@ PyObject* lnorm(PyObject*, Args a, Py_ssize_t n)
     Ctx ctx(a[0]);
     at::Tensor x = need_one(a[1], "x"), g = need_one(a[2], "g"), b = need_one(a[3], "b"), dzdy = need(a[4], "dzdy");
     on_device_of(x, {&g, &b, &dzdy});
-    Shape const s = shape4(x);
+    Shape const s = int_shape4(x, "X");
     int const H = (int)s.d[0], W = (int)s.d[1], C = (int)s.d[2], N = (int)s.d[3];
     double const eps = as_double(a[5]);
     if (g.numel() != C) fail(PyExc_ValueError, "The number of elements of G is not the same as the depth of X.");
@@ -675,7 +684,7 @@ PyObject* fcsoftmaxloss(PyObject*, Args a, Py_ssize_t n)
     Ctx ctx(a[0]);
     at::Tensor x = need_one(a[1], "x"), f = need_one(a[2], "f"), b = need(a[3], "b"), c = need_one(a[4], "c"), lse = need(a[6], "lse");
     on_device_of(x, {&f, &b, &c, &lse});
-    Shape const s = shape4(x), sf = shape4(f);
+    Shape const s = int_shape4(x, "X"), sf = int_shape4(f, "F");
     int const H = (int)s.d[0], W = (int)s.d[1], C = (int)s.d[2], N = (int)s.d[3], K = (int)sf.d[3];
     if (sf.d[0] != H || sf.d[1] != W || sf.d[2] != C) fail(PyExc_ValueError, "The FILTERS must be as large as the images of X.");
     if (b.defined() && b.numel() != K) fail(PyExc_ValueError, "The number of elements of BIASES is not the same as the number of filters.");

@@ -21,3 +21,47 @@ def test_muon_on_rows_of_more_than_a_million_columns(gpu, rows, cols):
     g[:] = np.nan
     nn.solver_update_("muon", muon._up(w, shape), {"s1": muon._up(m, shape), "t": 1}, muon._up(g, shape), 0.5, 0.0, 0.1, muon.OPTS)
     muon._check(nn, [shape], seed=31)
+
+
+LONG = 2 ** 32 + 5                          # what a 32-bit number has of it is 5
+
+
+def test_dimensions_beyond_32_bits_are_refused(gpu):
+    """Tensors without elements, so that nothing has to be held: each dimension in turn is LONG and another one 0."""
+    import torch
+    nn = gpu[0]
+    some = torch.zeros(5, 1, device="cuda")
+    empty = lambda *s: torch.empty(s, device="cuda")                                                # noqa: E731
+    for at in range(4):
+        shape = [0 if i == (at + 1) % 4 else 1 for i in range(4)]
+        shape[at] = LONG
+        x = empty(*shape)
+        assert x.numel() == 0
+        with pytest.raises(ValueError, match="too large"):
+            nn.vl_nnlayernorm(x, some, some)
+        with pytest.raises(ValueError, match="too large"):
+            nn.vl_nnlayernorm(x, some, some, x)
+        for dzdy in (None, 1.0):
+            with pytest.raises(ValueError, match="too large"):
+                nn.vl_nnfcsoftmaxloss(x, empty(1, 1, 1, 5), None, some, dzdy)
+    for dzdy in (None, 1.0):
+        with pytest.raises(ValueError, match="F is too large"):
+            nn.vl_nnfcsoftmaxloss(empty(0, 1, 1, 5), empty(0, 1, 1, LONG), None, some, dzdy)
+    with pytest.raises(ValueError, match="too large"):
+        nn.vl_nnlayernorm(empty(1, 0, 3, 2 ** 20, 2 ** 12), some, some)                             # (trailing dimensions count as the fourth)
+
+
+def test_more_positions_than_32_bits_hold_are_refused(gpu):
+    """17 GB of them.  Five positions would be computed and the others left as they were found."""
+    import torch
+    nn = gpu[0]
+    if torch.cuda.mem_get_info()[0] < 60e9:
+        pytest.skip("needs room for two tensors of 17 GB")
+    one = torch.zeros(1, 1, device="cuda")
+    x = torch.empty(LONG, device="cuda").view(1, 1, 1, LONG)
+    try:
+        with pytest.raises(ValueError, match="too large"):
+            nn.vl_nnlayernorm(x, one, one)
+    finally:
+        del x
+        torch.cuda.empty_cache()
