@@ -41,7 +41,7 @@ struct Product {
 };
 
 template <int kMax> struct Batch {
-  CUtensorMap map[4 * kMax];                            // of each product A along its rows, along its columns, B likewise; those that are used
+  CUtensorMap map[4 * kMax];                            // of each product A along its rows, along its columns, B likewise
   Product p[kMax];
   int count, work, three;
   int lead, behind, even;                               // item_at
@@ -772,7 +772,8 @@ make_pair_kernel(const __grid_constant__ SplitJobs jobs)
 }
 
 // ------------------------------------------------------------------ host
-// The maps of a side, along its rows and along its columns: hi and lo (or hi alone) in one copy.
+// The maps of a side, along its rows and along its columns: hi and lo (or hi alone) in one copy.  A way that no tile is read in has the other one's map: the kernel
+// asks for both ahead of time.
 bool encode_side(CUtensorMap* map, vlb::PairSide const& s, bool three)
 {
   EncodeTiledFn const encode = encode_tiled();
@@ -780,13 +781,16 @@ bool encode_side(CUtensorMap* map, vlb::PairSide const& s, bool three)
   cuuint64_t const dims[3] = {(cuuint64_t)s.m.cols, (cuuint64_t)s.m.rows, 2};
   cuuint64_t const strides[2] = {(cuuint64_t)s.m.ld * 2, (cuuint64_t)((char*)s.m.lo - (char*)s.m.hi)};
   cuuint32_t const one[3] = {1, 1, 1};
+  bool const read[2] = {!s.byCols, s.byCols || s.lower};
   for (int along = 0; along < 2; ++along) {
-    if (!(along ? s.byCols || s.lower : !s.byCols)) continue;
+    if (!read[along]) continue;
     cuuint32_t const box[3] = {64, along ? 64u : 128u, three ? 2u : 1u};
     if (encode(map + along, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, s.m.hi, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return false;
   }
+  for (int along = 0; along < 2; ++along)
+    if (!read[along]) map[along] = map[1 - along];
   return true;
 }
 
