@@ -89,7 +89,7 @@ int vlb_ctx_set_wait_limit(vlb_ctx* ctx, long long cycles);
 /* Test switches (0 = none).  Bit 0: the filter-tile loader of the tensor-memory convolution kernel stays idle, so every
  * wait behind it runs out: the kernel records its status word, releases its tensor memory and returns
  * (vlb_ctx_device_status then gives VLE_Timeout; the output of that call is undefined).  Nothing traps or spins.
- * The same for the products of matrices of vlb_fc_softmaxloss_* and vlb_muon_update_many.
+ * The same for the products of matrices of vlb_fc_softmaxloss_* and vlb_muon_update_many, and for the rows that vlb_lnorm_backward has copied ahead.
  * Bit 1: the tensor-memory convolution kernel gathers its input windows with per-thread loads even where it could have
  * them delivered by tensor-map copies; the two routes give the same result bit for bit, which is what a test compares.
  * Bit 2: the filter gradient of a convolution takes the kernel with both operands in shared memory even where the

@@ -112,7 +112,7 @@ constexpr int kStages = 3;
 template <int kThreads, int kVec, bool kWide>
 __global__ void __launch_bounds__(block_of(kThreads))
 rows_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* __restrict__ x, float const* __restrict__ g, float const* __restrict__ dy,
-                int rows, int C, int per, float eps, int* status)
+                int rows, int C, int per, float eps, int* status, int idle)
 {
   using R = Row<kThreads, kVec, kWide>;
   constexpr int kRows = block_of(kThreads) / kThreads, kWarps = block_of(kThreads) / 32;
@@ -130,7 +130,9 @@ rows_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* 
   }
   vlb::pdl_wait();
   bool dead = false;                                       // a wait ran out: nothing is waited for any more
+  int asked = 0;                                           // groups that were asked for
   auto fetch = [&](int it) {                               // by one thread
+    if (idle) return;                                      // (test switch: nothing comes, so that every wait runs out)
     int const st = it % kStages, row0 = ((int)blockIdx.x + it * (int)gridDim.x) * group, count = min(group, rows - row0);
     if (it >= kStages && !dead && !mbar_wait(smem_u32(&empty[st]), (uint32_t)(it / kStages - 1) & 1u)) dead = true;
     if (dead) return;
@@ -138,6 +140,7 @@ rows_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* 
     mbar_arrive_expect_tx(smem_u32(&full[st]), 2 * bytes);
     bulk_copy_g2s(to, x + (size_t)row0 * C, bytes, smem_u32(&full[st]));
     bulk_copy_g2s(to + (uint32_t)group * C * 4, dy + (size_t)row0 * C, bytes, smem_u32(&full[st]));
+    asked = it + 1;
   };
   if (kWide && threadIdx.x == 0)
     for (int it = 0; it < min(mine, kStages - 1); ++it) fetch(it);
@@ -196,6 +199,9 @@ rows_bwd_kernel(float* __restrict__ dx, float* __restrict__ parts, float const* 
     }
   }
   if (dead) atomicCAS(status, 0, 43);
+  // copies still on their way when the wait of the thread that asked for them ran out land before the block ends
+  if (kWide && threadIdx.x == 0 && dead)
+    for (int it = max(0, asked - kStages); it < asked; ++it) mbar_wait(smem_u32(&full[it % kStages]), (uint32_t)(it / kStages) & 1u, kWaitCycles);
   if (!parts) return;
   if (kRows > 1) {
     // the block's warps, added in order
@@ -717,7 +723,7 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
         ready[ctx->device & 63] = failed == cudaSuccess;
       }
       if (failed == cudaSuccess)
-        vlb::launch(ctx->stream, kernel, (unsigned)blocks, block_of(kThreads), smem, dX, parts, X, g, dY, N, C, per, (float)eps, ctx->deviceStatus);
+        vlb::launch(ctx->stream, kernel, (unsigned)blocks, block_of(kThreads), smem, dX, parts, X, g, dY, N, C, per, (float)eps, ctx->deviceStatus, ctx->testSwitch & 1);
     });
     if (failed != cudaSuccess) return vlb::set_error(ctx, VLB_Cuda, cudaGetErrorString(failed));
     if (!blocks) {

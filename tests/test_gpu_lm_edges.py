@@ -3,6 +3,7 @@ waits that run out, contexts of another device."""
 import numpy as np
 import pytest
 
+import test_gpu_lnorm as lnorm
 import test_gpu_muon as muon
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +66,24 @@ def test_more_positions_than_32_bits_hold_are_refused(gpu):
     finally:
         del x
         torch.cuda.empty_cache()
+
+
+def test_layer_normalisation_whose_waits_run_out(gpu):
+    """No row comes, so no wait is ever answered: the kernel gives up, says so and leaves everything as the next call needs it."""
+    from matconvnet_b200 import capi
+    nn, mat, _ = gpu
+    for shape in ((1, 1, 64, 5000), (1, 1, 1024, 900), (1, 1, 8192, 200)):
+        ctx = capi.Context()
+        x, g, b, dy = (mat.from_numpy(a) for a in lnorm._inputs(shape, 6))
+        want = nn.vl_nnlayernorm(x, g, b, dy, ctx=ctx)
+        assert ctx.device_status() == 0
+        try:
+            ctx.check(ctx.lib.vlb_ctx_set_wait_limit(ctx.handle, 200000))
+            ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 1))
+            nn.vl_nnlayernorm(x, g, b, dy, ctx=ctx)
+            with pytest.raises(capi.VlbError, match="TIMEOUT|Timeout|timeout"):
+                ctx.device_status()
+        finally:
+            ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 0))
+            ctx.check(ctx.lib.vlb_ctx_set_wait_limit(ctx.handle, 0))
+        assert all((p == q).all() for p, q in zip(nn.vl_nnlayernorm(x, g, b, dy, ctx=ctx), want)) and ctx.device_status() == 0
