@@ -101,13 +101,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 small_kernel(const __grid_constant__ Matrices all, bool three)
 {
   extern __shared__ char raw[];
-  __shared__ __align__(8) uint64_t through;
+  __shared__ __align__(8) uint64_t through, last;
   __shared__ uint32_t tmemAt;
   __shared__ double sums[kThreads / 32];
   char* const base = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   char* const gramAt = base + kMostBlocks * kBlock;           // A, then Q: two blocks
   int const warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = all.cluster, rank = (int)blockIdx.x % G, which = (int)blockIdx.x / G;
-  if (threadIdx.x == 0) { mbar_init(smem_u32(&through), 1); asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+  if (threadIdx.x == 0) { mbar_init(smem_u32(&through), 1); mbar_init(smem_u32(&last), 1); asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
   if (warp == 0) tmem_alloc(smem_u32(&tmemAt), 512);
   tc_fence_before();
   __syncthreads();
@@ -306,6 +306,9 @@ small_kernel(const __grid_constant__ Matrices all, bool three)
       }
   }
   if (dead && lane == 0) atomicCAS(all.status, 0, 44);
+  // products that still run when the wait of the thread that issued them ran out end before the shared memory and the tensor memory that they use is given back
+  if (dead && threadIdx.x == 0) { umma_commit(smem_u32(&last)); mbar_wait(smem_u32(&last), 0u, kWaitCycles); }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   cluster_sync();
