@@ -583,8 +583,9 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
           }
         }
         if (dead) atomicCAS(batch.status, 0, 40);
-        // copies still on their way when a wait ran out land before the block ends
-        if (dead && rank == 0)
+        // copies still on their way when a wait ran out -- this warp's, or that of the warp which issues the products and had these copies left to wait for -- land
+        // before the block ends
+        if (rank == 0)
           for (int j = max(0, it - kStages); j < it; ++j) mbar_wait(smem_u32(&full[j % kStages]), (uint32_t)(j / kStages) & 1u, kWaitCycles);
       }
     } else if (warp == 9) {
