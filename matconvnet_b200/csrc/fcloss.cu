@@ -138,9 +138,10 @@ __device__ __forceinline__ Part joined(Part p, F part)
 }
 
 // lse of 32 images per block from the parts of their predictions, and the loss by the block that is through last, which adds the blocks' sums in their order.
-// lse and labels: of the images first ... first + rows - 1; sums: one per block of 32 images of all `blocks`.
+// lse and labels: of the images first ... first + rows - 1; sums: one per block of 32 images of all `blocks`.  more: pieces of classes are still to come, and the parts
+// so far are left as one, the first.
 __global__ void __launch_bounds__(1024)
-lse_kernel(float* __restrict__ loss, float* __restrict__ lse, float2 const* __restrict__ parts, int count, float const* __restrict__ label,
+lse_kernel(float* __restrict__ loss, float* __restrict__ lse, float2* parts, int count, bool more, float const* __restrict__ label,
            float const* __restrict__ labels, int rows, int first, int N, int K, double* sums, int blocks, int* ticket, int* status)
 {
   vlb::pdl_wait();
@@ -151,13 +152,17 @@ lse_kernel(float* __restrict__ loss, float* __restrict__ lse, float2 const* __re
     for (int i0 = ty; i0 < count; i0 += 32 * 8)
       p = joined<8>(p, [&](int k) {
         int const i = i0 + 32 * k;
-        float2 const v = i < count ? __ldg(parts + (long long)i * rows + row) : make_float2(-INFINITY, 0.f);
+        float2 const v = i < count ? parts[(long long)i * rows + row] : make_float2(-INFINITY, 0.f);
         return Part{v.x, v.y};
       });
   all[ty][tx] = p;
   __syncthreads();
   if (ty) return;
   p = joined<31>(p, [&](int i) { return all[i + 1][tx]; });
+  if (more) {
+    if (row < rows) parts[row] = make_float2(p.top, p.sum);          // (an image's parts are read by this block alone)
+    return;
+  }
   double term = 0;
   if (row < rows) {
     Label const l = label_of(labels, row, K, status);
@@ -205,7 +210,7 @@ constexpr int kMostImages = 16384;          // images at a time
 constexpr int kDzExp = 14;                  // derivatives of the predictions, at most 1 in magnitude, times 2^14
 constexpr size_t kMostScratch = 1u << 30;   // what the pieces of classes may take
 
-// The call's scratch, cut up.
+// The call's scratch, cut up.  withSeen: the log-sum-exp are computed, from parts of what the pieces of classes show (the first: what the pieces before them showed).
 struct Plan {
   int images, piece;                        // images at a time, classes at a time
   size_t bytes;
@@ -215,11 +220,12 @@ struct Plan {
   float2* parts; float *label, *lse, *db;
   double* sums;
 
-  Plan(int N, int D, int K, bool back, size_t scratch, char* at = nullptr)
+  Plan(int N, int D, int K, bool back, bool withSeen, size_t scratch, char* at = nullptr)
   {
     images = std::min(N, kMostImages);
+    // (the parts of many images of few features, 8 bytes for 64 classes, can be more than the pairs: as much again at most)
     size_t const perClass = 4 * (size_t)vlb::pair_ld(D) + (back ? 4 * (size_t)images + (size_t)images / 8 + 64 : 0);
-    long long const most = std::max<long long>(256, (long long)(scratch / perClass) / 256 * 256);
+    long long const most = std::max<long long>(256, (long long)(scratch / std::max(perClass, withSeen ? (size_t)images / 8 : 0)) / 256 * 256);
     int const pieces = vlb::ceil_div(K, most);
     piece = (int)std::min<long long>(K, vlb::ceil_div(vlb::ceil_div(K, pieces), 256) * 256ll);
     bytes = 0;
@@ -230,22 +236,22 @@ struct Plan {
     x = take(vlb::pair_bytes(images, D));
     f = take(vlb::pair_bytes(piece, D));
     split = take(vlb::kPairSplitBytes);
-    parts = (float2*)take(sizeof(float2) * (size_t)images * vlb::pair_parts(piece, 128) * pieces);
-    label = (float*)take(sizeof(float) * (size_t)images);
-    lse = (float*)take(sizeof(float) * (size_t)images);
-    sums = (double*)take(sizeof(double) * (size_t)vlb::ceil_div(N, 32));
+    parts = withSeen ? (float2*)take(sizeof(float2) * (size_t)images * (vlb::pair_parts(piece, 128) + (pieces > 1 ? 1 : 0))) : nullptr;
+    label = withSeen ? (float*)take(sizeof(float) * (size_t)images) : nullptr;
+    lse = back && withSeen ? (float*)take(sizeof(float) * (size_t)images) : nullptr;
+    sums = back ? nullptr : (double*)take(sizeof(double) * (size_t)vlb::ceil_div(N, 32));
     dz = back ? take(vlb::pair_bytes(images, piece)) : nullptr;
     db = back ? (float*)take(sizeof(float) * (size_t)vlb::ceil_div(images, 32) * vlb::pair_ld(piece)) : nullptr;
   }
 };
 
 // A plan whose scratch there is: smaller pieces where there is less.
-bool plan_for(vlb_ctx* ctx, Plan& plan, int N, int D, int K, bool back)
+bool plan_for(vlb_ctx* ctx, Plan& plan, int N, int D, int K, bool back, bool withSeen)
 {
   for (size_t scratch = kMostScratch; scratch >= (16u << 20); scratch /= 4) {
-    plan = Plan(N, D, K, back, scratch);
+    plan = Plan(N, D, K, back, withSeen, scratch);
     void* const p = scratch / 4 >= (16u << 20) ? vlb::try_workspace(ctx, plan.bytes) : vlb::workspace(ctx, plan.bytes);
-    if (p) { plan = Plan(N, D, K, back, scratch, (char*)p); return true; }
+    if (p) { plan = Plan(N, D, K, back, withSeen, scratch, (char*)p); return true; }
   }
   return false;
 }
@@ -283,26 +289,25 @@ vlb::PairProduct predictions(Problem const& q, Plan const& plan, vlb::Pair x, vl
 // lse of images n0 ... and, after the last of them, the loss (either may be null).  The pairs of the images and of the last piece are left.
 int seen(Problem const& q, Plan const& plan, int n0, float* lse, float* loss, int* status)
 {
-  int count = 0;
   int const rows = std::min(plan.images, q.N - n0);
   for (int k0 = 0; k0 < q.K; k0 += plan.piece) {
     Sides const s = sides(q, plan, n0, k0, k0 == 0);
     vlb::PairProduct p = predictions(q, plan, s.x, s.f, n0, k0);
-    p.e.parts = plan.parts + (size_t)count * rows; p.e.label = plan.label;
+    int const before = k0 ? 1 : 0;          // what the pieces before this one have shown
+    p.e.parts = plan.parts + (size_t)before * rows; p.e.label = plan.label;
     int const tile = vlb::pair_tile(q.ctx, &p, 1);
     if (int const rc = vlb::products_of_pairs(q.ctx, vlb::kPairSeen, &p, 1, plan.split, tile)) return rc;
-    count += vlb::pair_parts(s.f.rows, tile);
+    vlb::launch(q.ctx->stream, lse_kernel, (unsigned)vlb::ceil_div(rows, 32), 1024, 0, loss, lse, plan.parts, before + vlb::pair_parts(s.f.rows, tile),
+                q.K - k0 > plan.piece, plan.label, q.labels + n0, rows, n0, q.N, q.K, plan.sums, vlb::ceil_div(q.N, 32), q.ctx->deviceStatus + 64 + 4095, status);
+    VLB_LAUNCHED(q.ctx, 1);
   }
-  vlb::launch(q.ctx->stream, lse_kernel, (unsigned)vlb::ceil_div(rows, 32), 1024, 0, loss, lse, plan.parts, count, plan.label, q.labels + n0, rows, n0,
-              q.N, q.K, plan.sums, vlb::ceil_div(q.N, 32), q.ctx->deviceStatus + 64 + 4095, status);
-  VLB_LAUNCHED(q.ctx, 1);
   return VLB_Success;
 }
 
 int forward_on_pairs(Problem const& q, float* loss, float* lse)
 {
-  Plan plan(1, 1, 1, false, 0);
-  if (!plan_for(q.ctx, plan, q.N, q.D, q.K, false)) return q.ctx->lastError;
+  Plan plan(1, 1, 1, false, false, 0);
+  if (!plan_for(q.ctx, plan, q.N, q.D, q.K, false, true)) return q.ctx->lastError;
   vlb::ProfScope prof(q.ctx, vlb::kProfFc);
   prof.rec.flops = 2.0 * q.N * q.D * q.K;
   for (int n0 = 0; n0 < q.N; n0 += plan.images)
@@ -312,8 +317,8 @@ int forward_on_pairs(Problem const& q, float* loss, float* lse)
 
 int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float const* lse, float scale)
 {
-  Plan plan(1, 1, 1, true, 0);
-  if (!plan_for(q.ctx, plan, q.N, q.D, q.K, true)) return q.ctx->lastError;
+  Plan plan(1, 1, 1, false, false, 0);
+  if (!plan_for(q.ctx, plan, q.N, q.D, q.K, true, !lse)) return q.ctx->lastError;
   vlb::ProfScope prof(q.ctx, vlb::kProfFc);
   prof.rec.flops = 2.0 * q.N * q.D * q.K * ((dX ? 1 : 0) + (dF ? 1 : 0) + (lse ? 1 : 2));
   for (int n0 = 0; n0 < q.N; n0 += plan.images) {

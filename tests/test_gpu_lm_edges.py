@@ -3,6 +3,7 @@ waits that run out, contexts of another device."""
 import numpy as np
 import pytest
 
+import test_gpu_fcloss as fcloss
 import test_gpu_lnorm as lnorm
 import test_gpu_muon as muon
 
@@ -87,3 +88,73 @@ def test_layer_normalisation_whose_waits_run_out(gpu):
             ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 0))
             ctx.check(ctx.lib.vlb_ctx_set_wait_limit(ctx.handle, 0))
         assert all((p == q).all() for p, q in zip(nn.vl_nnlayernorm(x, g, b, dy, ctx=ctx), want)) and ctx.device_status() == 0
+
+
+def _fcloss_data(n, d, k, seed):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x, f = torch.randn(n, d, device="cuda", generator=gen), torch.randn(k, d, device="cuda", generator=gen) * (2 / d ** 0.5)
+    b = torch.randn(k, 1, device="cuda", generator=gen)
+    c = torch.randint(0, k + 1, (n,), device="cuda", generator=gen).float()
+    up = lambda t: t.view(t.shape[0], t.shape[1], 1, 1).permute(3, 2, 1, 0)                         # noqa: E731
+    return x, f, b, c, up(x), up(f)
+
+
+@pytest.mark.parametrize("n,d,k", [(16384 + 300, 40, 15000)])
+def test_fcloss_in_pieces_of_classes_and_of_images(gpu, n, d, k):
+    """With the smallest pieces: dX is added up over pieces of classes, dF over pieces of images, the parts of a log-sum-exp over the former.  Tolerances as in
+    test_gpu_fcloss.py; sums in 64 bits on the device."""
+    import torch
+    from matconvnet_b200 import capi
+    nn = gpu[0]
+    x, f, b, c, xd, fd = _fcloss_data(n, d, k, 40)
+    xs, fs, bs = x.double(), f.double(), b.double().view(-1)
+    real, at = c > 0, (c.long() - 1).clamp(min=0)
+    lse, dx, df, db, loss = torch.zeros(n, device="cuda", dtype=torch.float64), torch.zeros_like(xs), torch.zeros_like(fs), torch.zeros_like(bs), 0.0
+    for i in range(0, n, 4096):
+        p = slice(i, min(n, i + 4096))
+        z = xs[p] @ fs.T + bs
+        lse[p] = torch.logsumexp(z, 1) * real[p]
+        loss += ((torch.logsumexp(z, 1) - z.gather(1, at[p, None])[:, 0]) * real[p]).sum() / n
+        z = (z - torch.logsumexp(z, 1, keepdim=True)).exp()
+        z.scatter_add_(1, at[p, None], -torch.ones_like(z[:, :1]))
+        z *= real[p, None] / n
+        dx[p] = z @ fs
+        df += z.T @ xs[p]
+        db += z.sum(0)
+    ctx = capi.Context()
+    ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 32))
+    gl, gs = nn.vl_nnfcsoftmaxloss(xd, fd, b, c, ctx=ctx)
+    assert abs(float(gl) - float(loss)) <= fcloss.TOL_LSE * 10 and float((gs - lse).abs().max()) <= fcloss.TOL_LSE * 10
+    rel = lambda a, r: float((a.double() - r).norm() / r.norm())                                    # noqa: E731
+    for kept in (gs, None):
+        gx, gf, gb = nn.vl_nnfcsoftmaxloss(xd, fd, b, c, 1.0, lse=kept, ctx=ctx)
+        for got, want in ((gx.permute(3, 2, 1, 0).reshape(n, d), dx), (gf.permute(3, 2, 1, 0).reshape(k, d), df), (gb.view(-1), db)):
+            assert rel(got, want) <= fcloss.TOL
+
+
+def test_fcloss_scratch_is_what_a_call_needs(gpu):
+    """Many images and classes of few features.  What the products' epilogues leave of a piece of classes -- 8 bytes for an image and 64 classes -- goes by the piece, and
+    is not taken where the log-sum-exp are given."""
+    from matconvnet_b200 import capi
+    nn = gpu[0]
+    n, d, k = 8192, 8, 300000
+    _, _, b, c, xd, fd = _fcloss_data(n, d, k, 41)
+    pairs, parts = 4 * 64 * n, n * 2 * (-(-k // 128)) * 8
+    assert parts > 300e6
+    ctx = capi.Context()
+    ctx.check(ctx.lib.vlb_ctx_set_test_switch(ctx.handle, 32))              # the smallest pieces: 16 MB for pairs, as much for parts
+    want = nn.vl_nnfcsoftmaxloss(xd, fd, b, c, ctx=ctx)
+    assert ctx.workspace_bytes < 2 * (16 << 20) + (64 << 20) + pairs + (1 << 20)
+    whole = nn.vl_nnfcsoftmaxloss(xd, fd, b, c, ctx=gpu[2])
+    for p, q in zip(want, whole):
+        assert float((p - q).abs().max()) <= 2 * fcloss.TOL_LSE * 15        # (lse near log(k) + 2, either side off by TOL_LSE of it)
+    # one piece, backward: pairs of X, F and the derivative of the predictions, its sums over 32 images, 64 MB for parts of sums
+    n, d, k = 4096, 8, 20032
+    _, _, b, c, xd, fd = _fcloss_data(n, d, k, 42)
+    lse = nn.vl_nnfcsoftmaxloss(xd, fd, b, c)[1]
+    need = 4 * 64 * (n + k) + 4 * n * k + 4 * (n // 32) * k + (64 << 20)
+    parts = n * 2 * (-(-k // 128)) * 8
+    ctx = capi.Context()
+    nn.vl_nnfcsoftmaxloss(xd, fd, b, c, 1.0, lse=lse, ctx=ctx)
+    assert need <= ctx.workspace_bytes < need + parts // 2
