@@ -198,18 +198,18 @@ int set_up(Jobs& jobs, int count, vlb_muon_param const* u)
   return blocks;
 }
 
-int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* o)
-{
-  // all small: all steps in one launch.  (Beside larger ones they cost next to nothing in the launches that those need.)
-  bool small = true;
-  for (int i = 0; i < count; ++i) small = small && vlb::small_fits(u[i].rows, u[i].cols, o->steps);
+// The scratch of a pass, cut up from `at` on.
+struct Layout {
+  size_t bytes = 0;
+  bool small = true;                 // all are: all steps in one launch.  (Beside larger ones they cost next to nothing in the launches that those need.)
+  char* split;
   Jobs jobs = {};
   vlb::Pair x[2][kMost], a[kMost], q[kMost];
-  size_t bytes = 0;
-  char *at = nullptr, *split = nullptr;
-  auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
-  for (int pass = 0; pass < 2; ++pass) {
-    bytes = 0;
+
+  Layout(int count, vlb_muon_param const* u, int steps, char* at)
+  {
+    auto take = [&](size_t n) { char* const p = at + bytes; bytes += (n + 255) / 256 * 256; return p; };
+    for (int i = 0; i < count; ++i) small = small && vlb::small_fits(u[i].rows, u[i].cols, steps);
     split = take(small ? 0 : vlb::kPairSplitBytes);
     for (int i = 0; i < count; ++i) {
       int const rows = u[i].rows, cols = u[i].cols, m = std::min(rows, cols);
@@ -221,8 +221,19 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
       a[i] = vlb::pair_at(take(vlb::pair_bytes(m, m)), m, m);
       q[i] = vlb::pair_at(take(vlb::pair_bytes(m, m)), m, m);
     }
-    if (pass == 0 && !(at = (char*)vlb::workspace(ctx, bytes))) return ctx->lastError;
   }
+};
+
+int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* o)
+{
+  char* const at = (char*)vlb::workspace(ctx, Layout(count, u, o->steps, nullptr).bytes);
+  if (!at) return ctx->lastError;
+  Layout l(count, u, o->steps, at);
+  bool const small = l.small;
+  char* const split = l.split;
+  Jobs& jobs = l.jobs;
+  auto const &x = l.x;
+  auto const &a = l.a, &q = l.q;
   int blocks = set_up(jobs, count, u);
   vlb::launch(ctx->stream, momentum_kernel, (unsigned)blocks, kThreads, 0, jobs, (float)gradMult, (float)o->momentum, o->nesterov);
   VLB_LAUNCHED(ctx, 1);
@@ -286,13 +297,19 @@ int update_on_pairs(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gra
   return VLB_Success;
 }
 
+size_t exact_bytes(vlb_muon_param const& u)
+{
+  size_t const n = (size_t)u.rows * u.cols, m = std::min(u.rows, u.cols);
+  return sizeof(double) * kMaxParts + sizeof(float) * (2 * n + 2 * m * m);
+}
+
 // VLB_PRECISION_FP32: products on CUDA cores, one parameter after the other.
 int update_exact(vlb_ctx* ctx, vlb_muon_param const& u, double gradMult, vlb_muon_opts const* o)
 {
   int const rows = u.rows, cols = u.cols, m = std::min(rows, cols);
   size_t const n = (size_t)rows * cols;
   Jobs jobs = {};
-  jobs.j[0].parts = (double*)vlb::workspace(ctx, sizeof(double) * kMaxParts + sizeof(float) * (2 * n + 2 * (size_t)m * m));
+  jobs.j[0].parts = (double*)vlb::workspace(ctx, exact_bytes(u));
   if (!jobs.j[0].parts) return ctx->lastError;
   float *x = jobs.j[0].u = (float*)(jobs.j[0].parts + kMaxParts), *next = x + n, *const a = next + n, *const q = a + (size_t)m * m;
   unsigned const blocks = (unsigned)set_up(jobs, 1, &u);
@@ -324,6 +341,16 @@ bool overlap(vlb_muon_param const& a, vlb_muon_param const& b)
   return overlap(b.W, m, a.G, n) || overlap(b.S1, m, a.G, n);
 }
 
+// Items first ... end - 1 go through all steps together: as many as fit a pass, each of them apart from those in front of it.
+int end_of_pass(int first, int count, vlb_muon_param const* u, bool exact)
+{
+  int end = first + 1;
+  for (; end < count && end - first < (exact ? 1 : kMost); ++end)
+    for (int i = first; i < end; ++i)
+      if (overlap(u[i], u[end])) return end;
+  return end;
+}
+
 }  // namespace
 
 extern "C" {
@@ -339,12 +366,15 @@ int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, doubl
     VLB_REQUIRE(ctx, u[i].W && u[i].S1 && u[i].G, "muon_update_many: null tensor");
   }
   bool const exact = ctx->precision == VLB_PRECISION_FP32;
+  // the scratch of the pass that needs most is there before the first one: a call that cannot have it has changed nothing
+  size_t most = 0;
   for (int first = 0, end; first < count; first = end) {
-    for (end = first + 1; end < count && end - first < (exact ? 1 : kMost); ++end) {
-      bool apart = true;
-      for (int i = first; apart && i < end; ++i) apart = !overlap(u[i], u[end]);
-      if (!apart) break;
-    }
+    end = end_of_pass(first, count, u, exact);
+    most = std::max(most, exact ? exact_bytes(u[first]) : Layout(end - first, u + first, o->steps, nullptr).bytes);
+  }
+  if (most && !vlb::workspace(ctx, most)) return vlb::pass_error(ctx, ctx->lastError, "vlb_muon_update_many");
+  for (int first = 0, end; first < count; first = end) {
+    end = end_of_pass(first, count, u, exact);
     int const rc = exact ? update_exact(ctx, u[first], gradMult, o) : update_on_pairs(ctx, end - first, u + first, gradMult, o);
     if (rc) return vlb::pass_error(ctx, rc, "vlb_muon_update_many");
   }

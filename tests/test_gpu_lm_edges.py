@@ -1,5 +1,7 @@
 """The operators of language models' training steps at the ends of what they take: long rows, dimensions beyond 32 bits, scratch that grows or is not to be had,
 waits that run out, contexts of another device."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -158,3 +160,27 @@ def test_fcloss_scratch_is_what_a_call_needs(gpu):
     ctx = capi.Context()
     nn.vl_nnfcsoftmaxloss(xd, fd, b, c, 1.0, lse=lse, ctx=ctx)
     assert need <= ctx.workspace_bytes < need + parts // 2
+
+
+@pytest.mark.parametrize("precision", ["3XTF32", "FP32"])
+def test_muon_whose_scratch_is_not_to_be_had_changes_nothing(gpu, precision):
+    """Sixteen banks and one behind them whose scratch no device has: the call is refused before the first of them is touched.  (Nothing looks at the last one's tensors.)"""
+    import torch
+    from matconvnet_b200 import capi
+    ctx = capi.Context(precision=getattr(capi, "PRECISION_" + precision))
+    w, s1, g = (torch.randn(17, 64, 40, device="cuda") for _ in range(3))
+    u = (capi.MuonParam * 17)()
+    for i in range(17):
+        u[i] = capi.MuonParam(w[i].data_ptr(), s1[i].data_ptr(), g[i].data_ptr(), 64, 40, 0.0, 0.1)
+    u[16] = capi.MuonParam(256, 512, 768, 2 ** 20, 2 ** 20, 0.0, 0.1)
+    o = capi.MuonOpts(0.95, 1e-7, 3.4445, -4.7750, 2.0315, 1, 5)
+    before = w.clone(), s1.clone()
+    torch.cuda.synchronize()
+    for alone in (False, True):              # the first banks in shared launches, and none of them in the same launch as another
+        if alone:
+            for i in range(1, 16):
+                u[i] = u[0]
+        assert ctx.lib.vlb_muon_update_many(ctx.handle, 17, u, 1.0, ctypes.byref(o)) == capi.ERROR_NAMES.index("VLE_OutOfGPUMemeory")
+        ctx.lib.vlb_ctx_reset_error(ctx.handle)
+        torch.cuda.synchronize()
+        assert (w == before[0]).all() and (s1 == before[1]).all()
