@@ -346,7 +346,8 @@ int vlb_sgd_update_many(vlb_ctx* ctx, int count, vlb_param_update const* u, doub
 int vlb_solver_update_many(vlb_ctx* ctx, int solver, int count, vlb_param_update const* u, double gradMult,
                            vlb_solver_opts const* opts);
 
-/* ---- operators of language models' training steps; no counterparts among the reference's operator classes ---- */
+/* ---- operators of language models' training steps; no counterparts among the reference's operator classes.  A context that was made on another device than
+ *      the current one is refused ---- */
 /* Layer normalisation over the channels of every position (h, w, n), as vlb_softmax_* and vlb_lrn_* treat positions; a sequence of tokens is a
  * batch of 1 x 1 x C images.  With the mean m and the variance v of a position's C values and r = 1/sqrt(v + eps):
  *   Y = g * (X - m) * r + b.

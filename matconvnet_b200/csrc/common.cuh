@@ -58,6 +58,8 @@ int pass_error(vlb_ctx* ctx, int code, char const* where);
 void* workspace(vlb_ctx* ctx, size_t bytes);
 // The same for a route that has another to fall back on: nullptr, and no error, where so much cannot be had.
 void* try_workspace(vlb_ctx* ctx, size_t bytes);
+// Whether the current device is the context's, whose scratch, status word and tickets a kernel of another one could not reach.
+bool on_its_device(vlb_ctx* ctx);
 // cudaPeekAtLastError after a launch, as the reference does (bits/datacu.cu:356-371).
 int check_launch(vlb_ctx* ctx, char const* where);
 

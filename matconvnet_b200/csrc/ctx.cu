@@ -67,6 +67,13 @@ void* try_workspace(vlb_ctx* ctx, size_t bytes)
   return grow_workspace(ctx, bytes == 0 ? 256 : bytes) == cudaSuccess ? ctx->workspace : nullptr;
 }
 
+bool on_its_device(vlb_ctx* ctx)
+{
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess) cudaGetLastError();
+  return device == ctx->device;
+}
+
 int check_launch(vlb_ctx* ctx, char const* where)
 {
   cudaError_t e = cudaPeekAtLastError();

@@ -723,6 +723,7 @@ int vlb_fc_softmaxloss_forward(vlb_ctx* ctx, float* loss, float* lse, float cons
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, good_shape(H, W, C, N, K), "fc_softmaxloss_forward: bad shape");
   VLB_REQUIRE(ctx, loss && X && F && labels, "fc_softmaxloss_forward: null tensor");
+  VLB_REQUIRE(ctx, vlb::on_its_device(ctx), "fc_softmaxloss_forward: the context belongs to another device than the current one");
   int const D = H * W * C;
   if (few_images(N, D)) return vlb::pass_error(ctx, forward_few({ctx, X, F, b, labels, N, D, K}, loss, lse), "vlb_fc_softmaxloss_forward");
   if (ctx->precision != VLB_PRECISION_FP32)
@@ -749,6 +750,7 @@ int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, f
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, good_shape(H, W, C, N, K), "fc_softmaxloss_backward: bad shape");
   VLB_REQUIRE(ctx, X && F && labels, "fc_softmaxloss_backward: null tensor");
+  VLB_REQUIRE(ctx, vlb::on_its_device(ctx), "fc_softmaxloss_backward: the context belongs to another device than the current one");
   int const D = H * W * C;
   if (few_images(N, D))
     return vlb::pass_error(ctx, backward_few({ctx, X, F, b, labels, N, D, K}, dX, dF, db, lse, (float)(dzdy / N)), "vlb_fc_softmaxloss_backward");

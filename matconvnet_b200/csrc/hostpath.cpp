@@ -666,6 +666,7 @@ PyObject* lnorm(PyObject*, Args a, Py_ssize_t n)
     Pair const given = two_items(a[6], held);
     int64_t const sc[2] = {C, 1};
     at::Tensor dx, dg = der_out(given.first, at::IntArrayRef(sc, 2), "DG"), db = der_out(given.second, at::IntArrayRef(sc, 2), "DB");
+    on_device_of(x, {&dg, &db});
     ctx.run([&] {
       dx = empty_cm(x.sizes(), x.device());
       if (!dg.defined()) dg = empty_cm(C, 1, x.device());
@@ -707,6 +708,7 @@ PyObject* fcsoftmaxloss(PyObject*, Args a, Py_ssize_t n)
     at::Tensor dx, df, db;
     if (wantF) df = der_out(given.first, at::IntArrayRef(sf.d, 4), "DF");
     if (wantB) db = der_out(given.second, at::IntArrayRef(sb, 2), "DB");
+    on_device_of(x, {&df, &db});
     ctx.run([&] {
       if (wantX) dx = empty4(s, x.device());
       if (wantF && !df.defined()) df = empty_cm(at::IntArrayRef(sf.d, 4), x.device());

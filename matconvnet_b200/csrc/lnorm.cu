@@ -648,6 +648,7 @@ int vlb_lnorm_forward(vlb_ctx* ctx, float* Y, float const* X, float const* g, fl
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, !bad_shape(H, W, C, N), "lnorm_forward: bad shape");
   VLB_REQUIRE(ctx, Y && X && g && b, "lnorm_forward: null tensor");
+  VLB_REQUIRE(ctx, vlb::on_its_device(ctx), "lnorm_forward: the context belongs to another device than the current one");
   VLB_REQUIRE(ctx, eps >= 0, "lnorm_forward: epsilon is negative");
   int const P = H * W, positions = P * N;
   bool done = false;
@@ -698,6 +699,7 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, !bad_shape(H, W, C, N), "lnorm_backward: bad shape");
   VLB_REQUIRE(ctx, X && g && dY, "lnorm_backward: null tensor");
+  VLB_REQUIRE(ctx, vlb::on_its_device(ctx), "lnorm_backward: the context belongs to another device than the current one");
   VLB_REQUIRE(ctx, eps >= 0, "lnorm_backward: epsilon is negative");
   if (!dX && !dG && !dB) return VLB_Success;
   int const P = H * W, positions = P * N, most = most_parts(ctx, C);

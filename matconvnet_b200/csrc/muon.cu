@@ -365,6 +365,7 @@ int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, doubl
     VLB_REQUIRE(ctx, u[i].rows > 0 && u[i].cols > 0 && std::max(u[i].rows, u[i].cols) <= INT32_MAX - (1 << 20), "muon_update_many: bad shape");
     VLB_REQUIRE(ctx, u[i].W && u[i].S1 && u[i].G, "muon_update_many: null tensor");
   }
+  VLB_REQUIRE(ctx, vlb::on_its_device(ctx), "muon_update_many: the context belongs to another device than the current one");
   bool const exact = ctx->precision == VLB_PRECISION_FP32;
   // the scratch of the pass that needs most is there before the first one: a call that cannot have it has changed nothing
   size_t most = 0;

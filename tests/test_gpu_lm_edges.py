@@ -184,3 +184,26 @@ def test_muon_whose_scratch_is_not_to_be_had_changes_nothing(gpu, precision):
         ctx.lib.vlb_ctx_reset_error(ctx.handle)
         torch.cuda.synchronize()
         assert (w == before[0]).all() and (s1 == before[1]).all()
+
+
+def test_a_context_of_another_device_is_refused(gpu):
+    """Its scratch and its status word are not this device's.  The number of the device is the first word of a context."""
+    from matconvnet_b200 import capi
+    nn, mat, _ = gpu
+    x, g, b, dy = (mat.from_numpy(a) for a in lnorm._inputs((1, 1, 40, 50), 1))
+    c = mat.from_numpy(np.ones(50, np.float32))
+    ctx = capi.Context()
+    device = ctypes.c_int.from_address(ctx.handle.value)
+    calls = [lambda: nn.vl_nnlayernorm(x, g, b, ctx=ctx), lambda: nn.vl_nnlayernorm(x, g, b, dy, ctx=ctx), lambda: nn.vl_nnfcsoftmaxloss(x, dy, None, c, ctx=ctx),
+             lambda: nn.vl_nnfcsoftmaxloss(x, dy, None, c, 1.0, ctx=ctx), lambda: nn.solver_update_("muon", x, {}, dy, 1.0, 0.0, 0.1, ctx=ctx)]
+    assert device.value == 0
+    device.value = 1
+    try:
+        for call in calls:
+            with pytest.raises(capi.VlbError, match="device"):
+                call()
+    finally:
+        device.value = 0
+    for call in calls:
+        call()
+    assert ctx.device_status() == 0
