@@ -242,7 +242,7 @@ def _muon_update_many(updates, grad_mult, opts, ctx):
             raise ValueError("parameter and gradient do not have the same number of elements.")
         if not mat.is_mat(w) or ("s1" in state and (state["s1"].shape != w.shape or not mat.is_mat(state["s1"]))):
             raise ValueError("parameter and momentum must be column-major tensors of one shape.")
-        if g.shape != w.shape:
+        if mat.shape4(g) != mat.shape4(w):
             raise ValueError("parameter and gradient must have the same shape.")
     if int(o["steps"]) < 0 or not o["epsilon"] >= 0:
         raise ValueError("steps and epsilon must not be negative.")

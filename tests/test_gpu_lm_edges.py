@@ -207,3 +207,18 @@ def test_a_context_of_another_device_is_refused(gpu):
     for call in calls:
         call()
     assert ctx.device_status() == 0
+
+
+def test_muon_on_a_bank_of_one_filter_whose_derivative_has_a_fourth_dimension(gpu):
+    """A bank FH x FW x FC is one of a single filter; its derivative, as vl_nnconv returns it, is FH x FW x FC x 1."""
+    import torch
+    nn, mat, _ = gpu
+    w, m, g = muon._inputs((3, 3, 8, 1), 50)
+    three = lambda a: torch.from_numpy(a.copy()).cuda().view(8, 3, 3).permute(2, 1, 0)               # noqa: E731
+    want, got, one, two = muon._up(w, (3, 3, 8, 1)), three(w), {}, {}
+    for _ in range(2):
+        nn.solver_update_("muon", want, one, muon._up(g, (3, 3, 8, 1)), 1.0, 0.0, 0.1, muon.OPTS)
+        nn.solver_update_("muon", got, two, muon._up(g, (3, 3, 8, 1)), 1.0, 0.0, 0.1, muon.OPTS)
+    assert got.shape == (3, 3, 8) and two["t"] == 2 and (got == want[..., 0]).all() and (two["s1"] == one["s1"][..., 0]).all()
+    with pytest.raises(ValueError, match="shape"):
+        nn.solver_update_("muon", got, two, muon._up(g, (3, 3, 8, 1)).reshape(8, 3, 3, 1), 1.0, 0.0, 0.1, muon.OPTS)
