@@ -375,7 +375,7 @@ int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, f
 /* The Muon solver (Jordan and others, "Muon: an optimizer for hidden layers in neural networks", 2024) after the gradient exchange, beside
  * vlb_solver_update_many.  A parameter is a matrix of `rows` rows of `cols` neighbouring floats: a filter bank FH x FW x FC x K has K rows.
  *   g = gradMult*G + decay*W;  S1 = momentum*S1 + g;  u = nesterov ? g + momentum*S1 : S1;  X = u / (|u| + epsilon), |.| the Frobenius norm;
- *   `steps` times:  A = X X',  X = a*X + (b*A + c*A*A) X     (rows > cols: A = X'X and products from the right, the same matrix);
+ *   `steps` times (fewer than 65536):  A = X X',  X = a*X + (b*A + c*A*A) X     (rows > cols: A = X'X and products from the right, the same matrix);
  *   W -= lr * sqrt(max(1, rows/cols)) * X.
  * W and S1 (zero before the first step) are updated in place, G is only read.  All parameters go through every step together, in shared launches;
  * the result is that of one after the other: an item whose tensors overlap an earlier one's begins a pass of its own. */

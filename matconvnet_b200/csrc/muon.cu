@@ -360,6 +360,7 @@ int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, doubl
   if (!ctx) return VLB_IllegalArgument;
   VLB_REQUIRE(ctx, count >= 0 && (u || count == 0) && o, "muon_update_many: null argument");
   VLB_REQUIRE(ctx, o->steps >= 0 && o->epsilon >= 0, "muon_update_many: steps and epsilon must not be negative");
+  VLB_REQUIRE(ctx, o->steps < 65536, "muon_update_many: fewer than 65536 steps expected");       // (their exponents are computed before the first one)
   for (int i = 0; i < count; ++i) {
     // (32-bit counters, in strides below a million)
     VLB_REQUIRE(ctx, u[i].rows > 0 && u[i].cols > 0 && std::max(u[i].rows, u[i].cols) <= INT32_MAX - (1 << 20), "muon_update_many: bad shape");

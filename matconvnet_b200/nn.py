@@ -246,6 +246,8 @@ def _muon_update_many(updates, grad_mult, opts, ctx):
             raise ValueError("parameter and gradient must have the same shape.")
     if int(o["steps"]) < 0 or not o["epsilon"] >= 0:
         raise ValueError("steps and epsilon must not be negative.")
+    if int(o["steps"]) >= 65536:
+        raise ValueError("fewer than 65536 steps expected.")
     fresh = {}                                # a state that is new and named twice is one momentum tensor
     items = []
     for w, state, g, decay, lr in updates:

@@ -222,3 +222,21 @@ def test_muon_on_a_bank_of_one_filter_whose_derivative_has_a_fourth_dimension(gp
     assert got.shape == (3, 3, 8) and two["t"] == 2 and (got == want[..., 0]).all() and (two["s1"] == one["s1"][..., 0]).all()
     with pytest.raises(ValueError, match="shape"):
         nn.solver_update_("muon", got, two, muon._up(g, (3, 3, 8, 1)).reshape(8, 3, 3, 1), 1.0, 0.0, 0.1, muon.OPTS)
+
+
+def test_muon_steps_beyond_reason_are_refused(gpu):
+    from matconvnet_b200 import capi
+    nn, _, ctx = gpu
+    w, _, g = muon._inputs((1, 1, 6, 8), 60)
+    for steps in (2 ** 32 + 5, 2 ** 16):      # (32 bits of the first are 5)
+        v, state = muon._up(w, (1, 1, 6, 8)), {}
+        with pytest.raises(ValueError, match="steps"):
+            nn.solver_update_("muon", v, state, muon._up(g, (1, 1, 6, 8)), 1.0, 0.0, 0.1, dict(muon.OPTS, steps=steps))
+        assert (muon._down(v) == w).all() and not state
+    v, s1, d = (muon._up(a, (1, 1, 6, 8)) for a in (w, w, g))
+    u = capi.MuonParam(v.data_ptr(), s1.data_ptr(), d.data_ptr(), 8, 6, 0.0, 0.1)
+    for steps in (2 ** 31 - 1, 2 ** 16):
+        o = capi.MuonOpts(0.95, 1e-7, 3.4445, -4.7750, 2.0315, 1, steps)
+        assert ctx.lib.vlb_muon_update_many(ctx.handle, 1, ctypes.byref(u), 1.0, ctypes.byref(o)) == 7
+        ctx.lib.vlb_ctx_reset_error(ctx.handle)
+        assert (muon._down(v) == w).all()
