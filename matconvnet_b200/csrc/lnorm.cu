@@ -714,11 +714,13 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
     bool const vec = wide(C, {dX, X, g, dY});
     with_row(C, [&](auto threads, auto count) {
       constexpr int kThreads = decltype(threads)::value, kVec = decltype(count)::value, kRows = block_of(kThreads) / kThreads;
-      // as many blocks as fit the device at once: half of its threads, with sixteen values each of three tensors in registers; groups of rows of 16 KB
+      // Groups of rows of 16 KB, for four blocks of 128 threads per SM or as many threads in larger ones; and as many blocks as fit the device at once, which a block's
+      // three groups of X and dY decide where it has a row to a warp: with two blocks per SM 16384 x 512 takes 28.5 us, with four, of which two wait, 32.6.
       int const perSm = std::max(1, std::min(4, 512 / block_of(kThreads))), per = kThreads == 32 ? std::max(1, std::min(4096 / (C * kRows), N / (kRows * ctx->smCount * perSm))) : 1;
-      blocks = std::min(vlb::ceil_div(N, kRows * per), std::min(most, ctx->smCount * perSm));
+      size_t const smem = vec ? sizeof(float) * kStages * 2 * per * kRows * C : 0, other = 2048 + sizeof(float) * (kRows - 1) * 2 * 32 * 4 * kVec;
+      int const fit = std::max(1, std::min(perSm, (int)(228 * 1024 / (smem + other))));
+      blocks = std::min(vlb::ceil_div(N, kRows * per), std::min(most, ctx->smCount * fit));
       auto const kernel = vec ? rows_bwd_kernel<kThreads, kVec, true> : rows_bwd_kernel<kThreads, kVec, false>;
-      size_t const smem = vec ? sizeof(float) * kStages * 2 * per * kRows * C : 0;
       static bool ready[64];                               // (of this kernel and device)
       if (smem > 32 * 1024 && !ready[ctx->device & 63]) {
         failed = vlb::allow_max_dynamic_smem(kernel);
