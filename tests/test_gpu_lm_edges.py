@@ -240,3 +240,16 @@ def test_muon_steps_beyond_reason_are_refused(gpu):
         assert ctx.lib.vlb_muon_update_many(ctx.handle, 1, ctypes.byref(u), 1.0, ctypes.byref(o)) == 7
         ctx.lib.vlb_ctx_reset_error(ctx.handle)
         assert (muon._down(v) == w).all()
+
+
+@pytest.mark.parametrize("n,d,k", [(4, 40, 50), (200, 136, 700)])
+def test_fcloss_with_scales_of_data_and_filters_far_from_one(gpu, n, d, k):
+    """As at 2^40 in test_gpu_fcloss.py: powers of two on one side and their inverses on the other change nothing but the derivatives' scale."""
+    nn, mat, _ = gpu
+    x, f, b, c = fcloss._inputs(n, (1, 1, d), k, 6)
+    base = fcloss._check(nn, mat, x, f, b, c, (1, 1, d))
+    for e in (-80, 80):
+        s = np.float32(2.0 ** e)
+        far = fcloss._check(nn, mat, x * s, f / s, b, c, (1, 1, d))
+        for p, q in zip(base, far):
+            assert (p[0] == q[0] * s).all() and (p[1] == q[1] / s).all() and (p[2] == q[2]).all()
