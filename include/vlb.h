@@ -58,9 +58,12 @@ enum {
 /* vlb_fc_softmaxloss_* of more than 16 images hold X, F and the derivative of the predictions as such halves.  64 images of X share a power of two, and 64
  * classes of F: what is down to 2^-28 of the largest of them keeps 22 bits, smaller values are off by at most 2^-50 of it, and nothing is shared beyond
  * them.  The derivative of the predictions before its factor dzdy / N, at most 1 in magnitude, keeps 22 bits down to 2^-28 and is off by at most 2^-50
- * below.  An infinity or a not-a-number among the 64 reaches the sums that it is part of and no others.  vlb_muon_update_many does the same with the
+ * below.  An infinity or a not-a-number among the 64 reaches the sums that it is part of and no others.  This holds where the largest of the 64 lies between
+ * 2^-101 and 2^100: smaller ones lose digits as they near the subnormal range, and sums of larger ones may overflow on their way.  vlb_muon_update_many does the same with the
  * matrices of its steps, measured against the largest value that their elements can have.  VLB_PRECISION_TF32 keeps 11 bits; VLB_PRECISION_FP32 takes
- * products on CUDA cores. */
+ * products on CUDA cores.
+ * Exponentials exp(z - lse): rounding the difference costs |z - lse| / 2 units of the last place of the result; the fast exponential that is taken up to 16 images in every
+ * mode, and above in all but VLB_PRECISION_FP32, up to 2 + 1.2 |z - lse| more.  A share of 2^-24 of the sum is within 3e-6 of itself. */
 
 /* ---- context: replaces vl::Context (bits/data.hpp:150-179) and the stream part of
  *      vl::CudaHelper (bits/datacu.hpp:60-158; setStream bits/datacu.cu:70-93) ---- */
@@ -96,7 +99,7 @@ int vlb_ctx_set_wait_limit(vlb_ctx* ctx, long long cycles);
  * tensor-memory kernel applies (the two differ in the order of the sums; a test checks both against the CPU checker).
  * Bit 4: the filter gradient takes the form with the images along the reduction wherever that is possible, not only where it pays.
  * Bit 5: scratch that a call can do without is refused, as where the device's memory does not hold it: gradients come from the kernels that need no copy
- * of the data or of the output derivative.
+ * of the data or of the output derivative, and vlb_fc_softmaxloss_* take the smallest pieces of classes.
  * Bit 3: the tensor-memory convolution kernel keeps the running sum of an output tile in shared memory even for the tile
  * widths (64 and 128 columns) whose sum fits the registers of its drain warps; same additions in the same order, so the
  * results are equal, which is what a test compares. */
@@ -360,7 +363,9 @@ int vlb_lnorm_backward(vlb_ctx* ctx, float* dX, float* dG, float* dB, float cons
                        int H, int W, int C, int N, double eps);
 
 /* A fully connected prediction layer over K classes and the softmax loss behind it, vlb_fc_forward followed by vlb_softmaxloss_forward, without the
- * predictions in between: they are made in pieces of classes, in scratch, and never kept, so that K can be a vocabulary.  X: H x W x C x N,
+ * predictions in between, so that K can be a vocabulary: they are made in pieces of classes.  Forward none is stored, but for VLB_PRECISION_FP32, which has a piece of
+ * about 64 MB in scratch; backward the derivative of a piece is, 4 bytes for an image (16384 at most at a time) and class, in pieces that with their filters take up to 1 GB.
+ * X: H x W x C x N,
  * F: H x W x C x K, b: K floats or NULL, labels: one 1-based class label (as float) per image; label 0 skips the image and a label above K is
  * skipped and reported, as vlb_softmaxloss_* do.  With z = F'x + b of an image:
  *   lse = log(sum of exp(z)), 0 for an image that is skipped;  loss = (sum over the other images of lse - z[label]) / N.
@@ -377,8 +382,10 @@ int vlb_fc_softmaxloss_backward(vlb_ctx* ctx, float* dX, float* dF, float* db, f
  *   g = gradMult*G + decay*W;  S1 = momentum*S1 + g;  u = nesterov ? g + momentum*S1 : S1;  X = u / (|u| + epsilon), |.| the Frobenius norm;
  *   `steps` times (fewer than 65536):  A = X X',  X = a*X + (b*A + c*A*A) X     (rows > cols: A = X'X and products from the right, the same matrix);
  *   W -= lr * sqrt(max(1, rows/cols)) * X.
+ * The decay is part of what is orthogonalised, as it is part of the gradient in every solver here; it is no factor on W.
  * W and S1 (zero before the first step) are updated in place, G is only read.  All parameters go through every step together, in shared launches;
- * the result is that of one after the other: an item whose tensors overlap an earlier one's begins a pass of its own. */
+ * the result is that of one after the other -- an item whose tensors overlap an earlier one's begins a pass of its own -- but for rounding (1e-6 of W): what else is in a
+ * pass decides where sums are cut and whether small matrices take all steps in one launch.  The scratch of all passes is there before the first, or nothing is changed. */
 typedef struct { double momentum, epsilon, a, b, c; int nesterov, steps; } vlb_muon_opts;
 typedef struct { float *W, *S1; float const* G; int rows, cols; double decay, lr; } vlb_muon_param;
 int vlb_muon_update_many(vlb_ctx* ctx, int count, vlb_muon_param const* u, double gradMult, vlb_muon_opts const* opts);

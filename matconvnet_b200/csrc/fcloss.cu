@@ -366,7 +366,14 @@ int backward_on_pairs(Problem const& q, float* dX, float* dF, float* db, float c
 
 // ------------------------------------------------------------------ few images: on CUDA cores, bound by reading F
 // Up to sixteen images: F is read as it is, once forward and twice backward (and its derivative written); with the images in shared memory a class costs as
-// many multiplications as there are images, exact ones, which the cores do in the time that its row takes to arrive.
+// many multiplications as there are images, exact ones, which the cores do in the time that its row takes to arrive.  Microseconds forward / backward, F not in L2, here and on
+// pairs:
+//   images                          1                    8                    12                   16
+//   32000 classes, 1024 features    39/75   132/219      59/139   122/208     84/257   120/208     92/256   122/209
+//   81631 classes,  242 features    37/66   108/192      45/129    97/187     66/248    97/187     72/262   108/193
+//    1000 classes, 4096 features    21/23    38/63       47/63     38/63      53/82     38/63      (twelve images fill the shared memory)
+// Forward sixteen images are the limit of what the sums of a class take in registers; backward the second launch is the slower one from nine images on, and so is all of it where
+// few classes of long rows leave most warps idle.  There the products stay exact for the more that they take.
 constexpr int kFew = 16;
 constexpr int kFewFloats = 49152;             // images that fit shared memory: 192 KB
 constexpr int kFewWarps = 16;
@@ -382,6 +389,7 @@ struct FewArgs {
   float *dz, *db; float scale;                // backward: dz[class * kImages + n]
 };
 
+// The exponentials are fast ones: off by at most 2 + 1.2 |z - lse| units of the last place, where rounding the difference itself costs |z - lse| / 2.
 // Predictions, kRows classes at a time to the warps of all blocks in turn (neighbouring ones to different blocks); forward their largest and sum of exponentials, backward the derivatives.
 template <int kImages, int kRows, bool kBack, bool kWide>
 __global__ void __launch_bounds__(kFewWarps * 32, 1)

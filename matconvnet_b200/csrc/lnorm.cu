@@ -288,10 +288,16 @@ rows_bwd_long_kernel(float* __restrict__ dx, float* __restrict__ parts, float co
 
 // ------------------------------------------------------------------ positions of maps
 // A block takes tiles of kQ neighbouring positions: a thread has kPos neighbouring ones -- 4, by 16-byte accesses, where planes and tensors allow it, or 1 -- of
-// kValues channels in its registers, a warp's lanes kQ / kPos groups of positions of as many channels as fit.Small blocks, several to an SM, and many
+// kValues channels in its registers, a warp's lanes kQ / kPos groups of positions of as many channels as fit.  Small blocks, several to an SM, and many
 // values to a thread: what waits at one block's sums is covered by the loads of another's, and the sums over channels go over few warps.  28 x 28 x 512 x 64 forward:
 // 36 us, by one block of 16 warps and 32 positions 49; backward 67 and 176 (a block of 32 warps); 64 x 64 x 64 x 64 backward 40, by blocks of 8 warps with 4 channels to
 // a thread 169.  Tiles that come ahead through a ring in shared memory gained nothing over that: 36 / 38 us forward, 67 / 68 backward.
+// A launch takes the smallest shape that holds the channels.  With the next larger one, 28 x 28 and 27 x 29 (accesses of 16 and of 4 bytes), 40 million values, us:
+//   channels          32         64         128        256        512        1024
+//   28 x 28 forward   62 (81)    68 (78)    69 (86)    60 (88)    60 (91)    68 (111)
+//           backward  112 (135)  89 (141)   90 (146)   92 (157)   106 (179)  131 (242)
+//   27 x 29 forward   64 (109)   64 (97)    71 (102)   71 (108)   82 (126)   92 (138)
+//           backward  109 (186)  104 (174)  107 (180)  118 (186)  126 (200)  137 (247)
 struct Place { size_t at; bool in; };
 
 __device__ __forceinline__ Place place_of(long long q, long long positions, int P, int C)

@@ -7,7 +7,7 @@ A network is ``{'layers': [layer, ...]}`` with layers shaped like the reference'
   {'type': 'normalize', 'param': [N kappa alpha beta]}   {'type': 'softmax'}
   {'type': 'layernorm', 'weights': [g, b], 'epsilon': e}
   {'type': 'fcsoftmaxloss', 'weights': [f, b], 'class': c}  (a fully connected layer and the softmax loss behind it, its predictions
-  never stored; the images' log-sum-exp are kept in res[i]['aux'] for the backward pass)
+  not among the results; the images' log-sum-exp are kept in res[i]['aux'] for the backward pass)
   {'type': 'dropout', 'rate': r}  (training mode: a new mask per forward pass, kept in res[i]['aux'] for the backward pass)
 ``vl_simplenn(net, x, dzdy)`` runs the forward pass storing every intermediate (res[i]['x'],
 vl_simplenn.m:294-398) and, when dzdy is given, the backward pass in reverse order

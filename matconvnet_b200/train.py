@@ -6,7 +6,8 @@ moments), move the stored moments towards the batch's (cnn_train.m:468-476).
 ``params``: dict with learning_rate, weight_decay, momentum, nesterov_update (cnn_train.m:17-45 defaults: 0.001, 0.0005,
 0.9, False) and optionally solver ('adagrad', 'adadelta', 'adam' or 'rmsprop': examples/+solver/*.m, called at
 cnn_train.m:503-507 instead of the momentum step) with solver_opts (the solver's own defaults otherwise).  The solver 'muon'
-takes the filter banks of conv and fcsoftmaxloss layers; biases and multipliers, which are no matrices, take the momentum step beside it.  A layer may carry 'learningRate' / 'weightDecay' lists (per parameter multipliers, default 1;
+takes the filter banks of conv and fcsoftmaxloss layers; biases and multipliers, which are no matrices, take the momentum step beside it, all at one
+learning rate times their own multipliers.  (Its publication leaves a network's last, predicting layer to another solver; here that layer takes part.)  A layer may carry 'learningRate' / 'weightDecay' lists (per parameter multipliers, default 1;
 vl_simplenn_tidy).  ``state`` maps (layer index, parameter index) to the momentum tensor, created as zeros on first use
 (cnn_train.m:292-301).  Every tensor operation is a call into the C ABI.
 """
