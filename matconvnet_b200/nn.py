@@ -304,7 +304,8 @@ def vl_nnfcsoftmaxloss(x, f, b, c, dzdy=None, lse=None, no_der_data=False, no_de
     """[LOSS, LSE] = VL_NNFCSOFTMAXLOSS(X, F, B, C) / [DX, DF, DB] = VL_NNFCSOFTMAXLOSS(X, F, B, C, DZDY, 'lse', LSE): a fully
     connected layer whose outputs are the predictions of K classes and the softmax loss behind it,
     vl_nnsoftmaxloss(vl_nnconv(X, F, B), C), without the predictions, so that K can be a vocabulary: they are made in pieces of
-    classes, of which the forward pass keeps none and the backward pass one piece's derivative at a time.  F is H x W x C x K, as large as X's images; B may be None; C holds one label (1-based, 0 skips the image) per
-    image.  LSE, the logarithm of the sum of exponentials of an image's predictions (0 where the image is skipped), spares the
-    backward pass a pass over F; without it the backward pass computes it.  The flags and der_out=(DF, DB) as in vl_nnconv."""
+    classes, of which the forward pass keeps none and the backward pass one piece's derivative at a time.  F is H x W x C x K, as
+    large as X's images; B may be None; C holds one label (1-based, 0 skips the image) per image.  LSE, the logarithm of the sum of
+    exponentials of an image's predictions (0 where the image is skipped), spares the backward pass a pass over F; without it the
+    backward pass computes it.  The flags and der_out=(DF, DB) as in vl_nnconv."""
     return _hostpath.fcsoftmaxloss(ctx or default_context(), x, f, b, c, dzdy, lse, no_der_data, no_der_filters, no_der_biases, der_out)

@@ -27,6 +27,12 @@ def test_muon_on_rows_of_more_than_a_million_columns(gpu, rows, cols):
     muon._check(nn, [shape], seed=31)
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 2050, 3), (1, 1, 5003, 300), (7, 7, 512, 130), (1, 1, 130, 25088), (1, 1, 65600, 40)])
+def test_muon_on_rows_and_columns_of_some_thousands(gpu, shape):
+    """Sums of up to 65600 products, in chains of 64 of which at most 1025 follow one another: rounded by less than one sum of 4096 is bounded by in test_gpu_muon.py."""
+    muon._check(gpu[0], [shape], seed=35)
+
+
 LONG = 2 ** 32 + 5                          # what a 32-bit number has of it is 5
 
 
