@@ -597,9 +597,9 @@ pairs_kernel(const __grid_constant__ Batch<kMax> batch)
           return mbar_wait(smem_u32(&full[j % kStages]), (uint32_t)(j / kStages) & 1u) &&
                  (j < kAcc || mbar_wait(smem_u32(&empty[j % kAcc]), (uint32_t)(j / kAcc - 1) & 1u));
         };
-        int j = 0;
-        if (place < batch.work) dead = !ready(0);
-        for (int i = 0, w = item_at(batch, place, places, 0), after; !dead && w >= 0; ++i, w = after) {
+        int j = 0, w = item_at(batch, place, places, 0);
+        if (w >= 0) dead = !ready(0);                       // (where both products have few items there are places without any)
+        for (int i = 0, after; !dead && w >= 0; ++i, w = after) {
           after = item_at(batch, place, places, i + 1);
           Item const t = item_of(batch, w);
           Product const& p = batch.p[t.prod];

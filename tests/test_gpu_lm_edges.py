@@ -259,3 +259,21 @@ def test_fcloss_with_scales_of_data_and_filters_far_from_one(gpu, n, d, k):
         far = fcloss._check(nn, mat, x * s, f / s, b, c, (1, 1, d))
         for p, q in zip(base, far):
             assert (p[0] == q[0] * s).all() and (p[1] == q[1] / s).all() and (p[2] == q[2]).all()
+
+
+@pytest.mark.parametrize("n,d,k", [(155, 441, 4385), (639, 274, 5051), (415, 187, 9123), (2949, 1523, 1968)])
+def test_fcloss_whose_derivatives_have_fewer_tiles_than_there_are_places(gpu, n, d, k):
+    """Some places have no tile of either derivative, and nothing to wait for.  (The images' derivative is a long sum and is cut; the tiles go to the places by what they take.)"""
+    from matconvnet_b200 import capi
+    nn, mat, _ = gpu
+    ctx = capi.Context()
+    fcloss._check(nn, mat, *fcloss._inputs(n, (1, 1, d), k, 70), (1, 1, d), ctx=ctx)
+    assert ctx.device_status() == 0
+
+
+def test_muon_whose_products_have_fewer_tiles_than_there_are_places(gpu):
+    from matconvnet_b200 import capi
+    ctx = capi.Context()
+    muon._check(gpu[0], [(1, 1, 167, 18), (1, 1, 82, 249), (1, 1, 70, 5), (1, 1, 4, 42), (1, 1, 7, 460), (1, 1, 96, 3), (3, 3, 9, 187), (1, 1, 2, 15), (3, 3, 64, 563), (1, 1, 2674, 650),
+                         (1, 1, 6, 50), (1, 1, 83, 52), (1, 1, 20, 1), (3, 3, 16, 6), (1, 1, 2, 1), (1, 1, 43, 142), (1, 1, 312, 3), (3, 3, 2, 4)], ctx=ctx, seed=71)
+    assert ctx.device_status() == 0
